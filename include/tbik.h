@@ -267,6 +267,72 @@ int tbik_ar_status(tbik_ar_t comm, uint32_t out[8]);
  * multi-rank kernel are timed without a profiler.  No counterpart in the reference. */
 int tbik_ar_trace(tbik_ar_t comm, uint64_t* out, int max_blocks, int* blocks);
 
+/* ---- rows grouped by id: products by expert, low-rank adapters, the router --------------------------------
+ * A grouping is offsets[0 .. G]: rows offsets[g] .. offsets[g+1]-1 belong to group g.  It lives in device memory and is
+ * read by the kernels alone, so every value is clamped to [0, M] there and nothing is ever read or written outside
+ * the operands; offsets that decrease give unspecified values in the rows concerned.  Groups may be empty.  None of
+ * the entry points below has a counterpart in the reference, whose products are dense. */
+
+/* Stable grouping of M ids.  order[p] = index of the row that comes p-th when rows are sorted by id, rows of one id
+ * in their own order; position = its inverse; offsets has groups + 1 entries.  Rows whose id is outside
+ * [0, groups) belong to no group and come last, behind offsets[groups].  groups <= TBIK_MAX_GROUPS. */
+#define TBIK_MAX_GROUPS 1024
+int tbik_group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets,
+                    tbik_stream_t stream);
+
+/* Router: for each of T rows of logits [T, E] (row stride ld elements, any dtype code) the k largest values, largest
+ * first, equal values by lower index, NaN above everything (ids [T, k]); their softmax weights in fp32 (weights
+ * [T, k]): with `renormalize` over the k chosen, else over all E.  A row that holds nothing but -inf gets weights 0.
+ * Then the grouping of the T * k entries of ids by expert, as tbik_group_rows(ids, T * k, E, ...).
+ * 1 <= k <= min(E, TBIK_MAX_TOPK), E <= TBIK_MAX_GROUPS. */
+#define TBIK_MAX_TOPK 32
+int tbik_route_topk(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize, float* weights,
+                    int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, tbik_stream_t stream);
+
+/* Gradient of the weights of tbik_route_topk with respect to the logits: dlogits [T, E] (row stride ldd, the dtype of
+ * the logits), from the forward's weights and ids and dweights [T, k] (contiguous). */
+int tbik_route_topk_backward(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize,
+                             const float* weights, const int32_t* ids, const float* dweights, void* dlogits, int64_t ldd,
+                             tbik_stream_t stream);
+
+/* C[i, :] = A[i, :] * W[g]^T for the rows i of group g: the product of tbik_gemm with fp32 nodes, row for row the same
+ * bits, with the weight chosen by the row's group.
+ *   A [M, K] row stride lda; W [G, N, K] with group stride stride_w and, by w_layout, TBIK_W_K_CONTIGUOUS: rows of K
+ *   contiguous elements, row stride ldw; TBIK_W_N_CONTIGUOUS: element (n, k) at k * ldw + n (a transposed weight,
+ *   what the input gradient multiplies with).  C [M, N] row stride ldc.
+ *   dtype bf16 or fp16; out_dtype the same, or TBIK_DTYPE_FP32 for the unrounded sums.
+ *   leaf: width of the leaves of the reduction tree over K (a multiple of 64 that divides K); 0 = K is one leaf, and K
+ *   may then be any positive number.  At most 3 tree levels on 128-column tiles, 15 in all, as with tbik_gemm.
+ *   outside: what happens to rows of C that belong to no group: 0 = left as they were, 1 = set to zero.
+ * A and W 16-byte aligned, lda, ldw, stride_w multiples of 8.  max_ctas 0 = one per SM; no choice changes a bit. */
+#define TBIK_W_K_CONTIGUOUS 0
+#define TBIK_W_N_CONTIGUOUS 1
+int tbik_grouped_gemm(const void* A, const void* W, void* C, const int32_t* offsets, int64_t M, int N, int K, int groups,
+                      int64_t lda, int64_t ldw, int64_t stride_w, int64_t ldc, int w_layout, int dtype, int out_dtype,
+                      int leaf, int outside, int max_ctas, tbik_stream_t stream);
+
+/* dW[g] = sum over the rows i of group g, in order, of dC[i, :]^T A[i, :] (fp32 sums, rounded once): the weight
+ * gradient of tbik_grouped_gemm.  dC [M, N], A [M, K] with row strides lddc, lda (16-byte aligned, multiples of 8);
+ * dW [G, N, K] contiguous, of the operand type or fp32.  An empty group's gradient is zero. */
+int tbik_grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* offsets, int64_t M, int N, int K,
+                            int groups, int64_t lddc, int64_t lda, int dtype, int out_dtype, int max_ctas,
+                            tbik_stream_t stream);
+
+/* Low-rank adapters of many requests: for the rows t = order[p], p in group a,
+ *   h[t, :] = A[a] x[t, :]              fp32; K cut into leaves, leaf sums added in the fixed tree
+ *   out[t, :] = y[t, :] + scales[a] * B[a] h[t, :]   fp32, rounded once
+ * and out = y for the rows of no adapter.  x [T, K], y and out [T, N] (out may be y itself), A [adapters, R, K],
+ * B [adapters, N, R] contiguous, scales fp32.  `order` and `offsets` are those of tbik_group_rows on the rows' ids.
+ * The three forms: `x` and `y` given: both steps in one launch; `y`, `out` and B null: h is computed and stored
+ * (h [T, R] fp32; rows of no adapter get zeros); `x` and A null: h is read instead of computed.  A row-split layer uses
+ * the last two with the fixed-order sum of the ranks' h in between.
+ * leaf: 0 = K/8 rounded up to a multiple of 32; else a multiple of 32 with at most 8 leaves covering K.
+ * R a multiple of 8, at most TBIK_MAX_RANK; K, N multiples of 8; pointers 16-byte aligned, strides multiples of 8. */
+#define TBIK_MAX_RANK 128
+int tbik_adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, const void* A,
+                  const void* B, const float* scales, float* h, const int32_t* order, const int32_t* offsets, int64_t T,
+                  int N, int K, int R, int adapters, int dtype, int leaf, tbik_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,6 +15,8 @@ LIB_PATH = os.path.join(PKG_DIR, "libtbik_b200.so")
 TBIK_OK = 0
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
 NODE_INPUT, NODE_FP32, NODE_FP32_OUT_FP32 = 0, 1, 2
+W_K_CONTIGUOUS, W_N_CONTIGUOUS = 0, 1
+MAX_GROUPS, MAX_TOPK, MAX_RANK = 1024, 32, 128
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -51,6 +53,14 @@ _PROTOTYPES = {
     "tbik_ar_graph_meta": (_i32, [_vp, _vp, ctypes.POINTER(_i64)]),
     "tbik_ar_register_graph_buffers": (_i32, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(ctypes.POINTER(_i64))]),
     "tbik_ar_status": (_i32, [_vp, ctypes.POINTER(ctypes.c_uint32)]),
+    "tbik_group_rows": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp]),
+    "tbik_route_topk": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "tbik_route_topk_backward": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "tbik_grouped_gemm": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
+                                 _i32, _i32, _vp]),
+    "tbik_grouped_gemm_wgrad": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _i64, _i32, _i32, _i32, _vp]),
+    "tbik_adapters": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32,
+                             _i32, _vp]),
 }
 
 AR_CFG_SCRATCH_BYTES, AR_CFG_ONESHOT_MAX_BYTES, AR_CFG_MAX_BLOCKS, AR_CFG_WAIT_LIMIT_NS = 1, 2, 3, 4

@@ -148,4 +148,43 @@ int tbik_ar_register_graph_buffers(tbik_ar_t comm, const void* const* handles, c
 
 int tbik_ar_status(tbik_ar_t comm, uint32_t out[8]) { return tbik::ar_status(comm, out); }
 
+int tbik_group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets,
+                    tbik_stream_t stream) {
+  return tbik::group_rows(ids, M, groups, order, position, offsets, static_cast<cudaStream_t>(stream));
+}
+
+int tbik_route_topk(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize, float* weights,
+                    int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, tbik_stream_t stream) {
+  return tbik::route_topk(logits, ld, T, E, k, dtype, renormalize, weights, ids, order, position, offsets,
+                          static_cast<cudaStream_t>(stream));
+}
+
+int tbik_route_topk_backward(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize,
+                             const float* weights, const int32_t* ids, const float* dweights, void* dlogits, int64_t ldd,
+                             tbik_stream_t stream) {
+  return tbik::route_topk_backward(logits, ld, T, E, k, dtype, renormalize, weights, ids, dweights, dlogits, ldd,
+                                   static_cast<cudaStream_t>(stream));
+}
+
+int tbik_grouped_gemm(const void* A, const void* W, void* C, const int32_t* offsets, int64_t M, int N, int K, int groups,
+                      int64_t lda, int64_t ldw, int64_t stride_w, int64_t ldc, int w_layout, int dtype, int out_dtype,
+                      int leaf, int outside, int max_ctas, tbik_stream_t stream) {
+  return tbik::grouped_gemm(A, W, C, offsets, M, N, K, groups, lda, ldw, stride_w, ldc, w_layout, dtype, out_dtype, leaf,
+                            outside, max_ctas, static_cast<cudaStream_t>(stream));
+}
+
+int tbik_grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* offsets, int64_t M, int N, int K,
+                            int groups, int64_t lddc, int64_t lda, int dtype, int out_dtype, int max_ctas,
+                            tbik_stream_t stream) {
+  return tbik::grouped_gemm_wgrad(dC, A, dW, offsets, M, N, K, groups, lddc, lda, dtype, out_dtype, max_ctas,
+                                  static_cast<cudaStream_t>(stream));
+}
+
+int tbik_adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, const void* A,
+                  const void* B, const float* scales, float* h, const int32_t* order, const int32_t* offsets, int64_t T,
+                  int N, int K, int R, int adapters, int dtype, int leaf, tbik_stream_t stream) {
+  return tbik::adapters(x, ldx, y, ldy, out, ldo, A, B, scales, h, order, offsets, T, N, K, R, adapters, dtype, leaf,
+                        static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -49,4 +49,20 @@ int ar_graph_meta(tbik_ar_t h, void* handles_out, int64_t* offsets_out);
 int ar_register_graph_buffers(tbik_ar_t h, const void* const* handles, const int64_t* const* offsets);
 int ar_status(tbik_ar_t h, uint32_t out[8]);
 
+int group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets,
+               cudaStream_t stream);
+int route_topk(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize, float* weights,
+               int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, cudaStream_t stream);
+int route_topk_backward(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize,
+                        const float* weights, const int32_t* ids, const float* dweights, void* dlogits, int64_t ldd,
+                        cudaStream_t stream);
+int grouped_gemm(const void* A, const void* W, void* C, const int32_t* offsets, int64_t M, int N, int K, int groups,
+                 int64_t lda, int64_t ldw, int64_t stride_w, int64_t ldc, int w_layout, int dtype, int out_dtype, int leaf,
+                 int outside, int max_ctas, cudaStream_t stream);
+int grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* offsets, int64_t M, int N, int K, int groups,
+                       int64_t lddc, int64_t lda, int dtype, int out_dtype, int max_ctas, cudaStream_t stream);
+int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, const void* A, const void* B,
+             const float* scales, float* h, const int32_t* order, const int32_t* offsets, int64_t T, int N, int K, int R,
+             int adapters, int dtype, int leaf, cudaStream_t stream);
+
 }  // namespace tbik

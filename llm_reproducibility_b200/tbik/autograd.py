@@ -17,7 +17,10 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
+from .grouped_matmul import _grouped, _weight_gradient
+from .row_groups import Routing, RowGroups, _route, _route_backward
 from .tree_based_matmul import _LEAF, matmul_tp_persistent
 
 
@@ -65,3 +68,47 @@ def tree_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if bias is not None:
         y = y + bias
     return y.reshape(*lead, weight.shape[0])
+
+
+class _TreeGroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets, leaf):
+        ctx.save_for_backward(x, weight, offsets)
+        return _grouped(x, weight, offsets, leaf)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, offsets = ctx.saved_tensors
+        dx = _grouped(dy, weight.transpose(1, 2), offsets) if ctx.needs_input_grad[0] else None
+        dw = _weight_gradient(dy, x, offsets) if ctx.needs_input_grad[1] else None
+        return dx, dw, None, None
+
+
+def tree_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, leaf: Optional[int] = None) -> torch.Tensor:
+    """Differentiable `grouped_matmul_tp_persistent(x, weight, offsets, leaf=leaf)`: x [M, K] sorted by group, weight
+    [G, N, K].  dx sums over N in one fp32 accumulation (row i of dx depends on row i of dy only), dw over the group's
+    rows in their order; rows of no group are zero in y and in dx and add nothing to dw."""
+    return _TreeGroupedLinear.apply(x, weight, offsets, leaf)
+
+
+class _TreeRouteTopk(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, renormalize):
+        r = _route(logits, k, renormalize)
+        ctx.save_for_backward(logits, r.weights, r.ids)
+        ctx.renormalize = renormalize
+        ctx.mark_non_differentiable(r.ids, *r.groups)
+        return (r.weights, r.ids) + tuple(r.groups)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dweights, *_):
+        logits, weights, ids = ctx.saved_tensors
+        return _route_backward(logits, weights, ids, dweights, ctx.renormalize), None, None
+
+
+def tree_route_topk(logits: torch.Tensor, k: int, *, renormalize: bool = True) -> Routing:
+    """`route_topk` whose weights carry a gradient to the logits (through the softmax; the choice itself has none)."""
+    weights, ids, order, position, offsets = _TreeRouteTopk.apply(logits, k, renormalize)
+    return Routing(weights, ids, RowGroups(order, position, offsets))

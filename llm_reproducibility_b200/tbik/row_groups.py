@@ -1,0 +1,152 @@
+"""Rows grouped by an id, and the router that gives rows their ids.
+
+`group_rows(ids, G)` sorts the rows of a batch by expert or by adapter, stably; `route_topk(logits, k)` picks each
+token's k experts with their softmax weights and groups the (token, slot) rows that result.  Both leave everything on
+the device: nothing here waits for the GPU, so both can be captured in a CUDA graph.  There is no CPU path.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from .. import _lib
+from .tree_based_matmul import _raw_stream
+
+_LOGITS_CODE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
+
+
+class RowGroups(NamedTuple):
+    """Rows sorted by group (int32 tensors).
+
+    order[p] is the row that comes p-th, rows of one group in their own order; position is its inverse;
+    offsets[g] .. offsets[g + 1] are group g's places.  Rows of no group come last, behind offsets[-1]."""
+    order: torch.Tensor
+    position: torch.Tensor
+    offsets: torch.Tensor
+
+
+class Routing(NamedTuple):
+    weights: torch.Tensor  # [T, k] float32, largest first
+    ids: torch.Tensor      # [T, k] int32
+    groups: RowGroups      # of the T * k flat entries of ids: row i is token i // k
+
+
+def on_device(device: torch.device, call) -> int:
+    """Run `call(stream)` with `device` current; the kernels go to that device's current stream."""
+    if torch.cuda.current_device() == device.index:
+        return call(_raw_stream(device.index))
+    with torch.cuda.device(device):
+        return call(_raw_stream(device.index))
+
+
+def need_cuda(what: str, *tensors: torch.Tensor) -> torch.device:
+    """The tensors' one CUDA device."""
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} needs CUDA tensors (there is no CPU fallback)")
+        if t.device != tensors[0].device:
+            raise RuntimeError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+    return tensors[0].device
+
+
+def refuse_grad(what: str, instead: str, *tensors) -> None:
+    """A call that records no gradient must not swallow one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} records no gradient: {instead}")
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the spans of memory that two tensors step over meet."""
+    def span(t):
+        if t.numel() == 0:
+            return 0, 0
+        steps = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (steps + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _empty_groups(M: int, groups: int, device: torch.device) -> RowGroups:
+    # one allocation; the three parts start on 16-byte boundaries
+    pad = (M + 3) // 4 * 4
+    buf = torch.empty(2 * pad + groups + 1, dtype=torch.int32, device=device)
+    return RowGroups(buf[:M], buf[pad:pad + M], buf[2 * pad:])
+
+
+def _check_groups(num_groups: int) -> None:
+    if not 1 <= num_groups <= _lib.MAX_GROUPS:
+        raise ValueError(f"the number of groups must be in 1 .. {_lib.MAX_GROUPS}, got {num_groups}")
+
+
+def group_rows(ids: torch.Tensor, num_groups: int) -> RowGroups:
+    """Stable grouping of the rows whose ids are given (int32, flattened).  An id outside 0 .. num_groups - 1 (-1, say:
+    a row without adapter, a padded token) puts its row in no group."""
+    if ids.dtype != torch.int32:
+        raise ValueError(f"group_rows: ids must be int32, got {ids.dtype}")
+    _check_groups(num_groups)
+    if ids.numel() >= 1 << 31:
+        raise ValueError("group_rows: fewer than 2^31 rows")
+    dev = need_cuda("group_rows", ids)
+    ids = ids.contiguous()
+    g = _empty_groups(ids.numel(), num_groups, dev)
+    rc = on_device(dev, lambda stream: _lib.lib().tbik_group_rows(
+        ids.data_ptr(), ids.numel(), num_groups, g.order.data_ptr(), g.position.data_ptr(), g.offsets.data_ptr(), stream))
+    if rc != 0:
+        _lib.check(rc, "tbik_group_rows")
+    return g
+
+
+def _check_logits(logits: torch.Tensor, k: int) -> torch.Tensor:
+    if logits.dim() != 2:
+        raise ValueError(f"route_topk: logits must be [tokens, experts], got {tuple(logits.shape)}")
+    if logits.dtype not in _LOGITS_CODE:
+        raise NotImplementedError(f"route_topk: dtype {logits.dtype} is not supported")
+    T, E = logits.shape
+    if not 1 <= E <= _lib.MAX_GROUPS:
+        raise ValueError(f"route_topk: the number of experts must be in 1 .. {_lib.MAX_GROUPS}, got {E}")
+    if not 1 <= k <= min(E, _lib.MAX_TOPK):
+        raise ValueError(f"route_topk: k must be in 1 .. {min(E, _lib.MAX_TOPK)}, got {k}")
+    if T * k >= 1 << 31:
+        raise ValueError("route_topk: fewer than 2^31 (token, slot) rows")
+    need_cuda("route_topk", logits)
+    # rows may be strided or broadcast; the experts of a row must be contiguous
+    return logits if logits.stride(1) == 1 or E == 1 else logits.contiguous()
+
+
+def route_topk(logits: torch.Tensor, k: int, *, renormalize: bool = True) -> Routing:
+    """The k experts with the largest logits of each token, their weights, and the rows grouped by expert.
+
+    Equal logits: the lower index first.  `renormalize`: the weights are the softmax over the k chosen, else their
+    share of the softmax over all experts.  -inf masks an expert (weight 0); a token whose experts are all masked gets
+    weights 0.  `tbik.autograd.tree_route_topk` is the differentiable form."""
+    refuse_grad("route_topk", "use tbik.autograd.tree_route_topk", logits)
+    return _route(logits, k, renormalize)
+
+
+def _route(logits: torch.Tensor, k: int, renormalize: bool) -> Routing:
+    logits = _check_logits(logits, k)
+    T, E = logits.shape
+    dev = logits.device
+    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
+    ids = torch.empty((T, k), dtype=torch.int32, device=dev)
+    g = _empty_groups(T * k, E, dev)
+    rc = on_device(dev, lambda stream: _lib.lib().tbik_route_topk(
+        logits.data_ptr(), logits.stride(0), T, E, k, _LOGITS_CODE[logits.dtype], int(renormalize), weights.data_ptr(),
+        ids.data_ptr(), g.order.data_ptr(), g.position.data_ptr(), g.offsets.data_ptr(), stream))
+    if rc != 0:
+        _lib.check(rc, "tbik_route_topk")
+    return Routing(weights, ids, g)
+
+
+def _route_backward(logits, weights, ids, dweights, renormalize: bool) -> torch.Tensor:
+    logits = _check_logits(logits, ids.shape[1])
+    T, E = logits.shape
+    dweights = dweights.to(torch.float32).contiguous()
+    dlogits = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+    rc = on_device(logits.device, lambda stream: _lib.lib().tbik_route_topk_backward(
+        logits.data_ptr(), logits.stride(0), T, E, ids.shape[1], _LOGITS_CODE[logits.dtype], int(renormalize),
+        weights.data_ptr(), ids.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), E, stream))
+    if rc != 0:
+        _lib.check(rc, "tbik_route_topk_backward")
+    return dlogits

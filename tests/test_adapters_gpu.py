@@ -1,0 +1,202 @@
+"""Low-rank adapters of many requests against a 64-bit restatement: bit for bit on small integers (every sum exact in any
+order, h below 2^16), within a derived bound on normal deviates."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def make(shape, dtype, kind, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    if kind == "int":
+        return torch.randint(-1, 2, shape, generator=g, device="cuda").to(dtype)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def case(T, L, R, K, N, dtype, kind, seed=0, none=0.2):
+    g = torch.Generator().manual_seed(seed + T)
+    ids = torch.randint(0, L, (T,), generator=g)
+    ids[torch.rand(T, generator=g) < none] = -1
+    scales = torch.full((L,), 2.0) if kind == "int" else torch.rand(L, generator=g) + 0.5
+    return (make((T, N), dtype, kind, seed + 1), make((T, K), dtype, kind, seed + 2), make((L, R, K), dtype, kind, seed + 3, K ** -0.5),
+            make((L, N, R), dtype, kind, seed + 4, 0.3), ids.to(torch.int32).cuda(), scales.cuda())
+
+
+def ref(y, x, A, B, ids, scales):
+    """(out, h, bound of the fp32 work) in fp64."""
+    out, size = y.double(), torch.zeros(y.shape, dtype=torch.float64, device=y.device)
+    h = torch.zeros(y.shape[0], A.shape[1], dtype=torch.float64, device=y.device)
+    K, R = A.shape[2], A.shape[1]
+    for a in range(A.shape[0]):
+        rows = torch.nonzero(ids == a).flatten()
+        xa, Aa, Ba, s = x[rows].double(), A[a].double(), B[a].double(), float(scales[a])
+        h[rows] = xa @ Aa.t()
+        out[rows] += s * (h[rows] @ Ba.t())
+        # h: K terms, each addition off by at most 2^-23 of the magnitudes; the second product reads h in two parts of the
+        # operand type (off by 2^-16 of h at most) and adds R terms; scale and y: three more roundings
+        mag = (xa.abs() @ Aa.abs().t()) * K * 2.0 ** -23 + h[rows].abs() * (2.0 ** -16 + (2 * R + 3) * 2.0 ** -23)
+        size[rows] = s * (mag @ Ba.abs().t()) + y[rows].double().abs() * 2.0 ** -22
+    return out, h, size
+
+
+def check(got, want, kind):
+    out, _, size = want
+    if kind == "int":
+        assert torch.equal(got, out.to(got.dtype)), (got.double() - out).abs().max()
+    else:
+        tol = HALF[got.dtype] * out.abs() + size * (1 + HALF[got.dtype]) + 2.0 ** -25
+        bad = (got.double() - out).abs() > tol
+        assert not bad.any(), (int(bad.sum()), ((got.double() - out).abs() - tol).max())
+
+
+SHAPES = [(1, 1, 8, 8, 8), (1, 16, 16, 4096, 4096), (3, 2, 64, 40, 24), (16, 5, 16, 256, 264), (17, 1, 32, 1000, 72), (65, 64, 8, 520, 1032),
+          (96, 48, 16, 2056, 512), (130, 3, 128, 776, 136), (300, 7, 24, 12288, 256), (33, 1024, 40, 264, 520), (2000, 4, 32, 512, 1024),
+          (4500, 9, 72, 136, 328)]
+
+
+@pytest.mark.parametrize("kind", ["int", "normal"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,L,R,K,N", SHAPES)
+def test_lora_add(T, L, R, K, N, dtype, kind):
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    y, x, A, B, ids, s = case(T, L, R, K, N, dtype, kind)
+    want = ref(y, x, A, B, ids, s)
+    groups = group_rows(ids, L)
+    keep = y.clone()
+    got = lora_add(y, x, A, B, groups, s)
+    check(got, want, kind)
+    assert torch.equal(y, keep) and torch.equal(got[ids < 0], y[ids < 0])  # rows without adapter: their bits
+    assert lora_add(y, x, A, B, groups, s, out=y) is y
+    assert torch.equal(y, got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,L,R,K,N", [(5, 3, 16, 512, 64), (200, 6, 32, 4096, 264), (1, 1, 8, 264, 8), (1500, 2, 128, 1024, 200)])
+def test_shrink_and_expand_are_the_two_halves(T, L, R, K, N, dtype):
+    from llm_reproducibility_b200.tbik.adapters import lora_add, lora_expand_add, lora_shrink
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    y, x, A, B, ids, s = case(T, L, R, K, N, dtype, "normal")
+    groups = group_rows(ids, L)
+    h = lora_shrink(x, A, groups)
+    want = ref(y, x, A, B, ids, s)[1]
+    assert h.dtype == torch.float32 and (h[ids < 0] == 0).all()
+    bound = sum(torch.where((ids == a)[:, None], x.double().abs() @ A[a].double().abs().t(), 0.0) for a in range(L)) * (K + 8) * 2.0 ** -23
+    assert ((h.double() - want).abs() <= bound + 2.0 ** -40).all()
+    assert torch.equal(lora_expand_add(y, h, B, groups, s), lora_add(y, x, A, B, groups, s))
+
+
+@pytest.mark.parametrize("K,tp", [(4096, 2), (4096, 8), (768, 4), (256, 8)])
+def test_shards_of_k_add_up_to_the_unsharded_bits(K, tp):
+    from llm_reproducibility_b200.tbik.adapters import leaf_for_adapters, lora_shrink
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    _, x, A, _, ids, _ = case(77, 5, 16, K, 8, torch.bfloat16, "normal")
+    groups, leaf, ks = group_rows(ids, 5), leaf_for_adapters(K, tp), K // tp
+    parts = [lora_shrink(x[:, r * ks:(r + 1) * ks], A[:, :, r * ks:(r + 1) * ks], groups, leaf=leaf) for r in range(tp)]
+    while len(parts) > 1:
+        parts = [parts[i] + parts[i + 1] for i in range(0, len(parts), 2)]
+    assert torch.equal(parts[0], lora_shrink(x, A, groups))
+
+
+def test_a_row_has_the_same_bits_in_every_batch():
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    y, x, A, B, ids, s = case(3000, 6, 16, 1032, 328, torch.bfloat16, "normal", none=0.1)
+    full = lora_add(y, x, A, B, group_rows(ids, 6), s)
+    for rows in (slice(0, 1), slice(5, 9), slice(100, 140), slice(700, 1900)):
+        part = lora_add(y[rows], x[rows], A, B, group_rows(ids[rows], 6), s)
+        assert torch.equal(part, full[rows])
+
+
+def test_values_beyond_the_operand_types_range_in_h():
+    """h is held in 32 bits: it may pass fp16's largest number."""
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    T, K, N, R = 20, 1024, 64, 16
+    x, A = torch.full((T, K), 16.0, dtype=torch.float16, device="cuda"), torch.full((1, R, K), 16.0, dtype=torch.float16, device="cuda")
+    B = torch.full((1, N, R), 2.0 ** -14, dtype=torch.float16, device="cuda")
+    A[:, 1] = -16.0
+    B[:, :, 3] = 0.0
+    y = torch.ones((T, N), dtype=torch.float16, device="cuda")
+    got = lora_add(y, x, A, B, group_rows(torch.zeros(T, dtype=torch.int32, device="cuda"), 1), torch.ones(1, device="cuda"))
+    assert torch.equal(got, torch.full_like(got, 1 + (R - 3) * 2.0 ** 18 * 2.0 ** -14))
+
+
+def test_infinities_and_nan_stay_in_their_rows():
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    for bad in (float("nan"), float("inf")):
+        y, x, A, B, ids, s = case(70, 3, 16, 512, 128, torch.bfloat16, "int", none=0.0)
+        want = ref(y, x, A, B, ids, s)[0].to(torch.bfloat16)
+        x[9] = bad
+        A[2, 5], B[2, 7] = bad, bad
+        got = lora_add(y, x, A, B, group_rows(ids, 3), s)
+        fine = [t for t in range(70) if t != 9 and int(ids[t]) != 2]
+        assert torch.equal(got[fine], want[fine]) and not got[9].isfinite().all()
+
+
+def test_no_adapters_at_all_and_no_rows():
+    from llm_reproducibility_b200.tbik.adapters import lora_add, lora_shrink
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    y, x, A, B, ids, s = case(50, 4, 16, 64, 72, torch.bfloat16, "normal", none=1.1)
+    groups = group_rows(ids, 4)
+    assert torch.equal(lora_add(y, x, A, B, groups, s), y)
+    assert (lora_shrink(x, A, groups) == 0).all()
+    empty = group_rows(ids[:0], 4)
+    assert lora_add(y[:0], x[:0], A, B, empty, s).shape == (0, 72)
+
+
+def test_strides_and_neighbours():
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    T, K, N = 37, 64, 72
+    y, x, A, B, ids, s = case(T, 3, 16, K, N, torch.bfloat16, "int")
+    groups, want = group_rows(ids, 3), ref(y, x, A, B, ids, s)[0].to(torch.bfloat16)
+    wx = torch.zeros(T, 3 * K + 3, dtype=torch.bfloat16, device="cuda")
+    for view in (wx[:, :K], wx[:, 1:K + 1], wx[:, ::3][:, :K]):
+        view.copy_(x)
+        assert torch.equal(lora_add(y, view, A, B, groups, s), want)
+    assert torch.equal(lora_add(y, x, A.transpose(1, 2).contiguous().transpose(1, 2), B.transpose(1, 2).contiguous().transpose(1, 2), groups, s), want)
+    buf = torch.full((T + 2, N + 16), 9.0, dtype=torch.bfloat16, device="cuda")
+    lora_add(y, x, A, B, groups, s, out=buf[1:T + 1, 8:8 + N])
+    assert torch.equal(buf[1:T + 1, 8:8 + N], want)
+    buf[1:T + 1, 8:8 + N] = 9.0
+    assert (buf == 9.0).all()
+    # one row for all: a broadcast x
+    same = x[:1].expand(T, K)
+    assert torch.equal(lora_add(y, same, A, B, groups, s), ref(y, same, A, B, ids, s)[0].to(torch.bfloat16))
+
+
+def test_bad_tables_touch_nothing_outside():
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import RowGroups
+    T, K, N = 40, 64, 64
+    y, x, A, B, ids, s = case(T, 3, 16, K, N, torch.bfloat16, "int")
+    buf = torch.full((T + 2, N), 9.0, dtype=torch.bfloat16, device="cuda")
+    for order, offsets in (([2 ** 31 - 1] * T, [0, 10, 20, 40]), ([-1] * T, [0, 10, 20, 40]), (list(range(T)), [0, 1000, 2000, 2 ** 31 - 1]),
+                           (list(range(T)), [-7, 30, 10, 50]), (list(range(T)), [2 ** 31 - 1, 0, 0, 0])):
+        g = RowGroups(torch.tensor(order, dtype=torch.int32, device="cuda"), None, torch.tensor(offsets, dtype=torch.int32, device="cuda"))
+        lora_add(y, x, A, B, g, s, out=buf[1:T + 1])
+        assert (buf[0] == 9).all() and (buf[-1] == 9).all()
+
+
+def test_streams_and_a_graph_that_follows_new_ids():
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    y, x, A, B, ids, s = case(64, 5, 16, 512, 256, torch.bfloat16, "int")
+    lora_add(y, x, A, B, group_rows(ids, 5), s)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = lora_add(y, x, A, B, group_rows(ids, 5), s)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, ref(y, x, A, B, ids, s)[0].to(torch.bfloat16))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lora_add(y, x, A, B, group_rows(ids, 5), s)
+    for shift in (1, 2):
+        ids.copy_((torch.arange(64, device="cuda") * shift) % 7 - 1)
+        graph.replay()
+        assert torch.equal(out, ref(y, x, A, B, torch.where(ids < 5, ids, -1), s)[0].to(torch.bfloat16))

@@ -1,0 +1,174 @@
+"""What the grouped operators refuse, through the Python entry points and through the C ABI, without a GPU: every check
+stands before the first launch."""
+import pytest
+import torch
+
+BF16 = torch.bfloat16
+
+
+def off(*values, dtype=torch.int32):
+    return torch.tensor(values, dtype=dtype)
+
+
+def test_grouped_matmul_refuses():
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent as f
+    A, W = torch.zeros(4, 128, dtype=BF16), torch.zeros(2, 8, 128, dtype=BF16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        f(A, W, off(0, 2, 4))
+    with pytest.raises(ValueError, match="A must be"):
+        f(A, W[0], off(0, 2, 4))
+    with pytest.raises(ValueError, match="A must be"):
+        f(A[:, :64], W, off(0, 2, 4))
+    with pytest.raises(NotImplementedError):
+        f(A.float(), W.float(), off(0, 2, 4))
+    with pytest.raises(ValueError, match="operands"):
+        f(A, W.half(), off(0, 2, 4))
+    with pytest.raises(ValueError, match="int32"):
+        f(A, W, off(0, 2, 4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="3 entries"):
+        f(A, W, off(0, 4))
+    for leaf in (0, 32, 96, 256, -64):
+        with pytest.raises(ValueError, match="leaf"):
+            f(A, W, off(0, 2, 4), leaf=leaf)
+    with pytest.raises(ValueError, match="out_dtype"):
+        f(A, W, off(0, 2, 4), out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="groups"):
+        f(A, torch.zeros(1025, 8, 128, dtype=BF16), torch.zeros(1026, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="tree_grouped_linear"):
+        f(A.clone().requires_grad_(True), W, off(0, 2, 4))
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        f(A.clone().requires_grad_(True), W, off(0, 2, 4))
+
+
+def test_weight_gradient_refuses():
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_weight_gradient as f
+    A, D = torch.zeros(4, 16, dtype=BF16), torch.zeros(4, 8, dtype=BF16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        f(D, A, off(0, 2, 4))
+    with pytest.raises(ValueError, match="dC must be"):
+        f(D[:3], A, off(0, 2, 4))
+    with pytest.raises(ValueError, match="groups"):
+        f(D, A, off(0))
+    with pytest.raises(ValueError, match="int32"):
+        f(D, A, off(0, 4, dtype=torch.int64))
+    with pytest.raises(ValueError, match="operands"):
+        f(D.half(), A, off(0, 4))
+
+
+def test_router_refuses():
+    from llm_reproducibility_b200.tbik.autograd import tree_route_topk
+    from llm_reproducibility_b200.tbik.row_groups import group_rows, route_topk
+    x = torch.zeros(4, 8)
+    for f in (route_topk, tree_route_topk):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            f(x, 2)
+        with pytest.raises(ValueError, match="k must"):
+            f(x, 9)
+        with pytest.raises(ValueError, match="k must"):
+            f(x, 0)
+        with pytest.raises(ValueError, match="tokens, experts"):
+            f(x[0], 2)
+        with pytest.raises(NotImplementedError):
+            f(x.double(), 2)
+        with pytest.raises(ValueError, match="experts must"):
+            f(torch.zeros(2, 1025), 2)
+        with pytest.raises(ValueError, match="k must"):
+            f(torch.zeros(2, 100), 33)
+    with pytest.raises(RuntimeError, match="tree_route_topk"):
+        route_topk(x.clone().requires_grad_(True), 2)
+    with pytest.raises(ValueError, match="int32"):
+        group_rows(torch.zeros(4, dtype=torch.int64), 2)
+    for n in (0, -1, 1025):
+        with pytest.raises(ValueError, match="groups"):
+            group_rows(torch.zeros(4, dtype=torch.int32), n)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        group_rows(torch.zeros(4, dtype=torch.int32), 2)
+
+
+def test_adapters_refuse():
+    from llm_reproducibility_b200.tbik.adapters import leaf_for_adapters, lora_add, lora_expand_add, lora_shrink
+    from llm_reproducibility_b200.tbik.row_groups import RowGroups
+    y, x = torch.zeros(4, 24, dtype=BF16), torch.zeros(4, 64, dtype=BF16)
+    A, B, s = torch.zeros(3, 8, 64, dtype=BF16), torch.zeros(3, 24, 8, dtype=BF16), torch.ones(3)
+    g = RowGroups(torch.arange(4, dtype=torch.int32), torch.arange(4, dtype=torch.int32), off(0, 1, 2, 4))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        lora_add(y, x, A, B, g, s)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        lora_shrink(x, A, g)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        lora_expand_add(y, torch.zeros(4, 8), B, g, s)
+    for bad in ((y, x, A[:2], B, g, s), (y, x[:, :32], A, B, g, s), (y[:3], x, A, B, g, s), (y[:, :16], x, A, B, g, s)):
+        with pytest.raises(ValueError, match="lora_add: y"):
+            lora_add(*bad)
+    with pytest.raises(ValueError, match="scales"):
+        lora_add(y, x, A, B, g, s[:2])
+    with pytest.raises(ValueError, match="scales"):
+        lora_add(y, x, A, B, g, s.half())
+    with pytest.raises(ValueError, match="offsets"):
+        lora_add(y, x, A, B, g._replace(offsets=off(0, 4)), s)
+    with pytest.raises(ValueError, match="order"):
+        lora_add(y, x, A, B, g._replace(order=g.order.long()), s)
+    with pytest.raises(ValueError, match="rank"):
+        lora_shrink(x, torch.zeros(3, 12, 64, dtype=BF16), g)
+    with pytest.raises(ValueError, match="rank"):
+        lora_shrink(x, torch.zeros(3, 136, 64, dtype=BF16), g)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        lora_shrink(x[:, :60], A[:, :, :60], g)
+    with pytest.raises(NotImplementedError):
+        lora_shrink(x.float(), A.float(), g)
+    for leaf in (16, 40, -32, 0):
+        with pytest.raises(ValueError, match="leaf"):
+            lora_shrink(x, A, g, leaf=leaf)
+    with pytest.raises(ValueError, match="h must"):
+        lora_expand_add(y, torch.zeros(4, 8, dtype=BF16), B, g, s)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        lora_add(y, x.clone().requires_grad_(True), A, B, g, s)
+    assert leaf_for_adapters(4096) == 512 and leaf_for_adapters(100, 1) == 32
+    with pytest.raises(ValueError):
+        leaf_for_adapters(100, 2)
+    with pytest.raises(ValueError):
+        leaf_for_adapters(4096, 3)
+
+
+def test_c_abi_refuses_before_any_launch():
+    from llm_reproducibility_b200 import _lib
+    L = _lib.lib()
+    p = 1 << 20  # a 16-byte aligned number that no check dereferences
+    ok = [p, p, p, p, 4, 8, 128, 2, 128, 128, 1024, 8, 0, 0, 0, 0, 0, 0, None]
+
+    def gemm(**at):
+        args = list(ok)
+        for i, v in at.items():
+            args[int(i[1:])] = v
+        return L.tbik_grouped_gemm(*args)
+
+    assert gemm(_4=0) == 0 and gemm(_5=0) == 0                         # nothing to do
+    assert gemm(_0=None) == -1 and gemm(_3=None) == -1 and gemm(_12=2) == -1
+    assert gemm(_6=0) == -2 and gemm(_7=0) == -2 and gemm(_7=1025) == -2 and gemm(_4=1 << 31) == -2 and gemm(_15=48) == -2
+    assert gemm(_8=120) == -2 and gemm(_9=64) == -2 and gemm(_10=512) == -2 and gemm(_11=4) == -2
+    assert gemm(_13=2) == -3 and gemm(_14=1) == -3
+    assert gemm(_0=p + 2) == -4 and gemm(_1=p + 8) == -4 and gemm(_8=129) == -4
+    assert "tbik_grouped_gemm" in _lib.last_error()
+    assert L.tbik_grouped_gemm_wgrad(p, p, None, p, 4, 8, 16, 2, 8, 16, 0, 0, 0, None) == -1
+    assert L.tbik_grouped_gemm_wgrad(p, p, p, p, 4, 8, 16, 2, 4, 16, 0, 0, 0, None) == -2
+    assert L.tbik_grouped_gemm_wgrad(p, p, p, p, 4, 8, 16, 2, 8, 17, 0, 0, 0, None) == -4
+    assert L.tbik_grouped_gemm_wgrad(p, p, p, p, 4, 8, 16, 2, 8, 16, 0, 1, 0, None) == -3
+    assert L.tbik_group_rows(p, 4, 0, p, p, p, None) == -2 and L.tbik_group_rows(None, 4, 2, p, p, p, None) == -1
+    assert L.tbik_group_rows(p, 4, 2, p, p, None, None) == -1 and L.tbik_group_rows(p, -1, 2, p, p, p, None) == -2
+    assert L.tbik_route_topk(p, 8, 4, 8, 9, 0, 1, p, p, p, p, p, None) == -2
+    assert L.tbik_route_topk(p, 8, 4, 8, 2, 7, 1, p, p, p, p, p, None) == -3
+    assert L.tbik_route_topk(None, 8, 4, 8, 2, 0, 1, p, p, p, p, p, None) == -1
+    assert L.tbik_route_topk_backward(p, 8, 4, 8, 2, 0, 1, p, p, None, p, 8, None) == -1
+    assert L.tbik_route_topk_backward(p, 8, 0, 8, 2, 0, 1, None, None, None, None, 8, None) == 0
+    base = [p, 64, p, 24, p, 24, p, p, p, None, p, p, 4, 24, 64, 8, 3, 0, 0, None]
+
+    def lora(**at):
+        args = list(base)
+        for i, v in at.items():
+            args[int(i[1:])] = v
+        return L.tbik_adapters(*args)
+
+    assert lora(_12=0) == 0
+    assert lora(_0=None) == -1 and lora(_2=None) == -1 and lora(_6=None) == -1 and lora(_10=None) == -1 and lora(_0=None, _2=None) == -1
+    assert lora(_13=20) == -2 and lora(_14=12) == -2 and lora(_15=12) == -2 and lora(_15=136) == -2 and lora(_16=0) == -2 and lora(_18=40) == -2
+    assert lora(_1=32) == -2 and lora(_3=16) == -2 and lora(_17=2) == -3 and lora(_2=p + 4) == -4 and lora(_1=65) == -4
