@@ -1,145 +1,693 @@
-// Products of rows grouped by expert, ragged sizes: C[i] = A[i] W[g(i)]^T and the weight gradient.
+// Products of rows grouped by expert for sm_100a, ragged sizes:
 //
-// First form: 64x64 tiles of fp32 fused multiply-adds from shared memory, one block per column tile and group.  Right for
-// every layout, type and size; bound by the fp32 pipe.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+//   forward   C[i, n] = sum_k A[i, k] W[g, n, k]        offsets[g] <= i < offsets[g+1]
+//   gradient  dW[g, n, k] = sum_i dC[i, n] A[i, k]      over the rows i of group g
+//
+// (the gradient with respect to A is the forward product with the transposed view of W).  All sums are tcgen05.mma
+// chains in fp32 tensor-memory accumulators, K in steps of 16 from the first to the last, rounded once.  With leaves
+// every leaf is a chain of its own and the leaves' sums are joined by fp32 adds in the tree of the dense kernel (level 0
+// F leaves left to right, binary above), the stack in spare tensor-memory columns.  Neither depends on the group's size,
+// the tile or the grid, so a row's bits are those of the dense kernel on the group's rows alone.
+//
+// What is ragged is only which tiles exist: every CTA builds the table of the groups' tiles in shared memory when it
+// starts (offsets are read on the device), then the persistent loop of each role finds its tile's group by binary search.
+// A tile's rows end with the group: rows beyond it are multiplied (they are the next group's) and not stored.
+//
+//   warp 0      TMA producer   128-byte swizzled boxes of 64 reduction steps; of A only 16, 32, 64 or 128 rows, as many as the
+//                              tile has rows, so a decode step's tiles of a few rows read W and little else
+//   warp 1      UMMA issuer    two accumulators: tile (or leaf) i+1 runs while i drains
+//   warp 2      tensor memory
+//   warps 4-11  epilogue       tcgen05.ld, tree, rounding, rows regrouped through 2 KiB of shared memory per warp so that a
+//                              store instruction writes whole 64-byte pieces of rows
+//
+// The operands' contiguous index is the reduction index (K-major) or the other one (MN-major); tensor memory does not
+// care, so the transposed weight and both operands of the weight gradient are read as they lie.  The weight gradient
+// reduces over a group's rows: its last step ends inside a box, and the rows of the next group that the box brought along
+// are overwritten with zeros in shared memory before the multiply, in both operands (a NaN there must not meet a zero).
+//
+// PAIR: a cluster of two CTAs per 256-row tile (cta_group::2), each with its own 128 rows and half of the columns' operand.
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
+#include "ptx_sm100a.cuh"
 #include "tbik_internal.h"
 
 namespace tbik {
 namespace {
 
-constexpr int TM = 64, TN = 64, TK = 16;
-constexpr int kMaxLevels = 16;
+constexpr int BM = 128;  // rows of a tile per CTA
+constexpr int BK = 64;   // reduction steps per stage
+constexpr int UMMA_K = 16;
+constexpr int NUM_THREADS = 384;
+constexpr int EPI_WARP0 = 4;
+constexpr int NUM_EPI_WARPS = 8;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr int CHUNK = 32;  // accumulator columns per tcgen05.ld
+constexpr uint64_t WAIT_LIMIT_NS = 2000000000ull;
+constexpr uint32_t A_STAGE_BYTES = BM * BK * 2;
+constexpr uint32_t STAGING_BYTES_PER_WARP = 2048;
+constexpr int GROUP_M = 8;  // row tiles that share a sweep over the columns
 
-__device__ __forceinline__ float f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+enum Mode { kForwardK = 0, kForwardN = 1, kWeightGrad = 2 };
 
-struct Params {
-  const void *A, *W;
-  void* C;
-  const int32_t* offsets;
-  int64_t M;
-  int N, K, groups;
-  int64_t lda, ldw, stride_w, ldc;
-  int w_n_contiguous, leaf, T, F, L, outside;
+__device__ uint32_t g_grouped_status[4];  // [0] a bounded wait ran out, [1] block, [2] role
+
+struct Maps {
+  CUtensorMap a[4];  // forward: A with boxes of 16, 32, 64, 128 rows; weight gradient: a[0] = dC
+  CUtensorMap b;     // W; weight gradient: A
 };
 
-// The group's rows, clamped to the operands whatever the table holds.
-__device__ __forceinline__ void group_rows_of(const int32_t* offsets, int g, int64_t M, int64_t& r0, int64_t& r1) {
-  r0 = min(max(static_cast<int64_t>(offsets[g]), int64_t(0)), M);
-  r1 = min(max(static_cast<int64_t>(offsets[g + 1]), r0), M);
-}
+struct Params {
+  void* C;
+  const int32_t* offsets;
+  int64_t ldc;
+  int M, groups;
+  int rows, cols, red;  // forward: -, N, K; weight gradient: N, K, -
+  int kblocks_per_leaf, T, F, L;
+  int tiles_c;          // column tiles
+  int tiles_r;          // weight gradient: row tiles
+  int half;             // 16-bit type of the operands: 1 bf16, 0 fp16 (the UMMA format code)
+  int out32;            // C is fp32
+  int zero_outside;     // forward: rows of no group are set to zero
+};
 
-template <typename T, typename O>
-__global__ void __launch_bounds__(256) grouped_kernel(const Params p) {
-  __shared__ float sa[TK][TM + 4], sw[TK][TN + 4];
-  const int g = blockIdx.y, n0 = blockIdx.x * TN;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  O* C = static_cast<O*>(p.C);
-  if (g == p.groups) {  // rows of no group
-    const int64_t lo = min(max(static_cast<int64_t>(p.offsets[0]), int64_t(0)), p.M);
-    const int64_t hi = min(max(static_cast<int64_t>(p.offsets[p.groups]), int64_t(0)), p.M);
-    for (int64_t i = threadIdx.x; i < p.M * TN; i += 256) {
-      const int64_t r = i / TN;
-      const int n = n0 + static_cast<int>(i % TN);
-      if ((r < lo || r >= hi) && n < p.N) put(C + r * p.ldc + n, 0.0f);
+template <int BN, int STAGES_, bool PAIR, int MODE>
+struct Cfg {
+  static constexpr int STAGES = STAGES_;
+  static constexpr int TILE_M = PAIR ? 2 * BM : BM;
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // columns' operand of this CTA
+  static constexpr bool B_MN = MODE != kForwardK;
+  static constexpr uint32_t B_STAGE_BYTES = (B_MN && B_ROWS < 64 ? 64 : B_ROWS) * BK * 2;
+  static constexpr uint32_t STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
+  static constexpr int EPI_HALVES = BN >= 64 ? 2 : 1;
+  static constexpr int CW = BN / EPI_HALVES;  // columns per epilogue warp
+  static constexpr int NCH = CW / CHUNK;
+  static constexpr uint32_t OFF_STAGING = STAGES * STAGE_BYTES;
+  static constexpr uint32_t OFF_BARS = OFF_STAGING + NUM_EPI_WARPS * STAGING_BYTES_PER_WARP;
+  static constexpr uint32_t OFF_FULL = OFF_BARS;
+  static constexpr uint32_t OFF_EMPTY = OFF_FULL + 8 * STAGES;
+  static constexpr uint32_t OFF_TFULL = OFF_EMPTY + 8 * STAGES;
+  static constexpr uint32_t OFF_TEMPTY = OFF_TFULL + 16;
+  static constexpr uint32_t OFF_TMEM_PTR = OFF_TEMPTY + 16;
+  static constexpr uint32_t OFF_ABORT = OFF_TMEM_PTR + 4;
+  static constexpr uint32_t OFF_TABLE = OFF_ABORT + 8;  // first[G], last[G], tiles before[G + 1]
+  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + 4 * (3 * groups + 1) + 1024; }
+  static_assert(smem_bytes(TBIK_MAX_GROUPS) <= 232448, "shared memory budget");
+};
+
+struct Tile {
+  int g, r0, r1;   // group; its rows (forward: rows of this tile; weight gradient: the rows summed over)
+  int row, col;    // first row and column of the result
+};
+
+template <int BN, int STAGES, bool PAIR, int MODE, bool TREE>
+__global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_constant__ Maps maps, const Params p) {
+  using C_ = Cfg<BN, STAGES, PAIR, MODE>;
+  constexpr uint32_t STAGE_BYTES = C_::STAGE_BYTES;
+  constexpr int TILE_M = C_::TILE_M;
+  constexpr bool WG = MODE == kWeightGrad;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t cta_rank = PAIR ? cluster_ctarank() : 0u;
+  const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int num_units = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  const bool leader = cta_rank == 0u;
+
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem_gen + C_::OFF_ABORT);
+  volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem_gen + C_::OFF_TMEM_PTR);
+  auto full_bar = [&](int s) { return smem_base + C_::OFF_FULL + 8u * s; };
+  auto empty_bar = [&](int s) { return smem_base + C_::OFF_EMPTY + 8u * s; };
+  auto tfull_bar = [&](int a) { return smem_base + C_::OFF_TFULL + 8u * a; };
+  auto tempty_bar = [&](int a) { return smem_base + C_::OFF_TEMPTY + 8u * a; };
+  int* first = reinterpret_cast<int*>(smem_gen + C_::OFF_TABLE);
+  int* last = first + p.groups;
+  int* before = last + p.groups;  // tiles of the groups before
+
+  if constexpr (PAIR) cluster_sync_all();
+  if (threadIdx.x == 0) {
+    *abort_flag = 0u;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), (PAIR && leader) ? 2 : 1);  // pair, leader: its own producer and the partner's relay
+      mbar_init(empty_bar(s), 1);
     }
-    return;
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), PAIR ? 2 * NUM_EPI_WARPS : NUM_EPI_WARPS);
+    }
+    fence_mbar_init();
   }
-  int64_t r0, r1;
-  group_rows_of(p.offsets, g, p.M, r0, r1);
-  const T* A = static_cast<const T*>(p.A);
-  const T* W = static_cast<const T*>(p.W) + static_cast<int64_t>(g) * p.stride_w;
-  for (int64_t m0 = r0; m0 < r1; m0 += TM) {
-    float level[kMaxLevels][4][4], node[4][4] = {};
-    int in_group = 0;
-    unsigned closed = 0;
-    for (int l = 0; l < p.T; ++l) {
-      float acc[4][4] = {};
-      const int k1 = min((l + 1) * p.leaf, p.K);
-      for (int k0 = l * p.leaf; k0 < k1; k0 += TK) {
-        for (int i = threadIdx.x; i < TM * TK; i += 256) {
-          const int m = i / TK, k = i % TK;
-          sa[k][m] = (m0 + m < r1 && k0 + k < k1) ? f32(A[(m0 + m) * p.lda + k0 + k]) : 0.0f;
-          sw[k][m] = (n0 + m < p.N && k0 + k < k1)
-                         ? f32(p.w_n_contiguous ? W[static_cast<int64_t>(k0 + k) * p.ldw + n0 + m]
-                                                : W[static_cast<int64_t>(n0 + m) * p.ldw + k0 + k]) : 0.0f;
-        }
-        __syncthreads();
-        for (int k = 0; k < TK; ++k)
-          for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty * 4 + i], sw[k][tx * 4 + j], acc[i][j]);
-        __syncthreads();
+  if (warp == 2) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_base + C_::OFF_TMEM_PTR, TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_base + C_::OFF_TMEM_PTR, TMEM_COLS);
+      tmem_relinquish();
+    }
+  }
+  for (int g = threadIdx.x; g < p.groups; g += NUM_THREADS) last[g] = min(max(p.offsets[g + 1], 0), p.M);
+  __syncthreads();
+  if (warp == 0) {
+    // Running maximum: whatever the table holds, the groups' rows are inside the operands and disjoint.
+    int run = 0, end = min(max(p.offsets[0], 0), p.M);
+    for (int g0 = 0; g0 < p.groups; g0 += 32) {
+      const int g = g0 + lane;
+      int hi = g < p.groups ? max(last[g], end) : end;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xFFFFFFFFu, hi, o);
+        if (lane >= o) hi = max(hi, v);
       }
-      // level 0: F leaves left to right; above it a binary tree
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) node[i][j] = in_group ? node[i][j] + acc[i][j] : acc[i][j];
-      if (++in_group < p.F) continue;
-      in_group = 0;
-      int lvl = 0;
-      for (unsigned c = closed++; c & 1u; c >>= 1, ++lvl)
-        for (int i = 0; i < 4; ++i)
-          for (int j = 0; j < 4; ++j) node[i][j] = level[lvl][i][j] + node[i][j];
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) level[lvl][i][j] = node[i][j];
+      int lo = __shfl_up_sync(0xFFFFFFFFu, hi, 1);
+      if (lane == 0) lo = end;
+      const int t = g < p.groups ? (WG ? p.tiles_r * p.tiles_c : (hi - lo + TILE_M - 1) / TILE_M * p.tiles_c) : 0;
+      int s = t;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xFFFFFFFFu, s, o);
+        if (lane >= o) s += v;
+      }
+      if (g < p.groups) {
+        first[g] = lo;
+        last[g] = hi;
+        before[g] = run + s - t;
+      }
+      run += __shfl_sync(0xFFFFFFFFu, s, 31);
+      end = __shfl_sync(0xFFFFFFFFu, hi, 31);
     }
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j)
-        if (m0 + ty * 4 + i < r1 && n0 + tx * 4 + j < p.N) put(C + (m0 + ty * 4 + i) * p.ldc + n0 + tx * 4 + j, node[i][j]);
+    if (lane == 0) before[p.groups] = run;
+  }
+  tc_fence_before_sync();
+  if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_ptr_smem;
+  const int num_tiles = before[p.groups];
+
+  auto tile_at = [&](int tile) {
+    int lo = 0, hi = p.groups;  // before[lo] <= tile < before[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= tile) lo = mid; else hi = mid;
+    }
+    const int local = tile - before[lo];
+    const int g0 = first[lo], g1 = last[lo];
+    const int tiles_r = WG ? p.tiles_r : (g1 - g0 + TILE_M - 1) / TILE_M;
+    // GROUP_M row tiles share a sweep over the columns
+    const int block = local / (GROUP_M * p.tiles_c);
+    const int in = local - block * GROUP_M * p.tiles_c;
+    const int height = min(tiles_r - block * GROUP_M, GROUP_M);
+    const int tr = block * GROUP_M + in % height, tc = in / height;
+    Tile t;
+    t.g = lo;
+    t.col = tc * BN;
+    if constexpr (WG) {
+      t.r0 = g0;
+      t.r1 = g1;
+      t.row = tr * TILE_M;
+    } else {
+      t.r0 = g0 + tr * TILE_M;
+      t.r1 = min(t.r0 + TILE_M, g1);
+      t.row = t.r0;
+    }
+    return t;
+  };
+  // stages of one accumulator chain: a leaf, or the group's rows
+  auto chain_blocks = [&](const Tile& t) { return WG ? (t.r1 - t.r0 + BK - 1) / BK : p.kblocks_per_leaf; };
+
+  int role_failed = 0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint64_t policy = l2_policy(0);
+      for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
+        const Tile t = tile_at(tile);
+        const int blocks = chain_blocks(t) * (WG ? 1 : p.T);
+        const int r = static_cast<int>(cta_rank);
+        const int have = WG ? BM : min(max(t.r1 - t.r0 - r * BM, 1), BM);
+        const int box = have <= 16 ? 0 : have <= 32 ? 1 : have <= 64 ? 2 : 3;
+        const CUtensorMap* ta = &maps.a[WG ? 0 : box];
+        const uint32_t bytes = (WG ? A_STAGE_BYTES : (16u << box) * BK * 2) + C_::B_STAGE_BYTES;
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
+            ok = false;
+            role_failed = 1;
+            break;
+          }
+          const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + A_STAGE_BYTES, bar = full_bar(stage);
+          mbar_arrive_expect_tx(bar, bytes);
+          const int x = kb * BK;
+          if constexpr (WG) {
+#pragma unroll
+            for (int u = 0; u < BM / 64; ++u) tma_load_2d_hint(sa + u * 8192, ta, t.row + r * BM + u * 64, t.r0 + x, bar, policy);
+#pragma unroll
+            for (int u = 0; u < C_::B_ROWS / 64; ++u)
+              tma_load_2d_hint(sb + u * 8192, &maps.b, t.col + r * C_::B_ROWS + u * 64, t.r0 + x, bar, policy);
+          } else {
+            tma_load_2d_hint(sa, ta, x, t.r0 + r * BM, bar, policy);
+            if constexpr (C_::B_MN) {
+#pragma unroll
+              for (int u = 0; u < (C_::B_ROWS + 63) / 64; ++u)
+                tma_load_3d_hint(sb + u * 8192, &maps.b, t.col + r * C_::B_ROWS + u * 64, x, t.g, bar, policy);
+            } else {
+              tma_load_3d_hint(sb, &maps.b, x, t.col + r * C_::B_ROWS, t.g, bar, policy);
+            }
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {  // copies that are still in flight get time to land before the CTA retires
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 200000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ UMMA issuer (pair: the partner relays "stage landed")
+    const uint32_t idesc = umma_idesc_f16(static_cast<uint32_t>(p.half), TILE_M, BN) | (WG ? kUmmaTransposeA : 0u) |
+                           (C_::B_MN ? kUmmaTransposeB : 0u);
+    const uint64_t desc_a0 = WG ? umma_desc_sw128_mnmajor(smem_base, 8192u) : umma_desc_sw128_kmajor(smem_base);
+    const uint64_t desc_b0 = C_::B_MN ? umma_desc_sw128_mnmajor(smem_base + A_STAGE_BYTES, 8192u)
+                                      : umma_desc_sw128_kmajor(smem_base + A_STAGE_BYTES);
+    constexpr uint64_t A_STEP = WG ? 2048 >> 4 : (UMMA_K * 2) >> 4, B_STEP = C_::B_MN ? 2048 >> 4 : (UMMA_K * 2) >> 4;
+    int stage = 0;
+    uint32_t phase = 0, chain = 0;
+    bool ok = true;
+    // Where the whole warp waits, its lanes have to agree on the outcome: the warp-wide instructions that follow need all.
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      const bool landed = mbar_wait_bounded(bar, parity, abort_flag, WAIT_LIMIT_NS);
+      return WG ? __all_sync(0xFFFFFFFFu, landed) != 0 : landed;
+    };
+    auto commit = [&](uint32_t bar) {
+      if constexpr (PAIR) {
+        umma_commit_pair(bar);
+        umma_commit_pair(map_to_cta(bar, 1));
+      } else {
+        umma_commit(bar);
+      }
+    };
+    auto advance = [&]() {
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    };
+    // Weight gradient, all lanes: rows left .. up to the next multiple of 16 of the staged boxes become zero.
+    auto zero_tail = [&](int left) {
+      const int upto = (left + UMMA_K - 1) / UMMA_K * UMMA_K;
+      uint8_t* st = smem_gen + stage * STAGE_BYTES;
+      constexpr int BOXES = BM / 64 + C_::B_ROWS / 64;
+      for (int i = lane; i < (upto - left) * 8 * BOXES; i += 32) {
+        const int piece = i & 7, box = (i >> 3) % BOXES, row = left + (i >> 3) / BOXES;
+        *reinterpret_cast<uint4*>(st + box * 8192 + row * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    if (PAIR && !leader) {
+      // the whole warp walks along where it may have to clear rows, one thread elsewhere
+      if (WG || elect_one()) {
+        for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
+          const Tile t = tile_at(tile);
+          const int blocks = chain_blocks(t) * (WG ? 1 : p.T);
+          for (int kb = 0; kb < blocks; ++kb) {
+            if (!wait(full_bar(stage), phase)) {
+              ok = false;
+              role_failed = 5;
+              break;
+            }
+            const uint32_t to = map_to_cta(full_bar(stage), 0);
+            if constexpr (WG) {
+              const int left = t.r1 - t.r0 - kb * BK;
+              const bool ragged = left < BK && left % UMMA_K != 0;
+              if (ragged) zero_tail(left);
+              if (elect_one()) {
+                if (ragged) mbar_arrive_cluster_release(to); else mbar_arrive_cluster(to);
+              }
+              __syncwarp();
+            } else {
+              mbar_arrive_cluster(to);
+            }
+            advance();
+          }
+        }
+      }
+    } else if (WG || elect_one()) {
+      for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
+        const Tile t = tile_at(tile);
+        const int blocks = chain_blocks(t);
+        if (WG && blocks == 0) continue;  // an empty group: the epilogue writes zeros
+        const int chains = WG ? 1 : p.T;
+        for (int l = 0; ok && l < chains; ++l, ++chain) {
+          const uint32_t a = chain & 1u;
+          if (!wait(tempty_bar(a), ((chain >> 1) & 1u) ^ 1u)) {
+            ok = false;
+            role_failed = 2;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t tmem_d = tmem_base + a * BN;
+          auto issue = [&](int kb, int steps) {
+            const uint64_t sd = static_cast<uint64_t>(stage) * (STAGE_BYTES >> 4);
+#pragma unroll
+            for (int k = 0; k < BK / UMMA_K; ++k) {
+              if (WG && k >= steps) break;
+              const uint32_t acc = (kb | k) != 0 ? 1u : 0u;
+              if constexpr (PAIR)
+                umma_f16_ss_pair(tmem_d, desc_a0 + sd + k * A_STEP, desc_b0 + sd + k * B_STEP, idesc, acc);
+              else
+                umma_f16_ss(tmem_d, desc_a0 + sd + k * A_STEP, desc_b0 + sd + k * B_STEP, idesc, acc);
+            }
+            commit(empty_bar(stage));
+          };
+          for (int kb = 0; kb < blocks; ++kb) {
+            if (!wait(full_bar(stage), phase)) {
+              ok = false;
+              role_failed = 3;
+              break;
+            }
+            tc_fence_after_sync();
+            if constexpr (WG) {
+              const int left = t.r1 - t.r0 - kb * BK;
+              if (left < BK && left % UMMA_K != 0) {
+                if constexpr (PAIR) fence_acq_rel_cluster();  // the partner's zeros
+                zero_tail(left);
+              }
+              if (elect_one()) issue(kb, left >= BK ? BK / UMMA_K : (left + UMMA_K - 1) / UMMA_K);
+              __syncwarp();
+            } else {
+              issue(kb, BK / UMMA_K);
+            }
+            advance();
+          }
+          if (ok) {
+            if constexpr (WG) {
+              if (elect_one()) commit(tfull_bar(a));
+              __syncwarp();
+            } else {
+              commit(tfull_bar(a));
+            }
+          }
+        }
+      }
+    }
+  } else if (warp >= EPI_WARP0) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;                 // tensor-memory lane quadrant of this warp
+    const int h = (warp - EPI_WARP0) >> 2;  // its half of the columns
+    const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t tempty0 = PAIR ? map_to_cta(tempty_bar(0), 0) : tempty_bar(0);
+    uint8_t* staging = smem_gen + C_::OFF_STAGING + (warp - EPI_WARP0) * STAGING_BYTES_PER_WARP;
+    const int es = p.out32 ? 4 : 2;
+    const bool vec_ok = (p.ldc * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.C) & 15u) == 0 &&
+                        (!WG || (static_cast<int64_t>(p.rows) * p.ldc * es) % 16 == 0);
+    bool ok = true;
+
+    // 32 columns of this warp's 32 rows from registers to C.  64 bytes of each row at a time meet in shared memory (their
+    // 16-byte pieces permuted against bank conflicts) and leave as whole pieces of 8 rows per instruction.
+    auto store_chunk = [&](const float (&v)[CHUNK], uint8_t* c_row0, int rows_left, int col0) {
+      // c_row0: element (first row of this warp, column 0); rows_left, p.cols: what exists
+      const int passes = p.out32 ? 2 : 1;
+      for (int ps = 0; ps < passes; ++ps) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint4 w;
+          if (p.out32) {
+            w = ps == 0 ? make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]))
+                        : make_uint4(__float_as_uint(v[16 + 4 * j]), __float_as_uint(v[17 + 4 * j]), __float_as_uint(v[18 + 4 * j]), __float_as_uint(v[19 + 4 * j]));
+          } else if (p.half) {
+            w = make_uint4(Pack16<__nv_bfloat16>::from_f32(v[8 * j], v[8 * j + 1]), Pack16<__nv_bfloat16>::from_f32(v[8 * j + 2], v[8 * j + 3]),
+                           Pack16<__nv_bfloat16>::from_f32(v[8 * j + 4], v[8 * j + 5]), Pack16<__nv_bfloat16>::from_f32(v[8 * j + 6], v[8 * j + 7]));
+          } else {
+            w = make_uint4(Pack16<__half>::from_f32(v[8 * j], v[8 * j + 1]), Pack16<__half>::from_f32(v[8 * j + 2], v[8 * j + 3]),
+                           Pack16<__half>::from_f32(v[8 * j + 4], v[8 * j + 5]), Pack16<__half>::from_f32(v[8 * j + 6], v[8 * j + 7]));
+          }
+          *reinterpret_cast<uint4*>(staging + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = w;
+        }
+        __syncwarp();
+        const int c0 = col0 + ps * 16;                      // first column of the 64 bytes
+        const int per = 16 / es;                            // columns of one piece
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const int r = it * 8 + (lane >> 2), piece = lane & 3;
+          const uint4 w = *reinterpret_cast<const uint4*>(staging + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
+          const int c = c0 + piece * per;
+          if (r < rows_left && c < p.cols) {
+            uint8_t* dst = c_row0 + (static_cast<int64_t>(r) * p.ldc + c) * es;
+            if (vec_ok && c + per <= p.cols) {
+              *reinterpret_cast<uint4*>(dst) = w;
+            } else {
+              const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                if (i < per && c + i < p.cols) {
+                  if (p.out32) reinterpret_cast<uint32_t*>(dst)[i] = u[i & 3];
+                  else reinterpret_cast<uint16_t*>(dst)[i] = static_cast<uint16_t>(i & 1 ? u[i >> 1] >> 16 : u[i >> 1] & 0xFFFFu);
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();
+      }
+    };
+
+    if (!WG && p.zero_outside) {
+      // rows of no group, before the first and behind the last: one warp per row
+      const int lo = first[0], hi = last[p.groups - 1];
+      const int outside = lo + (p.M - hi);
+      for (int64_t i = static_cast<int64_t>(blockIdx.x) * NUM_EPI_WARPS + warp - EPI_WARP0; i < outside;
+           i += static_cast<int64_t>(gridDim.x) * NUM_EPI_WARPS) {
+        const int64_t row = i < lo ? i : hi + (i - lo);
+        uint8_t* dst = static_cast<uint8_t*>(p.C) + row * p.ldc * es;
+        if (vec_ok && (p.cols * es) % 16 == 0) {
+          for (int c = lane; c < p.cols * es / 16; c += 32) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+          for (int c = lane; c < p.cols * es / 2; c += 32) reinterpret_cast<uint16_t*>(dst)[c] = 0;
+        }
+      }
+    }
+
+    uint32_t chain = 0;
+    for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
+      const Tile t = tile_at(tile);
+      const int chains = WG ? (t.r1 > t.r0 ? 1 : 0) : p.T;
+      const int row0 = t.row + static_cast<int>(cta_rank) * BM + q * 32;  // first row of this warp
+      const int rows_left = (WG ? p.rows : t.r1) - row0;
+      uint8_t* c_row0 = static_cast<uint8_t*>(p.C) +
+                        (WG ? (static_cast<int64_t>(t.g) * p.rows + row0) * p.ldc : static_cast<int64_t>(row0) * p.ldc) * es;
+      const int col0 = t.col + h * C_::CW;
+      if (WG && chains == 0) {
+        float zero[CHUNK];
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j) zero[j] = 0.0f;
+        for (int c = 0; c < C_::NCH; ++c) store_chunk(zero, c_row0, rows_left, col0 + c * CHUNK);
+        continue;
+      }
+      const bool busy = h < C_::EPI_HALVES && rows_left > 0 && col0 < p.cols;  // this warp has something to drain
+      [[maybe_unused]] float node[TREE ? C_::CW : 1];
+      int in_group = 0;
+      uint32_t closed = 0;
+      for (int l = 0; ok && l < chains; ++l, ++chain) {
+        const uint32_t a = chain & 1u;
+        if (!mbar_wait_bounded(tfull_bar(a), (chain >> 1) & 1u, abort_flag, WAIT_LIMIT_NS)) {
+          ok = false;
+          role_failed = 4;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t tacc = tmem_base + lane_off + a * BN + h * C_::CW;
+        auto release = [&]() {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * a);
+        };
+        if (!busy) {
+          release();
+          continue;
+        }
+        if constexpr (!TREE) {
+          uint32_t raw[2][CHUNK];
+          tmem_ld32(tacc, raw[0]);
+#pragma unroll
+          for (int c = 0; c < C_::NCH; ++c) {
+            tmem_wait_ld();
+            if (c + 1 < C_::NCH) tmem_ld32(tacc + (c + 1) * CHUNK, raw[(c + 1) & 1]); else release();
+            float v[CHUNK];
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(raw[c & 1][j]);
+            store_chunk(v, c_row0, rows_left, col0 + c * CHUNK);
+          }
+        } else {
+          constexpr int CW = C_::CW;
+          tmem_wait_st();  // stack stores of earlier leaves have landed
+          uint32_t raw[2][CHUNK];
+          tmem_ld32(tacc, raw[0]);
+#pragma unroll
+          for (int c = 0; c < C_::NCH; ++c) {
+            tmem_wait_ld();
+            if (c + 1 < C_::NCH) tmem_ld32(tacc + (c + 1) * CHUNK, raw[(c + 1) & 1]); else release();
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) {
+              const float v = __uint_as_float(raw[c & 1][j]);
+              node[c * CHUNK + j] = in_group > 0 ? __fadd_rn(node[c * CHUNK + j], v) : v;  // level 0: F leaves left to right
+            }
+          }
+          if (++in_group < p.F) continue;
+          in_group = 0;
+          uint32_t gb = closed++;
+          int lvl = 1;
+          auto stack_col = [&](int level, int c) -> uint32_t {
+            return tmem_base + lane_off + 2 * BN + static_cast<uint32_t>(level - 1) * BN + h * CW + c * CHUNK;
+          };
+          while (lvl < p.L && (gb & 1u)) {
+#pragma unroll
+            for (int c = 0; c < C_::NCH; ++c) {
+              uint32_t s[CHUNK];
+              tmem_ld32(stack_col(lvl, c), s);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < CHUNK; ++j) node[c * CHUNK + j] = __fadd_rn(__uint_as_float(s[j]), node[c * CHUNK + j]);
+            }
+            gb >>= 1;
+            ++lvl;
+          }
+          if (lvl < p.L) {
+#pragma unroll
+            for (int c = 0; c < C_::NCH; ++c) {
+              uint32_t s[CHUNK];
+#pragma unroll
+              for (int j = 0; j < CHUNK; ++j) s[j] = __float_as_uint(node[c * CHUNK + j]);
+              tmem_st32(stack_col(lvl, c), s);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < C_::NCH; ++c) {
+              float v[CHUNK];
+#pragma unroll
+              for (int j = 0; j < CHUNK; ++j) v[j] = node[c * CHUNK + j];
+              store_chunk(v, c_row0, rows_left, col0 + c * CHUNK);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- tear-down
+  tc_fence_before_sync();
+  __syncwarp();
+  if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
+  if (role_failed != 0 && atomicCAS(&g_grouped_status[0], 0u, 1u) == 0u) {
+    g_grouped_status[1] = blockIdx.x;
+    g_grouped_status[2] = static_cast<uint32_t>(role_failed);
+  }
+  if (warp == 2) {
+    tc_fence_after_sync();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS); else tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
 
-template <typename T, typename O>
-__global__ void __launch_bounds__(256) wgrad_kernel(const T* dC, const T* A, O* dW, const int32_t* offsets, int64_t M, int N,
-                                                    int K, int64_t lddc, int64_t lda) {
-  __shared__ float sd[TK][TN + 4], sa[TK][TM + 4];
-  const int k0 = blockIdx.x * TM, n0 = blockIdx.y * TN, g = blockIdx.z;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  int64_t r0, r1;
-  group_rows_of(offsets, g, M, r0, r1);
-  float acc[4][4] = {};
-  for (int64_t r = r0; r < r1; r += TK) {
-    for (int i = threadIdx.x; i < TM * TK; i += 256) {
-      const int c = i % TM, m = i / TM;
-      sd[m][c] = (r + m < r1 && n0 + c < N) ? f32(dC[(r + m) * lddc + n0 + c]) : 0.0f;
-      sa[m][c] = (r + m < r1 && k0 + c < K) ? f32(A[(r + m) * lda + k0 + c]) : 0.0f;
-    }
-    __syncthreads();
-    for (int m = 0; m < TK; ++m)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sd[m][ty * 4 + i], sa[m][tx * 4 + j], acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if (n0 + ty * 4 + i < N && k0 + tx * 4 + j < K)
-        put(dW + (static_cast<int64_t>(g) * N + n0 + ty * 4 + i) * K + k0 + tx * 4 + j, acc[i][j]);
+// ==================================================================== host side
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) == cudaSuccess &&
+        qres == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(ptr);
+    return static_cast<EncodeTiledFn>(nullptr);
+  }();
+  return fn;
 }
 
-template <typename T, typename O>
-int launch(const Params& p, cudaStream_t stream) {
-  const dim3 grid((p.N + TN - 1) / TN, p.groups + (p.outside ? 1 : 0));
-  grouped_kernel<T, O><<<grid, 256, 0, stream>>>(p);
-  const cudaError_t e = cudaGetLastError();
+// `rank` 2 or 3 dimensions of a 16-bit tensor, innermost first, strides in elements; box 64 wide, `box_rows` high.
+int make_map(CUtensorMap* tm, int dtype, const void* base, int rank, const int64_t* dims, const int64_t* strides, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return set_error(TBIK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t d[3], s[2];
+  cuuint32_t box[3] = {BK, static_cast<cuuint32_t>(box_rows), 1}, one[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) d[i] = static_cast<cuuint64_t>(dims[i]);
+  for (int i = 0; i + 1 < rank; ++i) s[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+  const CUresult r = fn(tm, dtype == TBIK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    char msg[160];
+    snprintf(msg, sizeof(msg), "cuTensorMapEncodeTiled failed with CUresult %d (%lld x %lld, stride %lld)", static_cast<int>(r),
+             static_cast<long long>(dims[1]), static_cast<long long>(dims[0]), static_cast<long long>(strides[0]));
+    return set_error(TBIK_ERR_CUDA, msg);
+  }
+  return TBIK_OK;
+}
+
+constexpr int kMaxDevices = 64;
+
+int sms() {
+  static std::atomic<int> cached[kMaxDevices];
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices) dev = 0;
+  n = cached[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = 148;
+    }
+    cached[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// `most_tiles`: more tiles than that cannot exist (0: unknown)
+template <int BN, int STAGES, bool PAIR, int MODE, bool TREE>
+int launch(const Maps& maps, const Params& p, int64_t most_tiles, int max_ctas, cudaStream_t stream) {
+  using C_ = Cfg<BN, STAGES, PAIR, MODE>;
+  auto kernel = grouped_kernel<BN, STAGES, PAIR, MODE, TREE>;
+  static std::atomic<bool> configured[kMaxDevices];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices || !configured[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(C_::smem_bytes(TBIK_MAX_GROUPS)));
+    if (e != cudaSuccess) return set_cuda_error(e, "cudaFuncSetAttribute(grouped_kernel)");
+    if (dev >= 0 && dev < kMaxDevices) configured[dev].store(true, std::memory_order_release);
+  }
+  int ctas = sms();
+  if (max_ctas > 0 && max_ctas < ctas) ctas = max_ctas;
+  int64_t units = PAIR ? (ctas / 2 > 0 ? ctas / 2 : 1) : ctas;
+  if (units > most_tiles) units = most_tiles > 0 ? most_tiles : 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * units : units));
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = C_::smem_bytes(p.groups);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, p);
   return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, "grouped_kernel launch");
-}
-
-template <typename T, typename O>
-int launch_wgrad(const void* dC, const void* A, void* dW, const int32_t* offsets, int64_t M, int N, int K, int groups,
-                 int64_t lddc, int64_t lda, cudaStream_t stream) {
-  const dim3 grid((K + TM - 1) / TM, (N + TN - 1) / TN, groups);
-  wgrad_kernel<T, O><<<grid, 256, 0, stream>>>(static_cast<const T*>(dC), static_cast<const T*>(A), static_cast<O*>(dW), offsets,
-                                               M, N, K, lddc, lda);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, "wgrad_kernel launch");
 }
 
 bool bad_align(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
@@ -154,8 +702,8 @@ int check_common(const char* what, int64_t M, int N, int K, int groups, int dtyp
     snprintf(msg, sizeof(msg), "%s: the result has the operand type or fp32", what);
     return set_error(TBIK_ERR_DTYPE, msg);
   }
-  if (M < 0 || M >= (int64_t(1) << 31) || N < 0 || K <= 0) {
-    snprintf(msg, sizeof(msg), "%s: M in 0 .. 2^31 - 1, N >= 0, K > 0", what);
+  if (M < 0 || M >= (int64_t(1) << 31) - 256 || N < 0 || N >= (1 << 30) || K <= 0 || K >= (1 << 30)) {
+    snprintf(msg, sizeof(msg), "%s: M below 2^31 - 256, N below 2^30, K in 1 .. 2^30 - 1", what);
     return set_error(TBIK_ERR_SHAPE, msg);
   }
   if (groups < 1 || groups > TBIK_MAX_GROUPS) {
@@ -163,6 +711,37 @@ int check_common(const char* what, int64_t M, int N, int K, int groups, int dtyp
     return set_error(TBIK_ERR_SHAPE, msg);
   }
   return TBIK_OK;
+}
+
+// Tile shape of a forward product, from the sizes alone (the groups' sizes are on the device).
+struct Choice {
+  int bn;
+  bool pair;
+};
+
+Choice choose(int64_t M, int N, int groups, int T, int L) {
+  // Levels above level 0 that the spare tensor-memory columns hold: 2 beside 128-column accumulators, 6 and 14 beside
+  // narrower ones, none beside 256-column ones.
+  const int levels = L - 1;
+  if (levels > 6) return {32, false};
+  if (levels > 2) return {64, false};
+  const int64_t rows = M / groups;  // per group, were they even
+  if (rows >= 192) return {T == 1 && N > 128 ? 256 : 128, true};
+  // Few rows: W streams from HBM and every SM has to pull.  The widest tile that still gives most SMs two tiles.
+  const int64_t busy = M < groups ? M : groups;
+  for (int bn = 128; bn > 32; bn /= 2)
+    if (busy * ((N + bn - 1) / bn) >= 2 * 148) return {bn, false};
+  return {32, false};
+}
+
+template <int MODE>
+int forward(const Choice& c, const Maps& maps, const Params& p, int64_t tiles_m, int max_ctas, cudaStream_t stream) {
+  const int64_t most = tiles_m * p.tiles_c;
+  if (c.pair && c.bn == 256) return launch<256, 6, true, MODE, false>(maps, p, most, max_ctas, stream);
+  if (c.pair) return launch<128, 8, true, MODE, true>(maps, p, most, max_ctas, stream);
+  if (c.bn == 128) return launch<128, 6, false, MODE, true>(maps, p, most, max_ctas, stream);
+  if (c.bn == 64) return launch<64, 8, false, MODE, true>(maps, p, most, max_ctas, stream);
+  return launch<32, 8, false, MODE, true>(maps, p, most, max_ctas, stream);
 }
 
 }  // namespace
@@ -174,40 +753,102 @@ int grouped_gemm(const void* A, const void* W, void* C, const int32_t* offsets, 
   if (rc != TBIK_OK) return rc;
   if (w_layout != TBIK_W_K_CONTIGUOUS && w_layout != TBIK_W_N_CONTIGUOUS)
     return set_error(TBIK_ERR_ARG, "tbik_grouped_gemm: unknown layout of W");
-  if (leaf < 0 || leaf % 64 != 0 || (leaf > 0 && K % leaf != 0))
+  if (leaf < 0 || leaf % BK != 0 || (leaf > 0 && K % leaf != 0))
     return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm: leaf must be 0 or a multiple of 64 that divides K");
   int T = 1, F = 1, L = 1;
   if (leaf > 0) (void)tree_shape(K, leaf, &T, &F, &L);
   if (L > 15) return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm: at most 15 tree levels: use a wider leaf");
   if (M == 0 || N == 0) return TBIK_OK;
   if (!A || !W || !C || !offsets) return set_error(TBIK_ERR_ARG, "tbik_grouped_gemm: null pointer");
-  const int64_t w_row = w_layout == TBIK_W_K_CONTIGUOUS ? K : N, w_rows = w_layout == TBIK_W_K_CONTIGUOUS ? N : K;
+  const bool kc = w_layout == TBIK_W_K_CONTIGUOUS;
+  const int64_t w_row = kc ? K : N, w_rows = kc ? N : K;
   if (lda < K || ldw < w_row || ldc < N || (groups > 1 && stride_w < (w_rows - 1) * ldw + w_row))
     return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm: stride smaller than what it steps over");
   if (bad_align(A) || bad_align(W) || lda % 8 || ldw % 8 || stride_w % 8)
     return set_error(TBIK_ERR_ALIGN, "tbik_grouped_gemm: A and W must be 16-byte aligned with strides that are multiples of 8 elements");
-  const Params p{A, W, C, offsets, M, N, K, groups, lda, ldw, stride_w, ldc, w_layout, leaf > 0 ? leaf : K, T, F, L, outside};
-  (void)max_ctas;
-  if (dtype == TBIK_DTYPE_BF16)
-    return out_dtype == TBIK_DTYPE_FP32 ? launch<__nv_bfloat16, float>(p, stream) : launch<__nv_bfloat16, __nv_bfloat16>(p, stream);
-  return out_dtype == TBIK_DTYPE_FP32 ? launch<__half, float>(p, stream) : launch<__half, __half>(p, stream);
+  if (reinterpret_cast<uintptr_t>(C) % (out_dtype == TBIK_DTYPE_FP32 ? 4 : 2))
+    return set_error(TBIK_ERR_ALIGN, "tbik_grouped_gemm: C must be aligned to its element size");
+
+  const Choice c = choose(M, N, groups, T, L);
+  Maps maps;
+  const int64_t da[2] = {K, M}, sa[1] = {lda};
+  for (int i = 0; i < 4; ++i) {
+    rc = make_map(&maps.a[i], dtype, A, 2, da, sa, 16 << i);
+    if (rc != TBIK_OK) return rc;
+  }
+  const int64_t dw[3] = {w_row, w_rows, groups}, sw[2] = {ldw, groups > 1 ? stride_w : (w_rows * ldw + 7) / 8 * 8};
+  rc = make_map(&maps.b, dtype, W, 3, dw, sw, kc ? (c.pair ? c.bn / 2 : c.bn) : BK);
+  if (rc != TBIK_OK) return rc;
+
+  Params p{};
+  p.C = C;
+  p.offsets = offsets;
+  p.ldc = ldc;
+  p.M = static_cast<int>(M);
+  p.groups = groups;
+  p.cols = N;
+  p.red = K;
+  p.kblocks_per_leaf = leaf > 0 ? leaf / BK : (K + BK - 1) / BK;
+  p.T = T;
+  p.F = F;
+  p.L = L;
+  p.tiles_c = (N + c.bn - 1) / c.bn;
+  p.half = dtype == TBIK_DTYPE_BF16 ? 1 : 0;
+  p.out32 = out_dtype == TBIK_DTYPE_FP32 ? 1 : 0;
+  p.zero_outside = outside;
+  const int tile_m = c.pair ? 2 * BM : BM;
+  const int64_t tiles_m = M / tile_m + (M < groups ? M : groups);  // a ragged last tile per group at most
+  if (tiles_m * p.tiles_c >= (int64_t(1) << 31)) return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm: too many tiles");
+  return kc ? forward<kForwardK>(c, maps, p, tiles_m, max_ctas, stream) : forward<kForwardN>(c, maps, p, tiles_m, max_ctas, stream);
 }
 
 int grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* offsets, int64_t M, int N, int K, int groups,
                        int64_t lddc, int64_t lda, int dtype, int out_dtype, int max_ctas, cudaStream_t stream) {
   int rc = check_common("tbik_grouped_gemm_wgrad", M, N, K, groups, dtype, out_dtype);
   if (rc != TBIK_OK || N == 0) return rc;
+  if (M == 0) return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm_wgrad: no rows: the gradient is zero");
   if (!dC || !A || !dW || !offsets) return set_error(TBIK_ERR_ARG, "tbik_grouped_gemm_wgrad: null pointer");
   if (lddc < N || lda < K) return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm_wgrad: leading dimension smaller than the row");
   if (bad_align(A) || bad_align(dC) || lda % 8 || lddc % 8)
     return set_error(TBIK_ERR_ALIGN, "tbik_grouped_gemm_wgrad: operands must be 16-byte aligned with row strides that are multiples of 8 elements");
-  (void)max_ctas;
-  if (dtype == TBIK_DTYPE_BF16)
-    return out_dtype == TBIK_DTYPE_FP32
-               ? launch_wgrad<__nv_bfloat16, float>(dC, A, dW, offsets, M, N, K, groups, lddc, lda, stream)
-               : launch_wgrad<__nv_bfloat16, __nv_bfloat16>(dC, A, dW, offsets, M, N, K, groups, lddc, lda, stream);
-  return out_dtype == TBIK_DTYPE_FP32 ? launch_wgrad<__half, float>(dC, A, dW, offsets, M, N, K, groups, lddc, lda, stream)
-                                      : launch_wgrad<__half, __half>(dC, A, dW, offsets, M, N, K, groups, lddc, lda, stream);
+  if (reinterpret_cast<uintptr_t>(dW) % (out_dtype == TBIK_DTYPE_FP32 ? 4 : 2))
+    return set_error(TBIK_ERR_ALIGN, "tbik_grouped_gemm_wgrad: dW must be aligned to its element size");
+  Maps maps;
+  const int64_t dd[2] = {N, M}, sd[1] = {lddc}, da[2] = {K, M}, sa[1] = {lda};
+  rc = make_map(&maps.a[0], dtype, dC, 2, dd, sd, BK);
+  if (rc != TBIK_OK) return rc;
+  for (int i = 1; i < 4; ++i) maps.a[i] = maps.a[0];
+  rc = make_map(&maps.b, dtype, A, 2, da, sa, BK);
+  if (rc != TBIK_OK) return rc;
+  const bool pair = N > BM && K > BM;
+  const int bn = pair ? 256 : 128, tile_m = pair ? 2 * BM : BM;
+  Params p{};
+  p.C = dW;
+  p.offsets = offsets;
+  p.ldc = K;
+  p.M = static_cast<int>(M);
+  p.groups = groups;
+  p.rows = N;
+  p.cols = K;
+  p.T = p.F = p.L = 1;
+  p.tiles_r = (N + tile_m - 1) / tile_m;
+  p.tiles_c = (K + bn - 1) / bn;
+  p.half = dtype == TBIK_DTYPE_BF16 ? 1 : 0;
+  p.out32 = out_dtype == TBIK_DTYPE_FP32 ? 1 : 0;
+  const int64_t most = static_cast<int64_t>(groups) * p.tiles_r * p.tiles_c;
+  if (most >= (int64_t(1) << 31)) return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm_wgrad: too many tiles");
+  return pair ? launch<256, 6, true, kWeightGrad, false>(maps, p, most, max_ctas, stream)
+              : launch<128, 6, false, kWeightGrad, false>(maps, p, most, max_ctas, stream);
+}
+
+int grouped_status(uint32_t out[4]) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, g_grouped_status, sizeof(uint32_t) * 4);
+  if (e != cudaSuccess) return set_cuda_error(e, "cudaMemcpyFromSymbol(g_grouped_status)");
+  if (out[0] != 0) {
+    const uint32_t zero[4] = {0, 0, 0, 0};
+    cudaMemcpyToSymbol(g_grouped_status, zero, sizeof(zero));
+  }
+  return TBIK_OK;
 }
 
 }  // namespace tbik

@@ -148,6 +148,14 @@ TBIK_DEVICE void tma_load_2d_hint(uint32_t smem_dst, const void* tmap, int32_t x
       : "memory");
 }
 
+TBIK_DEVICE void tma_load_3d_hint(uint32_t smem_dst, const void* tmap, int32_t x, int32_t y, int32_t z, uint32_t bar,
+                                  uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;"
+      ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
+
 // Tiled store shared memory -> global through the TMA unit (bulk async-group completion).
 TBIK_DEVICE void tma_store_2d(const void* tmap, uint32_t smem_src, int32_t x, int32_t y) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
@@ -202,6 +210,21 @@ TBIK_DEVICE uint64_t umma_desc_sw128_kmajor(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(2) << 61;                           // SWIZZLE_128B
   return d;
 }
+
+// Operand whose REDUCTION index runs over the rows of the staged tile (rows of 64 contiguous elements of the other
+// index, 128-byte swizzle).  8 rows are 1024 bytes; the next 64 elements of the other index lie `atom_bytes` further.
+// Sixteen reduction steps advance the start address by 2048 bytes.
+TBIK_DEVICE uint64_t umma_desc_sw128_mnmajor(uint32_t smem_addr, uint32_t atom_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);        // start address
+  d |= static_cast<uint64_t>((atom_bytes >> 4) & 0x3FFFu) << 16;  // leading byte offset: next 64 elements
+  d |= static_cast<uint64_t>((1024u >> 4) & 0x3FFFu) << 32;      // stride byte offset: next 8 reduction steps
+  d |= static_cast<uint64_t>(1) << 46;                           // descriptor version (sm_100)
+  d |= static_cast<uint64_t>(2) << 61;                           // SWIZZLE_128B
+  return d;
+}
+// Bits of the instruction descriptor for such operands.
+constexpr uint32_t kUmmaTransposeA = 1u << 15, kUmmaTransposeB = 1u << 16;
 
 // Instruction descriptor: fp32 accumulator, both operands K-major, same 16-bit input format.
 // fmt: 0 = fp16, 1 = bf16.
@@ -282,6 +305,12 @@ TBIK_DEVICE void cluster_sync_all() {
 TBIK_DEVICE void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
+
+// The same with a release that also covers this CTA's ordinary writes, for the other CTA of the cluster.
+TBIK_DEVICE void mbar_arrive_cluster_release(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+TBIK_DEVICE void fence_acq_rel_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 
 TBIK_DEVICE void tmem_alloc_pair(uint32_t smem_result, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_result), "r"(ncols)

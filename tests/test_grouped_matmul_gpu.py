@@ -299,3 +299,27 @@ def test_two_streams_and_a_graph():
     off.copy_(torch.tensor([0, 7, 250, 290], dtype=torch.int32))
     graph.replay()
     assert torch.equal(c, forward_ref(A, W, off)[0].to(torch.bfloat16)) and torch.equal(d, wgrad_ref(D, A, off)[0].to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes,K,N,leaf", [([1, 7, 16, 17, 33], 512, 384, 512), ([64, 0, 65, 128, 129], 1024, 256, 128),
+                                            ([300, 1, 1000], 768, 640, 96 * 8), ([700, 500], 2048, 512, 256), ([5, 6], 4096, 1024, 512),
+                                            ([40, 50], 2048, 128, 64)])
+def test_a_groups_rows_have_the_dense_products_bits(sizes, K, N, leaf, dtype):
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent
+    from llm_reproducibility_b200.tbik.tree_based_matmul import matmul_tp_persistent
+    M, G = sum(sizes), len(sizes)
+    A, W = make((M, K), dtype, "normal", 21), make((G, N, K), dtype, "normal", 22, 0.1)
+    off = offsets_of(sizes).cuda()
+    got = grouped_matmul_tp_persistent(A, W, off, leaf=leaf)
+    if leaf == K:
+        assert torch.equal(got, grouped_matmul_tp_persistent(A, W, off))  # K is one leaf by default
+    for g, (lo, hi) in enumerate(zip(off.tolist(), off.tolist()[1:])):
+        if hi > lo:
+            assert torch.equal(got[lo:hi], matmul_tp_persistent(A[lo:hi], W[g].t(), node_dtype=torch.float32, leaf=leaf)), g
+
+
+def test_device_status_stays_clean():
+    from llm_reproducibility_b200.tbik.tree_based_matmul import gemm_device_status
+    torch.cuda.synchronize()
+    assert gemm_device_status()[0] == 0
