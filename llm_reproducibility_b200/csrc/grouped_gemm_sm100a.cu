@@ -13,19 +13,21 @@
 // starts (offsets are read on the device), then the persistent loop of each role finds its tile's group by binary search.
 // A tile's rows end with the group: rows beyond it are multiplied (they are the next group's) and not stored.
 //
-//   warp 0      TMA producer   128-byte swizzled boxes of 64 reduction steps; of A only 16, 32, 64 or 128 rows, as many as the
-//                              tile has rows, so a decode step's tiles of a few rows read W and little else
+// Forward tiles put the WEIGHT's rows on the instruction's 128 (256) lanes and the tokens on its columns: the token count
+// of an instruction is a run-time field in steps of 16 (32), so a ragged group costs what it holds, and a decode step's
+// tiles of a few tokens read W and little else.  A group's tokens are dealt evenly to as few tiles as fit.
+//
+//   warp 0      TMA producer   128-byte swizzled boxes of 64 reduction steps; of the tokens 16, 32, 64 or 128 rows
 //   warp 1      UMMA issuer    two accumulators: tile (or leaf) i+1 runs while i drains
 //   warp 2      tensor memory
-//   warps 4-11  epilogue       tcgen05.ld, tree, rounding, rows regrouped through 2 KiB of shared memory per warp so that a
-//                              store instruction writes whole 64-byte pieces of rows
+//   warps 4-11  epilogue       tcgen05.ld, tree, rounding, store
 //
-// The operands' contiguous index is the reduction index (K-major) or the other one (MN-major); tensor memory does not
-// care, so the transposed weight and both operands of the weight gradient are read as they lie.  The weight gradient
+// The operands' contiguous index is the reduction index (K-major) or the other one (MN-major); the instruction takes
+// either, so the transposed weight and both operands of the weight gradient are read as they lie.  The weight gradient
 // reduces over a group's rows: its last step ends inside a box, and the rows of the next group that the box brought along
 // are overwritten with zeros in shared memory before the multiply, in both operands (a NaN there must not meet a zero).
 //
-// PAIR: a cluster of two CTAs per 256-row tile (cta_group::2), each with its own 128 rows and half of the columns' operand.
+// PAIR: a cluster of two CTAs per tile (cta_group::2), each with its own 128 rows and half of the columns' operand.
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -48,11 +50,8 @@ constexpr int NUM_EPI_WARPS = 8;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int CHUNK = 32;  // accumulator columns per tcgen05.ld
 constexpr uint64_t WAIT_LIMIT_NS = 2000000000ull;
-constexpr uint32_t A_STAGE_BYTES = BM * BK * 2;
 constexpr uint32_t STAGING_BYTES_PER_WARP = 2048;
 constexpr int GROUP_M = 8;  // row tiles that share a sweep over the columns
-
-enum Mode { kForwardK = 0, kForwardN = 1, kWeightGrad = 2 };
 
 __device__ uint32_t g_grouped_status[4];  // [0] a bounded wait ran out, [1] block, [2] role
 
@@ -61,34 +60,84 @@ struct Maps {
   CUtensorMap b;     // W; weight gradient: A
 };
 
-struct Params {
+// The groups' rows and tiles in shared memory: first[g], last[g] and before[g] = tiles of the groups before g (G + 1
+// entries), tiles_of(rows) tiles each.  Whatever `offsets` holds, the running maximum keeps the groups' rows inside
+// [0, M) and disjoint.  Called by all threads; one more barrier has to follow before the table is read.
+template <typename TilesOf>
+TBIK_DEVICE void build_table(const int32_t* offsets, int groups, int M, int* first, int* last, int* before, TilesOf tiles_of) {
+  for (int g = threadIdx.x; g < groups; g += NUM_THREADS) last[g] = min(max(offsets[g + 1], 0), M);
+  const int lane = threadIdx.x & 31;
+  int run = 0, end = threadIdx.x < 32 ? min(max(offsets[0], 0), M) : 0;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  for (int g0 = 0; g0 < groups; g0 += 32) {
+    const int g = g0 + lane;
+    int hi = g < groups ? max(last[g], end) : end;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, hi, o);
+      if (lane >= o) hi = max(hi, v);
+    }
+    int lo = __shfl_up_sync(0xFFFFFFFFu, hi, 1);
+    if (lane == 0) lo = end;
+    const int t = g < groups ? tiles_of(hi - lo) : 0;
+    int s = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, s, o);
+      if (lane >= o) s += v;
+    }
+    if (g < groups) {
+      first[g] = lo;
+      last[g] = hi;
+      before[g] = run + s - t;
+    }
+    run += __shfl_sync(0xFFFFFFFFu, s, 31);
+    end = __shfl_sync(0xFFFFFFFFu, hi, 31);
+  }
+  if (lane == 0) before[groups] = run;
+}
+
+// The group that a tile belongs to: before[g] <= tile < before[g + 1].
+TBIK_DEVICE int group_of(const int* before, int groups, int tile) {
+  int lo = 0, hi = groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (before[mid] <= tile) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// ---------------------------------------------------------------- forward
+struct ForwardParams {
   void* C;
   const int32_t* offsets;
   int64_t ldc;
-  int M, groups;
-  int rows, cols, red;  // forward: -, N, K; weight gradient: N, K, -
-  int kblocks_per_leaf, T, F, L;
-  int tiles_c;          // column tiles
-  int tiles_r;          // weight gradient: row tiles
-  int half;             // 16-bit type of the operands: 1 bf16, 0 fp16 (the UMMA format code)
-  int out32;            // C is fp32
-  int zero_outside;     // forward: rows of no group are set to zero
+  int M, N, groups;
+  int blocks_per_leaf, T, F, L;  // 64-step blocks per leaf; the tree
+  int tiles_w;                   // tiles over the weight's rows
+  int half;                      // 16-bit type of the operands: 1 bf16, 0 fp16 (the UMMA format code)
+  int out32;                     // C is fp32
+  int zero_outside;              // rows of no group are set to zero
 };
 
-template <int BN, int STAGES_, bool PAIR, int MODE>
-struct Cfg {
-  static constexpr int STAGES = STAGES_;
-  static constexpr int TILE_M = PAIR ? 2 * BM : BM;
-  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;  // columns' operand of this CTA
-  static constexpr bool B_MN = MODE != kForwardK;
-  static constexpr uint32_t B_STAGE_BYTES = (B_MN && B_ROWS < 64 ? 64 : B_ROWS) * BK * 2;
-  static constexpr uint32_t STAGE_BYTES = A_STAGE_BYTES + B_STAGE_BYTES;
-  static constexpr int EPI_HALVES = BN >= 64 ? 2 : 1;
-  static constexpr int CW = BN / EPI_HALVES;  // columns per epilogue warp
-  static constexpr int NCH = CW / CHUNK;
-  static constexpr uint32_t OFF_STAGING = STAGES * STAGE_BYTES;
-  static constexpr uint32_t OFF_BARS = OFF_STAGING + NUM_EPI_WARPS * STAGING_BYTES_PER_WARP;
-  static constexpr uint32_t OFF_FULL = OFF_BARS;
+// W_ROWS weight rows per CTA against up to TN tokens.  SUB 64-step blocks share a stage: a barrier round trip of the
+// single-thread roles costs about 300 cycles however little a block holds.
+template <int W_ROWS, int TN_, int SUB_, int STAGES_, bool PAIR, bool W_MN>
+struct ForwardCfg {
+  static constexpr int TN = TN_, SUB = SUB_, STAGES = STAGES_;
+  static constexpr int W_TILE = PAIR ? 2 * W_ROWS : W_ROWS;
+  static constexpr int STEP = PAIR ? 32 : 16;                 // granularity of an instruction's token count
+  static constexpr int T_ROWS = PAIR ? TN / 2 : TN;           // token rows this CTA stages
+  static constexpr uint32_t W_BYTES = (W_MN && W_ROWS < 64 ? 64 : W_ROWS) * BK * 2;  // one block of W
+  static constexpr uint32_t T_BYTES = T_ROWS * BK * 2;        // room for one block of tokens
+  static constexpr uint32_t STAGE_BYTES = SUB * (W_BYTES + T_BYTES);
+  // The instruction reads 128 rows of W whatever the box brought; with narrow tiles the surplus is whatever follows in
+  // the stage, and its results are never read.
+  static_assert(W_ROWS == 128 || (SUB - 1) * W_BYTES + 128 * BK * 2 <= STAGE_BYTES, "the surplus rows stay inside the stage");
+  static constexpr int EPI_HALVES = TN >= 64 ? 2 : 1;
+  static constexpr int CHUNKS = TN / CHUNK / EPI_HALVES;      // token chunks per epilogue warp
+  static constexpr uint32_t OFF_FULL = STAGES * STAGE_BYTES;
   static constexpr uint32_t OFF_EMPTY = OFF_FULL + 8 * STAGES;
   static constexpr uint32_t OFF_TFULL = OFF_EMPTY + 8 * STAGES;
   static constexpr uint32_t OFF_TEMPTY = OFF_TFULL + 16;
@@ -97,28 +146,26 @@ struct Cfg {
   static constexpr uint32_t OFF_TABLE = OFF_ABORT + 8;  // first[G], last[G], tiles before[G + 1]
   static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + 4 * (3 * groups + 1) + 1024; }
   static_assert(smem_bytes(TBIK_MAX_GROUPS) <= 232448, "shared memory budget");
+  // tokens per tile of a group of m rows: as few tiles as TN allows, evenly filled
+  static TBIK_DEVICE int tokens(int m) {
+    const int tiles = (m + TN - 1) / TN;
+    return tiles == 0 ? STEP : ((m + tiles - 1) / tiles + STEP - 1) / STEP * STEP;
+  }
 };
 
-struct Tile {
-  int g, r0, r1;   // group; its rows (forward: rows of this tile; weight gradient: the rows summed over)
-  int row, col;    // first row and column of the result
-};
-
-template <int BN, int STAGES, bool PAIR, int MODE, bool TREE>
-__global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_constant__ Maps maps, const Params p) {
-  using C_ = Cfg<BN, STAGES, PAIR, MODE>;
-  constexpr uint32_t STAGE_BYTES = C_::STAGE_BYTES;
-  constexpr int TILE_M = C_::TILE_M;
-  constexpr bool WG = MODE == kWeightGrad;
+template <int W_ROWS, int TN, int SUB, int STAGES, bool PAIR, bool W_MN, bool TREE>
+__global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_constant__ Maps maps, const ForwardParams p) {
+  using C_ = ForwardCfg<W_ROWS, TN, SUB, STAGES, PAIR, W_MN>;
+  constexpr uint32_t STAGE_BYTES = C_::STAGE_BYTES, T_OFF = SUB * C_::W_BYTES;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t cta_rank = PAIR ? cluster_ctarank() : 0u;
+  const int cta_rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
   const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
   const int num_units = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
-  const bool leader = cta_rank == 0u;
+  const bool leader = cta_rank == 0;
 
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem_gen + C_::OFF_ABORT);
   volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem_gen + C_::OFF_TMEM_PTR);
@@ -128,7 +175,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_co
   auto tempty_bar = [&](int a) { return smem_base + C_::OFF_TEMPTY + 8u * a; };
   int* first = reinterpret_cast<int*>(smem_gen + C_::OFF_TABLE);
   int* last = first + p.groups;
-  int* before = last + p.groups;  // tiles of the groups before
+  int* before = last + p.groups;
 
   if constexpr (PAIR) cluster_sync_all();
   if (threadIdx.x == 0) {
@@ -152,74 +199,34 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_co
       tmem_relinquish();
     }
   }
-  for (int g = threadIdx.x; g < p.groups; g += NUM_THREADS) last[g] = min(max(p.offsets[g + 1], 0), p.M);
-  __syncthreads();
-  if (warp == 0) {
-    // Running maximum: whatever the table holds, the groups' rows are inside the operands and disjoint.
-    int run = 0, end = min(max(p.offsets[0], 0), p.M);
-    for (int g0 = 0; g0 < p.groups; g0 += 32) {
-      const int g = g0 + lane;
-      int hi = g < p.groups ? max(last[g], end) : end;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xFFFFFFFFu, hi, o);
-        if (lane >= o) hi = max(hi, v);
-      }
-      int lo = __shfl_up_sync(0xFFFFFFFFu, hi, 1);
-      if (lane == 0) lo = end;
-      const int t = g < p.groups ? (WG ? p.tiles_r * p.tiles_c : (hi - lo + TILE_M - 1) / TILE_M * p.tiles_c) : 0;
-      int s = t;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xFFFFFFFFu, s, o);
-        if (lane >= o) s += v;
-      }
-      if (g < p.groups) {
-        first[g] = lo;
-        last[g] = hi;
-        before[g] = run + s - t;
-      }
-      run += __shfl_sync(0xFFFFFFFFu, s, 31);
-      end = __shfl_sync(0xFFFFFFFFu, hi, 31);
-    }
-    if (lane == 0) before[p.groups] = run;
-  }
+  build_table(p.offsets, p.groups, p.M, first, last, before,
+              [&](int m) { const int n = C_::tokens(m); return (m + n - 1) / n * p.tiles_w; });
   tc_fence_before_sync();
   if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_ptr_smem;
   const int num_tiles = before[p.groups];
 
+  struct Tile {
+    int g, t0, tokens, w0;  // group; first token row and number of rows; first weight row
+  };
   auto tile_at = [&](int tile) {
-    int lo = 0, hi = p.groups;  // before[lo] <= tile < before[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (before[mid] <= tile) lo = mid; else hi = mid;
-    }
-    const int local = tile - before[lo];
-    const int g0 = first[lo], g1 = last[lo];
-    const int tiles_r = WG ? p.tiles_r : (g1 - g0 + TILE_M - 1) / TILE_M;
-    // GROUP_M row tiles share a sweep over the columns
-    const int block = local / (GROUP_M * p.tiles_c);
-    const int in = local - block * GROUP_M * p.tiles_c;
-    const int height = min(tiles_r - block * GROUP_M, GROUP_M);
-    const int tr = block * GROUP_M + in % height, tc = in / height;
+    const int g = group_of(before, p.groups, tile);
+    const int local = tile - before[g], m = last[g] - first[g], n = C_::tokens(m), tiles_t = (m + n - 1) / n;
+    // GROUP_M token tiles share a sweep over the weight's rows
+    const int block = local / (GROUP_M * p.tiles_w);
+    const int in = local - block * GROUP_M * p.tiles_w;
+    const int height = min(tiles_t - block * GROUP_M, GROUP_M);
+    const int tt = block * GROUP_M + in % height;
     Tile t;
-    t.g = lo;
-    t.col = tc * BN;
-    if constexpr (WG) {
-      t.r0 = g0;
-      t.r1 = g1;
-      t.row = tr * TILE_M;
-    } else {
-      t.r0 = g0 + tr * TILE_M;
-      t.r1 = min(t.r0 + TILE_M, g1);
-      t.row = t.r0;
-    }
+    t.g = g;
+    t.t0 = first[g] + tt * n;
+    t.tokens = min(n, last[g] - t.t0);
+    t.w0 = in / height * C_::W_TILE;
     return t;
   };
-  // stages of one accumulator chain: a leaf, or the group's rows
-  auto chain_blocks = [&](const Tile& t) { return WG ? (t.r1 - t.r0 + BK - 1) / BK : p.kblocks_per_leaf; };
+  // token count of the instructions: whole steps
+  auto issue_tokens = [&](const Tile& t) { return (t.tokens + C_::STEP - 1) / C_::STEP * C_::STEP; };
 
   int role_failed = 0;
 
@@ -232,40 +239,53 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_co
       const uint64_t policy = l2_policy(0);
       for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
         const Tile t = tile_at(tile);
-        const int blocks = chain_blocks(t) * (WG ? 1 : p.T);
-        const int r = static_cast<int>(cta_rank);
-        const int have = WG ? BM : min(max(t.r1 - t.r0 - r * BM, 1), BM);
-        const int box = have <= 16 ? 0 : have <= 32 ? 1 : have <= 64 ? 2 : 3;
-        const CUtensorMap* ta = &maps.a[WG ? 0 : box];
-        const uint32_t bytes = (WG ? A_STAGE_BYTES : (16u << box) * BK * 2) + C_::B_STAGE_BYTES;
-        for (int kb = 0; kb < blocks; ++kb) {
+        const int rows = PAIR ? issue_tokens(t) / 2 : issue_tokens(t);  // token rows of this CTA
+        const int box = rows <= 16 ? 0 : rows <= 32 ? 1 : rows <= 64 ? 2 : 3;
+        const int box_rows = 16 << box;
+        const CUtensorMap* map_t = &maps.a[box];
+        const int t0 = t.t0 + cta_rank * rows, w0 = t.w0 + cta_rank * W_ROWS;
+        const uint32_t block_bytes = C_::W_BYTES + static_cast<uint32_t>(box_rows) * BK * 2;
+        // one stage: up to SUB blocks
+        auto load = [&](int x, int blocks) -> bool {
           if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
             ok = false;
             role_failed = 1;
-            break;
+            return false;
           }
-          const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + A_STAGE_BYTES, bar = full_bar(stage);
-          mbar_arrive_expect_tx(bar, bytes);
-          const int x = kb * BK;
-          if constexpr (WG) {
+          const uint32_t sw = smem_base + stage * STAGE_BYTES, st = sw + T_OFF, bar = full_bar(stage);
+          mbar_arrive_expect_tx(bar, static_cast<uint32_t>(blocks) * block_bytes);
 #pragma unroll
-            for (int u = 0; u < BM / 64; ++u) tma_load_2d_hint(sa + u * 8192, ta, t.row + r * BM + u * 64, t.r0 + x, bar, policy);
+          for (int u = 0; u < SUB; ++u) {
+            if (SUB == 1 || u < blocks) {
+              const int k = x + u * BK;
+              if constexpr (W_MN) {
 #pragma unroll
-            for (int u = 0; u < C_::B_ROWS / 64; ++u)
-              tma_load_2d_hint(sb + u * 8192, &maps.b, t.col + r * C_::B_ROWS + u * 64, t.r0 + x, bar, policy);
-          } else {
-            tma_load_2d_hint(sa, ta, x, t.r0 + r * BM, bar, policy);
-            if constexpr (C_::B_MN) {
-#pragma unroll
-              for (int u = 0; u < (C_::B_ROWS + 63) / 64; ++u)
-                tma_load_3d_hint(sb + u * 8192, &maps.b, t.col + r * C_::B_ROWS + u * 64, x, t.g, bar, policy);
-            } else {
-              tma_load_3d_hint(sb, &maps.b, x, t.col + r * C_::B_ROWS, t.g, bar, policy);
+                for (int v = 0; v < (W_ROWS + 63) / 64; ++v)
+                  tma_load_3d_hint(sw + u * C_::W_BYTES + v * 8192, &maps.b, w0 + v * 64, k, t.g, bar, policy);
+              } else {
+                tma_load_3d_hint(sw + u * C_::W_BYTES, &maps.b, k, w0, t.g, bar, policy);
+              }
+              tma_load_2d_hint(st + u * C_::T_BYTES, map_t, k, t0, bar, policy);
             }
           }
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
+          }
+          return true;
+        };
+        for (int l = 0; ok && l < p.T; ++l) {
+          const int x0 = l * p.blocks_per_leaf * BK;
+          if (SUB == 1 && (p.blocks_per_leaf & 3) == 0) {
+            // straight-line code for four blocks: a taken branch per block costs more than issuing its loads
+            for (int b = 0; ok && b < p.blocks_per_leaf; b += 4) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                if (!load(x0 + (b + u) * BK, 1)) break;
+            }
+          } else {
+            for (int b = 0; b < p.blocks_per_leaf; b += SUB)
+              if (!load(x0 + b * BK, min(SUB, p.blocks_per_leaf - b))) break;
           }
         }
       }
@@ -276,20 +296,419 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_co
       }
     }
   } else if (warp == 1) {
+    if (PAIR && !leader) {
+      // ------------------------------------------------------------ partner: relay "stage landed" to the leader
+      if (elect_one()) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const int stages_per_tile = p.T * ((p.blocks_per_leaf + SUB - 1) / SUB);
+        for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
+          for (int s = 0; s < stages_per_tile; ++s) {
+            if (!mbar_wait_bounded(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
+              ok = false;
+              role_failed = 5;
+              break;
+            }
+            mbar_arrive_cluster(map_to_cta(full_bar(stage), 0));
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+        }
+      }
+    } else if (elect_one()) {
+      // ------------------------------------------------------------ UMMA issuer
+      const uint64_t desc_w0 = W_MN ? umma_desc_sw128_mnmajor(smem_base, 8192u) : umma_desc_sw128_kmajor(smem_base);
+      const uint64_t desc_t0 = umma_desc_sw128_kmajor(smem_base + T_OFF);
+      constexpr uint64_t W_STEP = W_MN ? 2048 >> 4 : (UMMA_K * 2) >> 4, T_STEP = (UMMA_K * 2) >> 4;
+      int stage = 0;
+      uint32_t phase = 0, chain = 0;
+      bool ok = true;
+      auto commit = [&](uint32_t bar) {
+        if constexpr (PAIR) {
+          umma_commit_pair(bar);
+          umma_commit_pair(map_to_cta(bar, 1));
+        } else {
+          umma_commit(bar);
+        }
+      };
+      for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
+        const Tile t = tile_at(tile);
+        const uint32_t idesc = umma_idesc_f16(static_cast<uint32_t>(p.half), PAIR ? 256 : 128, static_cast<uint32_t>(issue_tokens(t))) |
+                               (W_MN ? kUmmaTransposeA : 0u);
+        for (int l = 0; ok && l < p.T; ++l, ++chain) {
+          const uint32_t a = chain & 1u;
+          if (!mbar_wait_bounded(tempty_bar(a), ((chain >> 1) & 1u) ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
+            ok = false;
+            role_failed = 2;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t tmem_d = tmem_base + a * TN;
+          auto stage_of = [&](int b, int blocks) -> bool {
+            if (!mbar_wait_bounded(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
+              ok = false;
+              role_failed = 3;
+              return false;
+            }
+            tc_fence_after_sync();
+            const uint64_t sd = static_cast<uint64_t>(stage) * (STAGE_BYTES >> 4);
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+              if (SUB == 1 || u < blocks) {
+#pragma unroll
+                for (int k = 0; k < BK / UMMA_K; ++k) {
+                  const uint64_t dw = desc_w0 + sd + u * (C_::W_BYTES >> 4) + k * W_STEP;
+                  const uint64_t dt = desc_t0 + sd + u * (C_::T_BYTES >> 4) + k * T_STEP;
+                  const uint32_t acc = (b | u | k) != 0 ? 1u : 0u;
+                  if constexpr (PAIR) umma_f16_ss_pair(tmem_d, dw, dt, idesc, acc);
+                  else umma_f16_ss(tmem_d, dw, dt, idesc, acc);
+                }
+              }
+            }
+            commit(empty_bar(stage));
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+            return true;
+          };
+          if (SUB == 1 && (p.blocks_per_leaf & 3) == 0) {
+            for (int b = 0; ok && b < p.blocks_per_leaf; b += 4) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u)
+                if (!stage_of(b + u, 1)) break;
+            }
+          } else {
+            for (int b = 0; b < p.blocks_per_leaf; b += SUB)
+              if (!stage_of(b, min(SUB, p.blocks_per_leaf - b))) break;
+          }
+          if (ok) commit(tfull_bar(a));
+        }
+      }
+    }
+  } else if (warp >= EPI_WARP0) {
+    // ------------------------------------------------------------ epilogue: lanes are weight rows, columns are tokens
+    const int q = warp & 3;                 // tensor-memory lane quadrant of this warp
+    const int h = (warp - EPI_WARP0) >> 2;  // it drains every second chunk of tokens
+    const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t tempty0 = PAIR ? map_to_cta(tempty_bar(0), 0) : tempty_bar(0);
+    const int es = p.out32 ? 4 : 2;
+    const bool pairs_ok = !p.out32 && p.ldc % 2 == 0 && (reinterpret_cast<uintptr_t>(p.C) & 3u) == 0;
+    bool ok = true;
+
+    if (p.zero_outside) {
+      // rows of no group, before the first and behind the last: one warp per row
+      const bool vec = (p.ldc * es) % 16 == 0 && (static_cast<int64_t>(p.N) * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.C) & 15u) == 0;
+      const int lo = first[0], hi = last[p.groups - 1];
+      for (int64_t i = static_cast<int64_t>(blockIdx.x) * NUM_EPI_WARPS + warp - EPI_WARP0; i < static_cast<int64_t>(lo) + (p.M - hi);
+           i += static_cast<int64_t>(gridDim.x) * NUM_EPI_WARPS) {
+        const int64_t row = i < lo ? i : hi + (i - lo);
+        uint8_t* dst = static_cast<uint8_t*>(p.C) + row * p.ldc * es;
+        if (vec) {
+          for (int64_t c = lane; c < static_cast<int64_t>(p.N) * es / 16; c += 32) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+          for (int64_t c = lane; c < static_cast<int64_t>(p.N) * es / 2; c += 32) reinterpret_cast<uint16_t*>(dst)[c] = 0;
+        }
+      }
+    }
+
+    uint32_t chain = 0;
+    for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
+      const Tile t = tile_at(tile);
+      const int n0 = t.w0 + cta_rank * W_ROWS + q * 32;  // this warp's 32 columns of C
+      const bool busy = h < C_::EPI_HALVES && q * 32 < W_ROWS && n0 < p.N;
+      // v[j]: column n0 + lane of token row tok + j.  A lane holds one column of 32 rows: lanes 2i and 2i + 1 swap halves
+      // of two rows, so that a store instruction writes 64 whole bytes of each of two rows.
+      auto store_chunk = [&](const float (&v)[CHUNK], int tok) {
+        const int left = t.tokens - tok;
+        if (p.out32) {
+          float* dst = static_cast<float*>(p.C) + static_cast<int64_t>(t.t0 + tok) * p.ldc + n0 + lane;
+          const bool in = n0 + lane < p.N;
+#pragma unroll
+          for (int j = 0; j < CHUNK; ++j, dst += p.ldc)
+            if (j < left && in) *dst = v[j];
+          return;
+        }
+        const bool odd = (lane & 1) != 0;
+        const int col = lane & ~1;
+        uint16_t* dst = static_cast<uint16_t*>(p.C) + static_cast<int64_t>(t.t0 + tok + (lane & 1)) * p.ldc + n0 + col;
+        const bool both = pairs_ok && n0 + col + 1 < p.N, one = n0 + col < p.N, two = n0 + col + 1 < p.N;
+#pragma unroll
+        for (int j = 0; j < CHUNK; j += 2, dst += 2 * p.ldc) {
+          const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1);
+          const float lo = odd ? other : v[j], hi = odd ? v[j + 1] : other;
+          const uint32_t w = p.half ? Pack16<__nv_bfloat16>::from_f32(lo, hi) : Pack16<__half>::from_f32(lo, hi);
+          if (j + (lane & 1) < left) {
+            if (both) {
+              *reinterpret_cast<uint32_t*>(dst) = w;
+            } else {
+              if (one) dst[0] = static_cast<uint16_t>(w & 0xFFFFu);
+              if (two) dst[1] = static_cast<uint16_t>(w >> 16);
+            }
+          }
+        }
+      };
+      [[maybe_unused]] float node[TREE ? C_::CHUNKS * CHUNK : 1];
+      int in_group = 0;
+      uint32_t closed = 0;
+      for (int l = 0; ok && l < p.T; ++l, ++chain) {
+        const uint32_t a = chain & 1u;
+        if (!mbar_wait_bounded(tfull_bar(a), (chain >> 1) & 1u, abort_flag, WAIT_LIMIT_NS)) {
+          ok = false;
+          role_failed = 4;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t tacc = tmem_base + lane_off + a * TN + h * CHUNK;
+        auto release = [&]() {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * a);
+        };
+        // chunks of this warp that hold tokens: h, h + 2, ...
+        const int have = busy ? ((t.tokens + CHUNK - 1) / CHUNK - h + C_::EPI_HALVES - 1) / C_::EPI_HALVES : 0;
+        if (have <= 0) {
+          release();
+          continue;
+        }
+        if constexpr (!TREE) {
+          uint32_t raw[2][CHUNK];
+          tmem_ld32(tacc, raw[0]);
+#pragma unroll
+          for (int c = 0; c < C_::CHUNKS; ++c) {
+            if (c < have) {
+              tmem_wait_ld();
+              if (c + 1 < C_::CHUNKS && c + 1 < have) tmem_ld32(tacc + (c + 1) * C_::EPI_HALVES * CHUNK, raw[(c + 1) & 1]); else release();
+              float v[CHUNK];
+#pragma unroll
+              for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(raw[c & 1][j]);
+              store_chunk(v, (c * C_::EPI_HALVES + h) * CHUNK);
+            }
+          }
+        } else {
+          tmem_wait_st();  // stack stores of earlier leaves have landed
+          uint32_t raw[C_::CHUNKS][CHUNK];
+#pragma unroll
+          for (int c = 0; c < C_::CHUNKS; ++c)
+            if (c < have) tmem_ld32(tacc + c * C_::EPI_HALVES * CHUNK, raw[c]);
+          tmem_wait_ld();
+          release();
+#pragma unroll
+          for (int c = 0; c < C_::CHUNKS; ++c) {
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) {
+              const float v = __uint_as_float(raw[c][j]);
+              node[c * CHUNK + j] = in_group > 0 ? __fadd_rn(node[c * CHUNK + j], v) : v;  // level 0: F leaves left to right
+            }
+          }
+          if (++in_group < p.F) continue;
+          in_group = 0;
+          uint32_t gb = closed++;
+          int lvl = 1;
+          auto stack_col = [&](int level, int c) -> uint32_t {
+            return tmem_base + lane_off + (1 + level) * TN + (c * C_::EPI_HALVES + h) * CHUNK;
+          };
+          while (lvl < p.L && (gb & 1u)) {
+#pragma unroll
+            for (int c = 0; c < C_::CHUNKS; ++c) {
+              if (c < have) {
+                uint32_t s[CHUNK];
+                tmem_ld32(stack_col(lvl, c), s);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < CHUNK; ++j) node[c * CHUNK + j] = __fadd_rn(__uint_as_float(s[j]), node[c * CHUNK + j]);
+              }
+            }
+            gb >>= 1;
+            ++lvl;
+          }
+#pragma unroll
+          for (int c = 0; c < C_::CHUNKS; ++c) {
+            if (c < have) {
+              if (lvl < p.L) {
+                uint32_t s[CHUNK];
+#pragma unroll
+                for (int j = 0; j < CHUNK; ++j) s[j] = __float_as_uint(node[c * CHUNK + j]);
+                tmem_st32(stack_col(lvl, c), s);
+              } else {
+                float v[CHUNK];
+#pragma unroll
+                for (int j = 0; j < CHUNK; ++j) v[j] = node[c * CHUNK + j];
+                store_chunk(v, (c * C_::EPI_HALVES + h) * CHUNK);
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ---------------------------------------------------------------- tear-down
+  tc_fence_before_sync();
+  __syncwarp();
+  if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
+  if (role_failed != 0 && atomicCAS(&g_grouped_status[0], 0u, 1u) == 0u) {
+    g_grouped_status[1] = blockIdx.x;
+    g_grouped_status[2] = static_cast<uint32_t>(role_failed);
+  }
+  if (warp == 2) {
+    tc_fence_after_sync();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS); else tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------- weight gradient
+struct WgradParams {
+  void* C;
+  const int32_t* offsets;
+  int M, groups;
+  int rows, cols;        // N, K: dW[g] is [N, K]
+  int tiles_r, tiles_c;
+  int half, out32;
+};
+
+template <int BN, int STAGES_, bool PAIR>
+struct WgradCfg {
+  static constexpr int STAGES = STAGES_;
+  static constexpr int TILE_M = PAIR ? 2 * BM : BM;
+  static constexpr int B_COLS = PAIR ? BN / 2 : BN;  // columns of A that this CTA stages
+  static constexpr uint32_t A_BYTES = BM * BK * 2;
+  static constexpr uint32_t STAGE_BYTES = A_BYTES + B_COLS * BK * 2;
+  static constexpr int CW = BN / 2;  // columns per epilogue warp
+  static constexpr int NCH = CW / CHUNK;
+  static constexpr uint32_t OFF_STAGING = STAGES * STAGE_BYTES;
+  static constexpr uint32_t OFF_FULL = OFF_STAGING + NUM_EPI_WARPS * STAGING_BYTES_PER_WARP;
+  static constexpr uint32_t OFF_EMPTY = OFF_FULL + 8 * STAGES;
+  static constexpr uint32_t OFF_TFULL = OFF_EMPTY + 8 * STAGES;
+  static constexpr uint32_t OFF_TEMPTY = OFF_TFULL + 16;
+  static constexpr uint32_t OFF_TMEM_PTR = OFF_TEMPTY + 16;
+  static constexpr uint32_t OFF_ABORT = OFF_TMEM_PTR + 4;
+  static constexpr uint32_t OFF_TABLE = OFF_ABORT + 8;
+  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + 4 * (3 * groups + 1) + 1024; }
+  static_assert(smem_bytes(TBIK_MAX_GROUPS) <= 232448, "shared memory budget");
+};
+
+template <int BN, int STAGES, bool PAIR>
+__global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_constant__ Maps maps, const WgradParams p) {
+  using C_ = WgradCfg<BN, STAGES, PAIR>;
+  constexpr uint32_t STAGE_BYTES = C_::STAGE_BYTES;
+  constexpr int TILE_M = C_::TILE_M;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int cta_rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int num_units = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  const bool leader = cta_rank == 0;
+
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem_gen + C_::OFF_ABORT);
+  volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem_gen + C_::OFF_TMEM_PTR);
+  auto full_bar = [&](int s) { return smem_base + C_::OFF_FULL + 8u * s; };
+  auto empty_bar = [&](int s) { return smem_base + C_::OFF_EMPTY + 8u * s; };
+  auto tfull_bar = [&](int a) { return smem_base + C_::OFF_TFULL + 8u * a; };
+  auto tempty_bar = [&](int a) { return smem_base + C_::OFF_TEMPTY + 8u * a; };
+  int* first = reinterpret_cast<int*>(smem_gen + C_::OFF_TABLE);
+  int* last = first + p.groups;
+  int* before = last + p.groups;
+
+  if constexpr (PAIR) cluster_sync_all();
+  if (threadIdx.x == 0) {
+    *abort_flag = 0u;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), (PAIR && leader) ? 2 : 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), PAIR ? 2 * NUM_EPI_WARPS : NUM_EPI_WARPS);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 2) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(smem_base + C_::OFF_TMEM_PTR, TMEM_COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_base + C_::OFF_TMEM_PTR, TMEM_COLS);
+      tmem_relinquish();
+    }
+  }
+  build_table(p.offsets, p.groups, p.M, first, last, before, [&](int) { return p.tiles_r * p.tiles_c; });
+  tc_fence_before_sync();
+  if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_ptr_smem;
+  const int num_tiles = p.groups * p.tiles_r * p.tiles_c;
+
+  struct Tile {
+    int g, r0, count, row, col;  // group, its first row and their number; first row and column of dW[g]
+  };
+  auto tile_at = [&](int tile) {
+    const int per = p.tiles_r * p.tiles_c;
+    const int g = tile / per, local = tile - g * per;
+    const int block = local / (GROUP_M * p.tiles_c);
+    const int in = local - block * GROUP_M * p.tiles_c;
+    const int height = min(p.tiles_r - block * GROUP_M, GROUP_M);
+    return Tile{g, first[g], last[g] - first[g], (block * GROUP_M + in % height) * TILE_M, in / height * BN};
+  };
+
+  int role_failed = 0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint64_t policy = l2_policy(0);
+      for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
+        const Tile t = tile_at(tile);
+        for (int b = 0; b < t.count; b += BK) {
+          if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
+            ok = false;
+            role_failed = 1;
+            break;
+          }
+          const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + C_::A_BYTES, bar = full_bar(stage);
+          mbar_arrive_expect_tx(bar, STAGE_BYTES);
+#pragma unroll
+          for (int u = 0; u < BM / 64; ++u)
+            tma_load_2d_hint(sa + u * 8192, &maps.a[0], t.row + cta_rank * BM + u * 64, t.r0 + b, bar, policy);
+#pragma unroll
+          for (int u = 0; u < C_::B_COLS / 64; ++u)
+            tma_load_2d_hint(sb + u * 8192, &maps.b, t.col + cta_rank * C_::B_COLS + u * 64, t.r0 + b, bar, policy);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 200000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
     // ------------------------------------------------------------ UMMA issuer (pair: the partner relays "stage landed")
-    const uint32_t idesc = umma_idesc_f16(static_cast<uint32_t>(p.half), TILE_M, BN) | (WG ? kUmmaTransposeA : 0u) |
-                           (C_::B_MN ? kUmmaTransposeB : 0u);
-    const uint64_t desc_a0 = WG ? umma_desc_sw128_mnmajor(smem_base, 8192u) : umma_desc_sw128_kmajor(smem_base);
-    const uint64_t desc_b0 = C_::B_MN ? umma_desc_sw128_mnmajor(smem_base + A_STAGE_BYTES, 8192u)
-                                      : umma_desc_sw128_kmajor(smem_base + A_STAGE_BYTES);
-    constexpr uint64_t A_STEP = WG ? 2048 >> 4 : (UMMA_K * 2) >> 4, B_STEP = C_::B_MN ? 2048 >> 4 : (UMMA_K * 2) >> 4;
+    // The whole warp walks along: it may have to clear rows.
+    const uint32_t idesc = umma_idesc_f16(static_cast<uint32_t>(p.half), TILE_M, BN) | kUmmaTransposeA | kUmmaTransposeB;
+    const uint64_t desc_a0 = umma_desc_sw128_mnmajor(smem_base, 8192u);
+    const uint64_t desc_b0 = umma_desc_sw128_mnmajor(smem_base + C_::A_BYTES, 8192u);
+    constexpr uint64_t STEP = 2048 >> 4;
     int stage = 0;
     uint32_t phase = 0, chain = 0;
     bool ok = true;
-    // Where the whole warp waits, its lanes have to agree on the outcome: the warp-wide instructions that follow need all.
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-      const bool landed = mbar_wait_bounded(bar, parity, abort_flag, WAIT_LIMIT_NS);
-      return WG ? __all_sync(0xFFFFFFFFu, landed) != 0 : landed;
+    // The lanes have to agree on the outcome: the warp-wide instructions that follow need all of them.
+    auto wait = [&](uint32_t bar, uint32_t parity, int role) {
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, parity, abort_flag, WAIT_LIMIT_NS)) != 0;
+      if (!ok) role_failed = role;
+      return ok;
     };
     auto commit = [&](uint32_t bar) {
       if constexpr (PAIR) {
@@ -305,11 +724,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_co
         phase ^= 1u;
       }
     };
-    // Weight gradient, all lanes: rows left .. up to the next multiple of 16 of the staged boxes become zero.
+    // Rows left .. up to the next multiple of 16 of the staged boxes become zero.
     auto zero_tail = [&](int left) {
       const int upto = (left + UMMA_K - 1) / UMMA_K * UMMA_K;
       uint8_t* st = smem_gen + stage * STAGE_BYTES;
-      constexpr int BOXES = BM / 64 + C_::B_ROWS / 64;
+      constexpr int BOXES = static_cast<int>(STAGE_BYTES / 8192);
       for (int i = lane; i < (upto - left) * 8 * BOXES; i += 32) {
         const int piece = i & 7, box = (i >> 3) % BOXES, row = left + (i >> 3) / BOXES;
         *reinterpret_cast<uint4*>(st + box * 8192 + row * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -318,102 +737,65 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_co
       __syncwarp();
     };
     if (PAIR && !leader) {
-      // the whole warp walks along where it may have to clear rows, one thread elsewhere
-      if (WG || elect_one()) {
-        for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
-          const Tile t = tile_at(tile);
-          const int blocks = chain_blocks(t) * (WG ? 1 : p.T);
-          for (int kb = 0; kb < blocks; ++kb) {
-            if (!wait(full_bar(stage), phase)) {
-              ok = false;
-              role_failed = 5;
-              break;
-            }
-            const uint32_t to = map_to_cta(full_bar(stage), 0);
-            if constexpr (WG) {
-              const int left = t.r1 - t.r0 - kb * BK;
-              const bool ragged = left < BK && left % UMMA_K != 0;
-              if (ragged) zero_tail(left);
-              if (elect_one()) {
-                if (ragged) mbar_arrive_cluster_release(to); else mbar_arrive_cluster(to);
-              }
-              __syncwarp();
-            } else {
-              mbar_arrive_cluster(to);
-            }
-            advance();
-          }
-        }
-      }
-    } else if (WG || elect_one()) {
       for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
         const Tile t = tile_at(tile);
-        const int blocks = chain_blocks(t);
-        if (WG && blocks == 0) continue;  // an empty group: the epilogue writes zeros
-        const int chains = WG ? 1 : p.T;
-        for (int l = 0; ok && l < chains; ++l, ++chain) {
-          const uint32_t a = chain & 1u;
-          if (!wait(tempty_bar(a), ((chain >> 1) & 1u) ^ 1u)) {
-            ok = false;
-            role_failed = 2;
-            break;
+        for (int b = 0; b < t.count; b += BK) {
+          if (!wait(full_bar(stage), phase, 5)) break;
+          const int left = t.count - b;
+          const bool ragged = left < BK && left % UMMA_K != 0;
+          if (ragged) zero_tail(left);
+          if (elect_one()) {
+            const uint32_t to = map_to_cta(full_bar(stage), 0);
+            if (ragged) mbar_arrive_cluster_release(to); else mbar_arrive_cluster(to);
           }
+          __syncwarp();
+          advance();
+        }
+      }
+    } else {
+      for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
+        const Tile t = tile_at(tile);
+        if (t.count == 0) continue;  // an empty group: the epilogue writes zeros
+        const uint32_t a = chain & 1u;
+        if (!wait(tempty_bar(a), ((chain >> 1) & 1u) ^ 1u, 2)) break;
+        ++chain;
+        tc_fence_after_sync();
+        const uint32_t tmem_d = tmem_base + a * BN;
+        for (int b = 0; b < t.count; b += BK) {
+          if (!wait(full_bar(stage), phase, 3)) break;
           tc_fence_after_sync();
-          const uint32_t tmem_d = tmem_base + a * BN;
-          auto issue = [&](int kb, int steps) {
+          const int left = t.count - b;
+          if (left < BK && left % UMMA_K != 0) {
+            if constexpr (PAIR) fence_acq_rel_cluster();  // the partner's zeros
+            zero_tail(left);
+          }
+          if (elect_one()) {
             const uint64_t sd = static_cast<uint64_t>(stage) * (STAGE_BYTES >> 4);
+            const int steps = left >= BK ? BK / UMMA_K : (left + UMMA_K - 1) / UMMA_K;
 #pragma unroll
             for (int k = 0; k < BK / UMMA_K; ++k) {
-              if (WG && k >= steps) break;
-              const uint32_t acc = (kb | k) != 0 ? 1u : 0u;
-              if constexpr (PAIR)
-                umma_f16_ss_pair(tmem_d, desc_a0 + sd + k * A_STEP, desc_b0 + sd + k * B_STEP, idesc, acc);
-              else
-                umma_f16_ss(tmem_d, desc_a0 + sd + k * A_STEP, desc_b0 + sd + k * B_STEP, idesc, acc);
+              if (k >= steps) break;
+              const uint32_t acc = (b | k) != 0 ? 1u : 0u;
+              if constexpr (PAIR) umma_f16_ss_pair(tmem_d, desc_a0 + sd + k * STEP, desc_b0 + sd + k * STEP, idesc, acc);
+              else umma_f16_ss(tmem_d, desc_a0 + sd + k * STEP, desc_b0 + sd + k * STEP, idesc, acc);
             }
             commit(empty_bar(stage));
-          };
-          for (int kb = 0; kb < blocks; ++kb) {
-            if (!wait(full_bar(stage), phase)) {
-              ok = false;
-              role_failed = 3;
-              break;
-            }
-            tc_fence_after_sync();
-            if constexpr (WG) {
-              const int left = t.r1 - t.r0 - kb * BK;
-              if (left < BK && left % UMMA_K != 0) {
-                if constexpr (PAIR) fence_acq_rel_cluster();  // the partner's zeros
-                zero_tail(left);
-              }
-              if (elect_one()) issue(kb, left >= BK ? BK / UMMA_K : (left + UMMA_K - 1) / UMMA_K);
-              __syncwarp();
-            } else {
-              issue(kb, BK / UMMA_K);
-            }
-            advance();
+            if (left <= BK) commit(tfull_bar(a));
           }
-          if (ok) {
-            if constexpr (WG) {
-              if (elect_one()) commit(tfull_bar(a));
-              __syncwarp();
-            } else {
-              commit(tfull_bar(a));
-            }
-          }
+          __syncwarp();
+          advance();
         }
       }
     }
   } else if (warp >= EPI_WARP0) {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3;                 // tensor-memory lane quadrant of this warp
-    const int h = (warp - EPI_WARP0) >> 2;  // its half of the columns
+    const int q = warp & 3;
+    const int h = (warp - EPI_WARP0) >> 2;
     const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
     const uint32_t tempty0 = PAIR ? map_to_cta(tempty_bar(0), 0) : tempty_bar(0);
     uint8_t* staging = smem_gen + C_::OFF_STAGING + (warp - EPI_WARP0) * STAGING_BYTES_PER_WARP;
     const int es = p.out32 ? 4 : 2;
-    const bool vec_ok = (p.ldc * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.C) & 15u) == 0 &&
-                        (!WG || (static_cast<int64_t>(p.rows) * p.ldc * es) % 16 == 0);
+    const bool vec_ok = (static_cast<int64_t>(p.cols) * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.C) & 15u) == 0;
     bool ok = true;
 
     // 32 columns of this warp's 32 rows from registers to C.  64 bytes of each row at a time meet in shared memory (their
@@ -446,7 +828,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_co
           const uint4 w = *reinterpret_cast<const uint4*>(staging + r * 64 + ((piece ^ ((r >> 1) & 3)) << 4));
           const int c = c0 + piece * per;
           if (r < rows_left && c < p.cols) {
-            uint8_t* dst = c_row0 + (static_cast<int64_t>(r) * p.ldc + c) * es;
+            uint8_t* dst = c_row0 + (static_cast<int64_t>(r) * p.cols + c) * es;
             if (vec_ok && c + per <= p.cols) {
               *reinterpret_cast<uint4*>(dst) = w;
             } else {
@@ -465,124 +847,48 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_co
       }
     };
 
-    if (!WG && p.zero_outside) {
-      // rows of no group, before the first and behind the last: one warp per row
-      const int lo = first[0], hi = last[p.groups - 1];
-      const int outside = lo + (p.M - hi);
-      for (int64_t i = static_cast<int64_t>(blockIdx.x) * NUM_EPI_WARPS + warp - EPI_WARP0; i < outside;
-           i += static_cast<int64_t>(gridDim.x) * NUM_EPI_WARPS) {
-        const int64_t row = i < lo ? i : hi + (i - lo);
-        uint8_t* dst = static_cast<uint8_t*>(p.C) + row * p.ldc * es;
-        if (vec_ok && (p.cols * es) % 16 == 0) {
-          for (int c = lane; c < p.cols * es / 16; c += 32) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0u, 0u, 0u, 0u);
-        } else {
-          for (int c = lane; c < p.cols * es / 2; c += 32) reinterpret_cast<uint16_t*>(dst)[c] = 0;
-        }
-      }
-    }
-
     uint32_t chain = 0;
     for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
       const Tile t = tile_at(tile);
-      const int chains = WG ? (t.r1 > t.r0 ? 1 : 0) : p.T;
-      const int row0 = t.row + static_cast<int>(cta_rank) * BM + q * 32;  // first row of this warp
-      const int rows_left = (WG ? p.rows : t.r1) - row0;
-      uint8_t* c_row0 = static_cast<uint8_t*>(p.C) +
-                        (WG ? (static_cast<int64_t>(t.g) * p.rows + row0) * p.ldc : static_cast<int64_t>(row0) * p.ldc) * es;
+      const int row0 = t.row + cta_rank * BM + q * 32;  // first row of this warp
+      const int rows_left = p.rows - row0;
+      uint8_t* c_row0 = static_cast<uint8_t*>(p.C) + (static_cast<int64_t>(t.g) * p.rows + row0) * p.cols * es;
       const int col0 = t.col + h * C_::CW;
-      if (WG && chains == 0) {
+      if (t.count == 0) {
         float zero[CHUNK];
 #pragma unroll
         for (int j = 0; j < CHUNK; ++j) zero[j] = 0.0f;
         for (int c = 0; c < C_::NCH; ++c) store_chunk(zero, c_row0, rows_left, col0 + c * CHUNK);
         continue;
       }
-      const bool busy = h < C_::EPI_HALVES && rows_left > 0 && col0 < p.cols;  // this warp has something to drain
-      [[maybe_unused]] float node[TREE ? C_::CW : 1];
-      int in_group = 0;
-      uint32_t closed = 0;
-      for (int l = 0; ok && l < chains; ++l, ++chain) {
-        const uint32_t a = chain & 1u;
-        if (!mbar_wait_bounded(tfull_bar(a), (chain >> 1) & 1u, abort_flag, WAIT_LIMIT_NS)) {
-          ok = false;
-          role_failed = 4;
-          break;
-        }
-        tc_fence_after_sync();
-        const uint32_t tacc = tmem_base + lane_off + a * BN + h * C_::CW;
-        auto release = [&]() {
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * a);
-        };
-        if (!busy) {
-          release();
-          continue;
-        }
-        if constexpr (!TREE) {
-          uint32_t raw[2][CHUNK];
-          tmem_ld32(tacc, raw[0]);
+      const uint32_t a = chain & 1u;
+      if (!mbar_wait_bounded(tfull_bar(a), (chain >> 1) & 1u, abort_flag, WAIT_LIMIT_NS)) {
+        ok = false;
+        role_failed = 4;
+        break;
+      }
+      ++chain;
+      tc_fence_after_sync();
+      const uint32_t tacc = tmem_base + lane_off + a * BN + h * C_::CW;
+      auto release = [&]() {
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * a);
+      };
+      if (rows_left <= 0 || col0 >= p.cols) {
+        release();
+        continue;
+      }
+      uint32_t raw[2][CHUNK];
+      tmem_ld32(tacc, raw[0]);
 #pragma unroll
-          for (int c = 0; c < C_::NCH; ++c) {
-            tmem_wait_ld();
-            if (c + 1 < C_::NCH) tmem_ld32(tacc + (c + 1) * CHUNK, raw[(c + 1) & 1]); else release();
-            float v[CHUNK];
+      for (int c = 0; c < C_::NCH; ++c) {
+        tmem_wait_ld();
+        if (c + 1 < C_::NCH) tmem_ld32(tacc + (c + 1) * CHUNK, raw[(c + 1) & 1]); else release();
+        float v[CHUNK];
 #pragma unroll
-            for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(raw[c & 1][j]);
-            store_chunk(v, c_row0, rows_left, col0 + c * CHUNK);
-          }
-        } else {
-          constexpr int CW = C_::CW;
-          tmem_wait_st();  // stack stores of earlier leaves have landed
-          uint32_t raw[2][CHUNK];
-          tmem_ld32(tacc, raw[0]);
-#pragma unroll
-          for (int c = 0; c < C_::NCH; ++c) {
-            tmem_wait_ld();
-            if (c + 1 < C_::NCH) tmem_ld32(tacc + (c + 1) * CHUNK, raw[(c + 1) & 1]); else release();
-#pragma unroll
-            for (int j = 0; j < CHUNK; ++j) {
-              const float v = __uint_as_float(raw[c & 1][j]);
-              node[c * CHUNK + j] = in_group > 0 ? __fadd_rn(node[c * CHUNK + j], v) : v;  // level 0: F leaves left to right
-            }
-          }
-          if (++in_group < p.F) continue;
-          in_group = 0;
-          uint32_t gb = closed++;
-          int lvl = 1;
-          auto stack_col = [&](int level, int c) -> uint32_t {
-            return tmem_base + lane_off + 2 * BN + static_cast<uint32_t>(level - 1) * BN + h * CW + c * CHUNK;
-          };
-          while (lvl < p.L && (gb & 1u)) {
-#pragma unroll
-            for (int c = 0; c < C_::NCH; ++c) {
-              uint32_t s[CHUNK];
-              tmem_ld32(stack_col(lvl, c), s);
-              tmem_wait_ld();
-#pragma unroll
-              for (int j = 0; j < CHUNK; ++j) node[c * CHUNK + j] = __fadd_rn(__uint_as_float(s[j]), node[c * CHUNK + j]);
-            }
-            gb >>= 1;
-            ++lvl;
-          }
-          if (lvl < p.L) {
-#pragma unroll
-            for (int c = 0; c < C_::NCH; ++c) {
-              uint32_t s[CHUNK];
-#pragma unroll
-              for (int j = 0; j < CHUNK; ++j) s[j] = __float_as_uint(node[c * CHUNK + j]);
-              tmem_st32(stack_col(lvl, c), s);
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < C_::NCH; ++c) {
-              float v[CHUNK];
-#pragma unroll
-              for (int j = 0; j < CHUNK; ++j) v[j] = node[c * CHUNK + j];
-              store_chunk(v, c_row0, rows_left, col0 + c * CHUNK);
-            }
-          }
-        }
+        for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(raw[c & 1][j]);
+        store_chunk(v, c_row0, rows_left, col0 + c * CHUNK);
       }
     }
   }
@@ -600,6 +906,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) grouped_kernel(const __grid_co
     if constexpr (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS); else tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
+
 
 // ==================================================================== host side
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -656,38 +963,51 @@ int sms() {
   return n;
 }
 
-// `most_tiles`: more tiles than that cannot exist (0: unknown)
-template <int BN, int STAGES, bool PAIR, int MODE, bool TREE>
-int launch(const Maps& maps, const Params& p, int64_t most_tiles, int max_ctas, cudaStream_t stream) {
-  using C_ = Cfg<BN, STAGES, PAIR, MODE>;
-  auto kernel = grouped_kernel<BN, STAGES, PAIR, MODE, TREE>;
-  static std::atomic<bool> configured[kMaxDevices];
+// `most`: more tiles than that cannot exist
+template <typename Kernel, typename P>
+int launch(Kernel kernel, std::atomic<bool>* configured, size_t smem_max, size_t smem, bool pair, const Maps& maps, const P& p,
+           int64_t most, int max_ctas, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices || !configured[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(C_::smem_bytes(TBIK_MAX_GROUPS)));
-    if (e != cudaSuccess) return set_cuda_error(e, "cudaFuncSetAttribute(grouped_kernel)");
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_max));
+    if (e != cudaSuccess) return set_cuda_error(e, "cudaFuncSetAttribute(grouped product)");
     if (dev >= 0 && dev < kMaxDevices) configured[dev].store(true, std::memory_order_release);
   }
   int ctas = sms();
   if (max_ctas > 0 && max_ctas < ctas) ctas = max_ctas;
-  int64_t units = PAIR ? (ctas / 2 > 0 ? ctas / 2 : 1) : ctas;
-  if (units > most_tiles) units = most_tiles > 0 ? most_tiles : 1;
+  int64_t units = pair ? (ctas / 2 > 0 ? ctas / 2 : 1) : ctas;
+  if (units > most) units = most > 0 ? most : 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(PAIR ? 2 * units : units));
+  cfg.gridDim = dim3(static_cast<unsigned>(pair ? 2 * units : units));
   cfg.blockDim = dim3(NUM_THREADS);
-  cfg.dynamicSmemBytes = C_::smem_bytes(p.groups);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+  attr[0].val.clusterDim.x = pair ? 2 : 1;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = PAIR ? 1 : 0;
+  cfg.numAttrs = pair ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, p);
-  return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, "grouped_kernel launch");
+  return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, "grouped product launch");
+}
+
+template <int W_ROWS, int TN, int SUB, int STAGES, bool PAIR, bool W_MN, bool TREE>
+int launch_forward(const Maps& maps, const ForwardParams& p, int64_t most, int max_ctas, cudaStream_t stream) {
+  using C_ = ForwardCfg<W_ROWS, TN, SUB, STAGES, PAIR, W_MN>;
+  static std::atomic<bool> configured[kMaxDevices];
+  return launch(forward_kernel<W_ROWS, TN, SUB, STAGES, PAIR, W_MN, TREE>, configured, C_::smem_bytes(TBIK_MAX_GROUPS),
+                C_::smem_bytes(p.groups), PAIR, maps, p, most, max_ctas, stream);
+}
+
+template <int BN, int STAGES, bool PAIR>
+int launch_wgrad(const Maps& maps, const WgradParams& p, int64_t most, int max_ctas, cudaStream_t stream) {
+  using C_ = WgradCfg<BN, STAGES, PAIR>;
+  static std::atomic<bool> configured[kMaxDevices];
+  return launch(wgrad_kernel<BN, STAGES, PAIR>, configured, C_::smem_bytes(TBIK_MAX_GROUPS), C_::smem_bytes(p.groups), PAIR,
+                maps, p, most, max_ctas, stream);
 }
 
 bool bad_align(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
@@ -714,34 +1034,28 @@ int check_common(const char* what, int64_t M, int N, int K, int groups, int dtyp
 }
 
 // Tile shape of a forward product, from the sizes alone (the groups' sizes are on the device).
-struct Choice {
-  int bn;
+struct Shape {
+  int w_rows, tokens;
   bool pair;
 };
+constexpr Shape kPair{128, 256, true}, kPairTree{128, 128, true}, kWide{128, 64, false}, kNarrow{32, 32, false};
 
-Choice choose(int64_t M, int N, int groups, int T, int L) {
-  // Levels above level 0 that the spare tensor-memory columns hold: 2 beside 128-column accumulators, 6 and 14 beside
-  // narrower ones, none beside 256-column ones.
-  const int levels = L - 1;
-  if (levels > 6) return {32, false};
-  if (levels > 2) return {64, false};
+Shape choose(int64_t M, int N, int groups, int T, int L) {
+  // Tree levels above level 0 that the tensor-memory columns beside the accumulators hold: none, 2, 6 and 14.
+  if (L - 1 > 6) return kNarrow;
   const int64_t rows = M / groups;  // per group, were they even
-  if (rows >= 192) return {T == 1 && N > 128 ? 256 : 128, true};
-  // Few rows: W streams from HBM and every SM has to pull.  The widest tile that still gives most SMs two tiles.
+  if (rows >= 48 && L - 1 <= 2) return T == 1 ? kPair : kPairTree;
+  // Few rows: W streams from HBM and every SM has to pull; the wide tile if it still gives most SMs two tiles.
   const int64_t busy = M < groups ? M : groups;
-  for (int bn = 128; bn > 32; bn /= 2)
-    if (busy * ((N + bn - 1) / bn) >= 2 * 148) return {bn, false};
-  return {32, false};
+  return L - 1 > 2 || busy * ((N + 127) / 128) >= 2 * 148 ? kWide : kNarrow;
 }
 
-template <int MODE>
-int forward(const Choice& c, const Maps& maps, const Params& p, int64_t tiles_m, int max_ctas, cudaStream_t stream) {
-  const int64_t most = tiles_m * p.tiles_c;
-  if (c.pair && c.bn == 256) return launch<256, 6, true, MODE, false>(maps, p, most, max_ctas, stream);
-  if (c.pair) return launch<128, 8, true, MODE, true>(maps, p, most, max_ctas, stream);
-  if (c.bn == 128) return launch<128, 6, false, MODE, true>(maps, p, most, max_ctas, stream);
-  if (c.bn == 64) return launch<64, 8, false, MODE, true>(maps, p, most, max_ctas, stream);
-  return launch<32, 8, false, MODE, true>(maps, p, most, max_ctas, stream);
+template <bool W_MN>
+int forward(const Shape& c, const Maps& maps, const ForwardParams& p, int64_t most, int max_ctas, cudaStream_t stream) {
+  if (c.pair && c.tokens == 256) return launch_forward<128, 256, 1, 6, true, W_MN, false>(maps, p, most, max_ctas, stream);
+  if (c.pair) return launch_forward<128, 128, 1, 8, true, W_MN, true>(maps, p, most, max_ctas, stream);
+  if (c.w_rows == 128) return launch_forward<128, 64, 2, 4, false, W_MN, true>(maps, p, most, max_ctas, stream);
+  return launch_forward<32, 32, W_MN ? 2 : 4, W_MN ? 7 : 6, false, W_MN, true>(maps, p, most, max_ctas, stream);
 }
 
 }  // namespace
@@ -769,37 +1083,37 @@ int grouped_gemm(const void* A, const void* W, void* C, const int32_t* offsets, 
   if (reinterpret_cast<uintptr_t>(C) % (out_dtype == TBIK_DTYPE_FP32 ? 4 : 2))
     return set_error(TBIK_ERR_ALIGN, "tbik_grouped_gemm: C must be aligned to its element size");
 
-  const Choice c = choose(M, N, groups, T, L);
+  const Shape c = choose(M, N, groups, T, L);
   Maps maps;
   const int64_t da[2] = {K, M}, sa[1] = {lda};
   for (int i = 0; i < 4; ++i) {
     rc = make_map(&maps.a[i], dtype, A, 2, da, sa, 16 << i);
     if (rc != TBIK_OK) return rc;
   }
-  const int64_t dw[3] = {w_row, w_rows, groups}, sw[2] = {ldw, groups > 1 ? stride_w : (w_rows * ldw + 7) / 8 * 8};
-  rc = make_map(&maps.b, dtype, W, 3, dw, sw, kc ? (c.pair ? c.bn / 2 : c.bn) : BK);
+  const int64_t dw[3] = {w_row, w_rows, groups}, sw[2] = {ldw, groups > 1 ? stride_w : w_rows * ldw};
+  rc = make_map(&maps.b, dtype, W, 3, dw, sw, kc ? c.w_rows : BK);
   if (rc != TBIK_OK) return rc;
 
-  Params p{};
+  ForwardParams p{};
   p.C = C;
   p.offsets = offsets;
   p.ldc = ldc;
   p.M = static_cast<int>(M);
+  p.N = N;
   p.groups = groups;
-  p.cols = N;
-  p.red = K;
-  p.kblocks_per_leaf = leaf > 0 ? leaf / BK : (K + BK - 1) / BK;
+  p.blocks_per_leaf = leaf > 0 ? leaf / BK : (K + BK - 1) / BK;
   p.T = T;
   p.F = F;
   p.L = L;
-  p.tiles_c = (N + c.bn - 1) / c.bn;
+  const int w_tile = c.pair ? 2 * c.w_rows : c.w_rows;
+  p.tiles_w = (N + w_tile - 1) / w_tile;
   p.half = dtype == TBIK_DTYPE_BF16 ? 1 : 0;
   p.out32 = out_dtype == TBIK_DTYPE_FP32 ? 1 : 0;
   p.zero_outside = outside;
-  const int tile_m = c.pair ? 2 * BM : BM;
-  const int64_t tiles_m = M / tile_m + (M < groups ? M : groups);  // a ragged last tile per group at most
-  if (tiles_m * p.tiles_c >= (int64_t(1) << 31)) return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm: too many tiles");
-  return kc ? forward<kForwardK>(c, maps, p, tiles_m, max_ctas, stream) : forward<kForwardN>(c, maps, p, tiles_m, max_ctas, stream);
+  // token tiles: at most one ragged one per group that has rows
+  const int64_t most = (M / c.tokens + (M < groups ? M : groups)) * p.tiles_w;
+  if (most >= (int64_t(1) << 31)) return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm: too many tiles");
+  return kc ? forward<false>(c, maps, p, most, max_ctas, stream) : forward<true>(c, maps, p, most, max_ctas, stream);
 }
 
 int grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* offsets, int64_t M, int N, int K, int groups,
@@ -822,23 +1136,20 @@ int grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* o
   if (rc != TBIK_OK) return rc;
   const bool pair = N > BM && K > BM;
   const int bn = pair ? 256 : 128, tile_m = pair ? 2 * BM : BM;
-  Params p{};
+  WgradParams p{};
   p.C = dW;
   p.offsets = offsets;
-  p.ldc = K;
   p.M = static_cast<int>(M);
   p.groups = groups;
   p.rows = N;
   p.cols = K;
-  p.T = p.F = p.L = 1;
   p.tiles_r = (N + tile_m - 1) / tile_m;
   p.tiles_c = (K + bn - 1) / bn;
   p.half = dtype == TBIK_DTYPE_BF16 ? 1 : 0;
   p.out32 = out_dtype == TBIK_DTYPE_FP32 ? 1 : 0;
   const int64_t most = static_cast<int64_t>(groups) * p.tiles_r * p.tiles_c;
   if (most >= (int64_t(1) << 31)) return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm_wgrad: too many tiles");
-  return pair ? launch<256, 6, true, kWeightGrad, false>(maps, p, most, max_ctas, stream)
-              : launch<128, 6, false, kWeightGrad, false>(maps, p, most, max_ctas, stream);
+  return pair ? launch_wgrad<256, 6, true>(maps, p, most, max_ctas, stream) : launch_wgrad<128, 6, false>(maps, p, most, max_ctas, stream);
 }
 
 int grouped_status(uint32_t out[4]) {
