@@ -1,25 +1,43 @@
-// Low-rank adapters of many requests: out[t] = round(y[t] + s_a B_a h[t]), h[t] = A_a x[t] in fp32, a = adapter of row t.
+// Low-rank adapters of many requests beside a shared projection:
 //
-// First form: one block per row, every dot product by one warp, nothing shared between rows.  K is summed leaf by leaf,
-// the leaves' sums are added pairwise.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+//   h[t]   = A_a x[t]                       fp32, K cut into at most 8 leaves, ((0+1)+(2+3))+((4+5)+(6+7))
+//   out[t] = round(y[t] + s_a B_a h[t])     fp32, a = adapter of row t
+//
+// Both products are skinny (R = 8 .. 128), so what has to move is x, y, out and the adapters in use: memory bound, and
+// mma.sync m16n8k16 keeps up with it while its operands come straight from global memory -- no tensor-memory round trip
+// for 16 columns.  The k index of an instruction may be permuted as long as both operands agree: a lane takes 8
+// neighbouring elements of its row as its share of two instructions, which makes every operand load 16 bytes wide; in the
+// second product the columns are permuted the same way, so that a lane ends up with 8 neighbouring results.
+//
+// One cluster of 1 .. 8 CTAs per (adapter, tile of rows), both products in one launch.  The CTAs split K by leaves, add
+// the leaves through distributed shared memory, and split N for the second product.  Few rows: 16-row tiles and bulk
+// copies of the leaf into shared memory, so that a decode step pays one memory latency; many rows: 32-row tiles, one
+// leaf per warp, operands straight into registers.  Either way a leaf is one chain of instructions over its columns, so
+// a row's bits depend on the row and its adapter alone.
+//
+// h is held in fp32; the second product reads it as the sum of two values of the operand type (16 bits of mantissa for
+// bf16, 22 for fp16, whose rows are scaled by a power of two into its range first).
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
+#include "ptx_sm100a.cuh"
 #include "tbik_internal.h"
 
 namespace tbik {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kLeaves = 8;
+namespace cg = cooperative_groups;
 
-__device__ __forceinline__ float f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float f32(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T rounded(float v);
-template <> __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half rounded<__half>(float v) { return __float2half_rn(v); }
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kLeaves = 8;
+constexpr uint32_t kStageBytes = 49152;  // one of the two buffers of a staged leaf
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+__device__ uint32_t g_adapters_status[4];
 
 struct Params {
   const void *x, *y, *A, *B;
@@ -29,58 +47,497 @@ struct Params {
   const int32_t *order, *offsets;
   int64_t T, ldx, ldy, ldo;
   int N, K, R, adapters, leaf;
+  int cluster;     // CTAs per item
+  int rest;        // rows of no adapter have work to do too (copy y, or zero h)
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) adapters_kernel(const Params p) {
-  __shared__ float hs[TBIK_MAX_RANK];
-  __shared__ int adapter;
-  const int64_t place = blockIdx.x;
-  const int64_t t = p.order[place];
-  if (t < 0 || t >= p.T) return;
-  if (threadIdx.x == 0) {
-    int a = -1;
-    for (int g = 0; g < p.adapters; ++g)
-      if (place >= p.offsets[g] && place < p.offsets[g + 1]) a = g;
-    adapter = a;
+template <typename T> struct Half;
+template <> struct Half<__nv_bfloat16> {
+  TBIK_DEVICE static float f32(uint32_t w, int hi) { return __uint_as_float(hi ? (w & 0xFFFF0000u) : (w << 16)); }
+  TBIK_DEVICE static uint32_t pack(float lo, float hi) { return Pack16<__nv_bfloat16>::from_f32(lo, hi); }
+  TBIK_DEVICE static float round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
+  TBIK_DEVICE static void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
   }
-  __syncthreads();
-  const int a = adapter, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (p.x && a >= 0) {
-    const T* x = static_cast<const T*>(p.x) + t * p.ldx;
-    for (int r = warp; r < p.R; r += kThreads / 32) {
-      const T* w = static_cast<const T*>(p.A) + (static_cast<int64_t>(a) * p.R + r) * p.K;
-      float sum[kLeaves];
+};
+template <> struct Half<__half> {
+  TBIK_DEVICE static float f32(uint32_t w, int hi) {
+    const __half2 v = *reinterpret_cast<const __half2*>(&w);
+    return hi ? __high2float(v) : __low2float(v);
+  }
+  TBIK_DEVICE static uint32_t pack(float lo, float hi) { return Pack16<__half>::from_f32(lo, hi); }
+  TBIK_DEVICE static float round(float v) { return __half2float(__float2half_rn(v)); }
+  TBIK_DEVICE static void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+  }
+};
+
+TBIK_DEVICE void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
+}
+TBIK_DEVICE void prefetch_l2(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(src)), "r"(bytes) : "memory");
+}
+
+TBIK_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Shared memory: [rows TM][item 4][barriers 2][abort][row factors TM] | leaf sums [8 / cluster][TM][R] | h [TM][R] |
+// h as operand [MT][ceil(R / 16)][32 lanes] x 32 bytes | two staging buffers
+struct Layout {
+  uint32_t sums, h, frags, stage, total;
+};
+template <int MT, bool STAGED>
+__host__ __device__ inline Layout layout(int R, int cluster) {
+  constexpr int TM = MT * 16;
+  Layout l;
+  l.sums = 512;
+  l.h = l.sums + (kLeaves / cluster) * TM * R * 4;
+  l.frags = l.h + TM * R * 4;
+  l.stage = (l.frags + MT * ((R + 15) / 16) * 1024 + 127) / 128 * 128;
+  l.total = l.stage + (STAGED ? 2 * kStageBytes : 0);
+  return l;
+}
+
+template <typename T, int MT, bool STAGED>
+__global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
+  constexpr int TM = MT * 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const Layout lay = layout<MT, STAGED>(p.R, p.cluster);
+  int* rows = reinterpret_cast<int*>(smem);                 // row index or -1
+  int* item = rows + TM;                                    // adapter, first place, rows
+  float* factor = reinterpret_cast<float*>(smem + 256);     // what a row of h was divided by (fp16)
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + 240);
+  const uint32_t bars = smem_u32(smem + 224);
+  float* sums = reinterpret_cast<float*>(smem + lay.sums);
+  float* hs = reinterpret_cast<float*>(smem + lay.h);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int C = p.cluster, rank = static_cast<int>(blockIdx.x) % C, want = static_cast<int>(blockIdx.x) / C;
+  const int R = p.R, K = p.K;
+
+  if (tid == 0) {
+    *abort_flag = 0u;
+    item[0] = -2;
+    mbar_init(bars, 1);
+    mbar_init(bars + 8, 1);
+    fence_mbar_init();
+  }
+  // ---- which adapter and rows: tiles of the groups in order, then tiles of the rows of no adapter
+  {
+    int* warp_sum = reinterpret_cast<int*>(smem + lay.sums);  // free until the leaves' sums
+    const int all = static_cast<int>(p.T);
+    const int per = ceil_div(p.adapters, kThreads);
+    int first[4], count[4], mine = 0;                         // adapters <= 1024 = 4 x 256
+    int carry = 0;
 #pragma unroll
-      for (int l = 0; l < kLeaves; ++l) {
-        sum[l] = 0.0f;
-        for (int64_t k = static_cast<int64_t>(l) * p.leaf + lane; k < min(static_cast<int64_t>(l + 1) * p.leaf, static_cast<int64_t>(p.K)); k += 32)
-          sum[l] = fmaf(f32(x[k]), f32(w[k]), sum[l]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum[l] += __shfl_xor_sync(0xFFFFFFFFu, sum[l], o);
+    for (int u = 0; u < 4; ++u) {
+      const int g = tid * per + u;
+      first[u] = count[u] = 0;
+      if (u < per && g < p.adapters) {
+        const int lo = min(max(p.offsets[g], 0), all), hi = min(max(p.offsets[g + 1], lo), all);
+        first[u] = lo;
+        count[u] = hi - lo;
+        mine += ceil_div(hi - lo, TM);
       }
-      if (lane == 0) hs[r] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
     }
-  } else {
-    for (int r = threadIdx.x; r < p.R; r += kThreads) hs[r] = (p.x || a < 0) ? 0.0f : p.h[t * p.R + r];
+    int run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, run, o);
+      if (lane >= o) run += v;
+    }
+    if (lane == 31) warp_sum[warp] = run;
+    __syncthreads();
+    int total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) carry += warp_sum[w];
+      total += warp_sum[w];
+    }
+    int at = carry + run - mine;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int tiles = ceil_div(count[u], TM);
+      if (want >= at && want < at + tiles) {
+        item[1] = first[u] + (want - at) * TM;
+        item[2] = min(TM, first[u] + count[u] - item[1]);
+        item[0] = tid * per + u;
+      }
+      at += tiles;
+    }
+    if (p.rest && tid == 0 && want >= total) {
+      const int lo = min(max(p.offsets[0], 0), all), hi = min(max(p.offsets[p.adapters], lo), all);
+      const int i = (want - total) * TM;  // i-th row of no adapter
+      if (i < lo + all - hi) {
+        item[0] = -1;
+        item[1] = i;
+        item[2] = min(TM, lo + all - hi - i);
+        item[3] = lo;
+      }
+    }
+    __syncthreads();
+  }
+  const int adapter = item[0], place = item[1], count = item[2];
+  if (adapter < -1) return;  // the whole cluster has no item
+  if (tid < TM) {
+    int t = -1;
+    if (tid < count) {
+      int at = place + tid;
+      if (adapter < 0 && at >= item[3]) at += min(max(p.offsets[p.adapters], item[3]), static_cast<int>(p.T)) - item[3];
+      t = p.order[at];
+      if (t < 0 || t >= p.T) t = -1;
+    }
+    rows[tid] = t;
   }
   __syncthreads();
-  if (!p.y) {
-    for (int r = threadIdx.x; r < p.R; r += kThreads) p.h[t * p.R + r] = hs[r];
+  const bool shrink = p.x != nullptr, expand = p.y != nullptr;
+
+  if (adapter < 0) {
+    // rows of no adapter: out = y, or h = 0
+    for (int i = warp * C + rank; i < count; i += kWarps * C) {
+      const int t = rows[i];
+      if (t < 0) continue;
+      if (expand) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + static_cast<int64_t>(t) * p.ldy);
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<int64_t>(t) * p.ldo);
+        for (int c = lane; c < p.N / 8; c += 32) dst[c] = src[c];
+      } else {
+        for (int r = lane; r < R; r += 32) p.h[static_cast<int64_t>(t) * R + r] = 0.0f;
+      }
+    }
     return;
   }
-  const T* y = static_cast<const T*>(p.y) + t * p.ldy;
-  T* out = static_cast<T*>(p.out) + t * p.ldo;
-  for (int n = threadIdx.x; n < p.N; n += kThreads) {
-    if (a < 0) {
-      out[n] = y[n];
-      continue;
+
+  const int g = lane >> 2, c = lane & 3;  // the lane's row (and row + 8) and its place in a row
+  const int nblocks = ceil_div(p.N, 32);
+  const T* B = static_cast<const T*>(p.B) + static_cast<int64_t>(adapter) * p.N * R;
+
+  // ---- first product
+  if (shrink) {
+    const T* A = static_cast<const T*>(p.A) + static_cast<int64_t>(adapter) * R * K;
+    const T* x = static_cast<const T*>(p.x);
+    const int own = kLeaves / C;  // leaves of this CTA
+    const int ntiles = R / 8;
+    if constexpr (STAGED) {
+      // columns per buffer, a multiple of 32; a row's pitch is 64 bytes off a multiple of 128, so that the 16-byte pieces
+      // that 8 lanes read together lie in different banks
+      const int cols = min(static_cast<int>((kStageBytes / (R + TM) - 64) / 128 * 64), (p.leaf + 63) / 64 * 64);
+      const uint32_t pitch = static_cast<uint32_t>(cols) * 2 + 64;
+      const int per_leaf = ceil_div(p.leaf, cols), steps = own * per_leaf;
+      if (expand && warp == 1) {
+        // this CTA's share of B and of the rows of y is wanted right after: on its way to L2 meanwhile
+        const int per = ceil_div(nblocks, C) * 32, n0 = min(rank * per, p.N), n1 = min(n0 + per, p.N);
+        if (lane == 0 && n1 > n0) prefetch_l2(B + static_cast<int64_t>(n0) * R, static_cast<uint32_t>(n1 - n0) * R * 2);
+        if (lane < TM && n1 > n0 && rows[lane] >= 0)
+          prefetch_l2(static_cast<const T*>(p.y) + static_cast<int64_t>(rows[lane]) * p.ldy + n0, static_cast<uint32_t>(n1 - n0) * 2);
+      }
+      auto range = [&](int s, int& k0, int& k1) {
+        const int l = rank * own + s / per_leaf;
+        const int64_t b = static_cast<int64_t>(l) * p.leaf, e = min(b + p.leaf, static_cast<int64_t>(K));
+        const int64_t f = min(b + static_cast<int64_t>(s % per_leaf) * cols, e);
+        k0 = static_cast<int>(f);
+        k1 = static_cast<int>(min(f + cols, e));
+      };
+      auto load = [&](int s) {  // warp 0
+        int k0, k1;
+        range(s, k0, k1);
+        if (k1 <= k0) return;
+        const uint32_t bytes = static_cast<uint32_t>(k1 - k0) * 2, buf = smem_u32(smem + lay.stage) + (s & 1) * kStageBytes, bar = bars + 8 * (s & 1);
+        int live = 0;
+        for (int i = 0; i < TM; ++i) live += rows[i] >= 0 ? 1 : 0;
+        if (lane == 0) mbar_arrive_expect_tx(bar, bytes * static_cast<uint32_t>(R + live));
+        __syncwarp();
+        for (int r = lane; r < R; r += 32) bulk_load(buf + r * pitch, A + static_cast<int64_t>(r) * K + k0, bytes, bar);
+        if (lane < TM && rows[lane] >= 0)
+          bulk_load(buf + (R + lane) * pitch, x + static_cast<int64_t>(rows[lane]) * p.ldx + k0, bytes, bar);
+      };
+      if (warp == 0) {
+        load(0);
+        if (steps > 1) load(1);
+      }
+      float acc[2][4];  // this warp's column tiles: warp, warp + 8
+      uint32_t used[2] = {0u, 0u};
+      bool dead = false;
+      for (int s = 0; s < steps; ++s) {
+        int k0, k1;
+        range(s, k0, k1);
+        if (s % per_leaf == 0) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+        }
+        if (k1 > k0) {
+          // after a wait that ran out the warp keeps step with the barriers and computes on what is there
+          if (!dead && !mbar_wait_bounded(bars + 8 * (s & 1), used[s & 1] & 1u, abort_flag, kWaitNs)) dead = true;
+          ++used[s & 1];
+          const uint8_t* buf = smem + lay.stage + (s & 1) * kStageBytes;
+          const uint8_t* x0 = buf + (R + g) * pitch + c * 16;
+          const bool r0 = rows[g] >= 0, r1 = rows[g + 8] >= 0;
+          const int n = k1 - k0;
+          if (warp < ntiles) {
+#pragma unroll 4
+            for (int k = 0; k < n; k += 32) {
+              const bool in = k + c * 8 < n;
+              const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+              const uint4 a0 = in && r0 ? *reinterpret_cast<const uint4*>(x0 + k * 2) : zero;
+              const uint4 a1 = in && r1 ? *reinterpret_cast<const uint4*>(x0 + 8 * pitch + k * 2) : zero;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                if (warp + 8 * i < ntiles) {
+                  const uint4 b = in ? *reinterpret_cast<const uint4*>(buf + ((warp + 8 * i) * 8 + g) * pitch + c * 16 + k * 2) : zero;
+                  Half<T>::mma(acc[i], make_uint4(a0.x, a1.x, a0.y, a1.y), b.x, b.y);
+                  Half<T>::mma(acc[i], make_uint4(a0.z, a1.z, a0.w, a1.w), b.z, b.w);
+                }
+              }
+            }
+          }
+        }
+        if ((s + 1) % per_leaf == 0) {
+          float* out = sums + (s / per_leaf) * TM * R;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int n = (warp + 8 * i) * 8 + c * 2;
+            if (warp + 8 * i < ntiles) {
+              *reinterpret_cast<float2*>(out + g * R + n) = make_float2(acc[i][0], acc[i][1]);
+              *reinterpret_cast<float2*>(out + (g + 8) * R + n) = make_float2(acc[i][2], acc[i][3]);
+            }
+          }
+        }
+        if (s + 2 < steps) {
+          __syncthreads();  // everyone is done with the buffer
+          if (warp == 0 && !dead) load(s + 2);
+        }
+      }
+      if (dead) {
+        g_adapters_status[1] = blockIdx.x;
+        g_adapters_status[0] = 1u;
+        const uint64_t t0 = global_timer_ns();  // copies in flight get time to land
+        while (global_timer_ns() - t0 < 200000ull) {
+        }
+      }
+    } else {
+      // one leaf per C warps; a warp's column tiles are part, part + C, ... in runs of four
+      const int leaf = rank * own + warp / C, part = warp % C;
+      const int64_t kb = min(static_cast<int64_t>(leaf) * p.leaf, static_cast<int64_t>(K));
+      const int k0 = static_cast<int>(kb), k1 = static_cast<int>(min(kb + p.leaf, static_cast<int64_t>(K)));
+      const T* xr[2 * MT];
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) {
+        const int t = rows[i * 8 + g];
+        xr[i] = t >= 0 ? x + static_cast<int64_t>(t) * p.ldx + c * 8 : nullptr;
+      }
+      float* out = sums + (warp / C) * TM * R;
+      for (int n0 = part; n0 < ntiles; n0 += 4 * C) {
+        float acc[MT][4][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
+        const T* ar = A + static_cast<int64_t>(n0 * 8 + g) * K + c * 8;
+        const int64_t a_step = static_cast<int64_t>(C) * 8 * K;
+#pragma unroll 2
+        for (int k = k0; k < k1; k += 32) {
+          const bool in = k + c * 8 < k1;
+          const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+          uint4 a[2 * MT], b[4];
+#pragma unroll
+          for (int i = 0; i < 2 * MT; ++i) a[i] = in && xr[i] ? __ldg(reinterpret_cast<const uint4*>(xr[i] + k)) : zero;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            b[i] = in && n0 + i * C < ntiles ? __ldg(reinterpret_cast<const uint4*>(ar + i * a_step + k)) : zero;
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              Half<T>::mma(acc[m][i], make_uint4(a[2 * m].x, a[2 * m + 1].x, a[2 * m].y, a[2 * m + 1].y), b[i].x, b[i].y);
+              Half<T>::mma(acc[m][i], make_uint4(a[2 * m].z, a[2 * m + 1].z, a[2 * m].w, a[2 * m + 1].w), b[i].z, b[i].w);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (n0 + i * C < ntiles) {
+            const int n = (n0 + i * C) * 8 + c * 2;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              *reinterpret_cast<float2*>(out + (m * 16 + g) * R + n) = make_float2(acc[m][i][0], acc[m][i][1]);
+              *reinterpret_cast<float2*>(out + (m * 16 + g + 8) * R + n) = make_float2(acc[m][i][2], acc[m][i][3]);
+            }
+          }
+        }
+      }
     }
-    const T* b = static_cast<const T*>(p.B) + (static_cast<int64_t>(a) * p.N + n) * p.R;
-    float d = 0.0f;
-    for (int r = 0; r < p.R; ++r) d = fmaf(hs[r], f32(b[r]), d);
-    out[n] = rounded<T>(f32(y[n]) + p.scales[a] * d);
+    // ---- the leaves' sums, from wherever in the cluster they are
+    cg::cluster_group cluster = cg::this_cluster();
+    if (C > 1) cluster.sync(); else __syncthreads();
+    for (int i = tid; i < TM * R / 4; i += kThreads) {
+      float4 s[kLeaves];
+#pragma unroll
+      for (int l = 0; l < kLeaves; ++l) {
+        const float* from = C > 1 ? cluster.map_shared_rank(sums, l / own) : sums;
+        s[l] = reinterpret_cast<const float4*>(from + (l % own) * TM * R)[i];
+      }
+#pragma unroll
+      for (int d = 1; d < kLeaves; d *= 2)
+#pragma unroll
+        for (int l = 0; l < kLeaves; l += 2 * d)
+          s[l] = make_float4(s[l].x + s[l + d].x, s[l].y + s[l + d].y, s[l].z + s[l + d].z, s[l].w + s[l + d].w);
+      reinterpret_cast<float4*>(hs)[i] = s[0];
+    }
+    if (C > 1) cluster.sync(); else __syncthreads();  // nobody leaves while its sums may still be read
+    if (!expand) {
+      for (int i = tid; i < TM * R / 4; i += kThreads) {
+        const int t = rows[i / (R / 4)];
+        if (t >= 0 && i / (R / 4) % C == rank)
+          reinterpret_cast<float4*>(p.h + static_cast<int64_t>(t) * R)[i % (R / 4)] = reinterpret_cast<const float4*>(hs)[i];
+      }
+      return;
+    }
+  } else {
+    for (int i = tid; i < TM * R / 4; i += kThreads) {
+      const int t = rows[i / (R / 4)];
+      reinterpret_cast<float4*>(hs)[i] = t >= 0 ? reinterpret_cast<const float4*>(p.h + static_cast<int64_t>(t) * R)[i % (R / 4)]
+                                               : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    __syncthreads();
   }
+
+  // ---- h as an operand: high and low parts, arranged per lane
+  constexpr bool kScaled = sizeof(T) == 2 && Pack16<T>::kUmmaFmt == 0;  // fp16
+  if constexpr (kScaled) {
+    for (int i = warp; i < TM; i += kWarps) {
+      float top = 0.0f;
+      for (int r = lane; r < R; r += 32) top = fmaxf(top, fabsf(hs[i * R + r]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      // the largest of the row to about 2^14; 0 and infinity as they are
+      int e = 0;
+      if (top > 0.0f && top < __uint_as_float(0x7F800000u)) e = min(max(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
+      if (lane == 0) factor[i] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    }
+    __syncthreads();
+  }
+  uint4* frags = reinterpret_cast<uint4*>(smem + lay.frags);
+  const int ksteps = (R + 15) / 16;
+  for (int i = tid; i < MT * ksteps * 32; i += kThreads) {
+    const int ln = i & 31, s = (i >> 5) % ksteps, m = (i >> 5) / ksteps;
+    const int r = 16 * s + 4 * (ln & 3);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {  // rows ln / 4 and + 8
+      const int row = m * 16 + (ln >> 2) + 8 * u;
+      float4 v = r < R ? *reinterpret_cast<const float4*>(hs + row * R + r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if constexpr (kScaled) {
+        const float f = factor[row];
+        v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+      }
+      const float t[4] = {Half<T>::round(v.x), Half<T>::round(v.y), Half<T>::round(v.z), Half<T>::round(v.w)};
+      const float w[4] = {v.x, v.y, v.z, v.w};
+      float d[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) d[j] = fabsf(t[j]) < __uint_as_float(0x7F800000u) ? w[j] - t[j] : 0.0f;  // infinity has no low part
+      hi[u] = Half<T>::pack(t[0], t[1]);
+      hi[u + 2] = Half<T>::pack(t[2], t[3]);
+      lo[u] = Half<T>::pack(d[0], d[1]);
+      lo[u + 2] = Half<T>::pack(d[2], d[3]);
+    }
+    frags[2 * i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    frags[2 * i + 1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+  __syncthreads();
+
+  // ---- second product, 32 columns per warp and trip
+  const float scale = p.scales[adapter];
+  const T* y = static_cast<const T*>(p.y);
+  T* out = static_cast<T*>(p.out);
+  const int per = ceil_div(nblocks, C), b1 = min((rank + 1) * per, nblocks);
+  for (int blk = rank * per + warp; blk < b1; blk += kWarps) {
+    const int col = blk * 32 + c * 8;  // the lane's 8 columns
+    const bool in = col < p.N;
+    uint4 yv[2 * MT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const int t = rows[i * 8 + g];
+      if (in && t >= 0) yv[i] = *reinterpret_cast<const uint4*>(y + static_cast<int64_t>(t) * p.ldy + col);
+    }
+    float acc[MT][4][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
+    // column of B that this lane brings for instruction j: 8 (g / 2) + 2 j + g % 2
+    const int n0 = blk * 32 + 8 * (g >> 1) + (g & 1);
+    const T* br = B + static_cast<int64_t>(n0) * R + 4 * c;
+#pragma unroll 2
+    for (int s = 0; s < ksteps; ++s) {
+      uint2 b[4];
+      const bool ok = n0 < p.N && 16 * s + 4 * c < R;  // N is a multiple of 8: all four columns are in or out
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = ok ? __ldg(reinterpret_cast<const uint2*>(br + 2 * j * R + 16 * s)) : make_uint2(0u, 0u);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const uint4 hi = frags[2 * ((m * ksteps + s) * 32 + lane)], lo = frags[2 * ((m * ksteps + s) * 32 + lane) + 1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          Half<T>::mma(acc[m][j], hi, b[j].x, b[j].y);
+          Half<T>::mma(acc[m][j], lo, b[j].x, b[j].y);
+        }
+      }
+    }
+    if (in) {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) {
+        const int t = rows[i * 8 + g];
+        if (t < 0) continue;
+        float s = scale;
+        if constexpr (kScaled) s = scale / factor[i * 8 + g];  // a power of two: exact
+        const uint32_t yw[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float d0 = acc[i >> 1][j][2 * (i & 1)], d1 = acc[i >> 1][j][2 * (i & 1) + 1];
+          o[j] = Half<T>::pack(fmaf(s, d0, Half<T>::f32(yw[j], 0)), fmaf(s, d1, Half<T>::f32(yw[j], 1)));
+        }
+        *reinterpret_cast<uint4*>(out + static_cast<int64_t>(t) * p.ldo + col) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side
+constexpr int kMaxDevices = 64;
+
+template <typename T, int MT, bool STAGED>
+int launch(const Params& p, int64_t items, cudaStream_t stream) {
+  auto kernel = adapters_kernel<T, MT, STAGED>;
+  static std::atomic<bool> configured[kMaxDevices];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices || !configured[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) return set_cuda_error(e, "cudaFuncSetAttribute(adapters_kernel)");
+    if (dev >= 0 && dev < kMaxDevices) configured[dev].store(true, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * p.cluster));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = layout<MT, STAGED>(p.R, p.cluster).total;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(p.cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, "adapters_kernel launch");
 }
 
 bool bad_align(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
@@ -91,8 +548,8 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
              const float* scales, float* h, const int32_t* order, const int32_t* offsets, int64_t T, int N, int K, int R,
              int adapters, int dtype, int leaf, cudaStream_t stream) {
   if (dtype != TBIK_DTYPE_BF16 && dtype != TBIK_DTYPE_FP16) return set_error(TBIK_ERR_DTYPE, "tbik_adapters supports bf16 and fp16");
-  if (T < 0 || T >= (int64_t(1) << 31) || N < 8 || N % 8 || K < 8 || K % 8)
-    return set_error(TBIK_ERR_SHAPE, "tbik_adapters: T in 0 .. 2^31 - 1, N and K positive multiples of 8");
+  if (T < 0 || T >= (int64_t(1) << 25) || N < 8 || N % 8 || N >= (1 << 28) || K < 8 || K % 8 || K >= (1 << 28))
+    return set_error(TBIK_ERR_SHAPE, "tbik_adapters: T in 0 .. 2^25 - 1, N and K positive multiples of 8 below 2^28");
   if (R < 8 || R % 8 || R > TBIK_MAX_RANK) return set_error(TBIK_ERR_SHAPE, "tbik_adapters: R must be a multiple of 8 up to 128");
   if (adapters < 1 || adapters > TBIK_MAX_GROUPS) return set_error(TBIK_ERR_SHAPE, "tbik_adapters: 1 .. 1024 adapters");
   if (leaf == 0) leaf = (K + 255) / 256 * 32;
@@ -106,11 +563,26 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
     return set_error(TBIK_ERR_SHAPE, "tbik_adapters: row stride smaller than the row");
   if (bad_align(x) || bad_align(y) || bad_align(out) || bad_align(A) || bad_align(B) || bad_align(h) || ldx % 8 || ldy % 8 || ldo % 8)
     return set_error(TBIK_ERR_ALIGN, "tbik_adapters: pointers must be 16-byte aligned, row strides multiples of 8 elements");
-  const Params p{x, y, A, B, out, scales, h, order, offsets, T, ldx, ldy, ldo, N, K, R, adapters, leaf};
-  if (dtype == TBIK_DTYPE_BF16) adapters_kernel<__nv_bfloat16><<<static_cast<unsigned>(T), kThreads, 0, stream>>>(p);
-  else adapters_kernel<__half><<<static_cast<unsigned>(T), kThreads, 0, stream>>>(p);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, "adapters_kernel launch");
+  Params p{x, y, A, B, out, scales, h, order, offsets, T, ldx, ldy, ldo, N, K, R, adapters, leaf, 1, 0};
+  p.rest = (expand ? out != y : 1) ? 1 : 0;
+  // Few rows: 16-row tiles.  CTAs per tile: as many as keep the grid near two CTAs per SM.
+  const bool few = T <= 1024;
+  const int rows = few ? 16 : 32;
+  const int64_t items = T / rows + (T < adapters ? T : adapters) + (p.rest ? 1 : 0);
+  while (p.cluster < kLeaves && items * p.cluster * 2 <= 2 * 148 + 148) p.cluster *= 2;
+  if (dtype == TBIK_DTYPE_BF16)
+    return few ? launch<__nv_bfloat16, 1, true>(p, items, stream) : launch<__nv_bfloat16, 2, false>(p, items, stream);
+  return few ? launch<__half, 1, true>(p, items, stream) : launch<__half, 2, false>(p, items, stream);
+}
+
+int adapters_status(uint32_t out[4]) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, g_adapters_status, sizeof(uint32_t) * 4);
+  if (e != cudaSuccess) return set_cuda_error(e, "cudaMemcpyFromSymbol(g_adapters_status)");
+  if (out[0] != 0) {
+    const uint32_t zero[4] = {0, 0, 0, 0};
+    cudaMemcpyToSymbol(g_adapters_status, zero, sizeof(zero));
+  }
+  return TBIK_OK;
 }
 
 }  // namespace tbik

@@ -1045,9 +1045,9 @@ Shape choose(int64_t M, int N, int groups, int T, int L) {
   if (L - 1 > 6) return kNarrow;
   const int64_t rows = M / groups;  // per group, were they even
   if (rows >= 48 && L - 1 <= 2) return T == 1 ? kPair : kPairTree;
-  // Few rows: W streams from HBM and every SM has to pull; the wide tile if it still gives most SMs two tiles.
-  const int64_t busy = M < groups ? M : groups;
-  return L - 1 > 2 || busy * ((N + 127) / 128) >= 2 * 148 ? kWide : kNarrow;
+  // Few rows: W streams from HBM.  An instruction takes about 70 cycles however few rows and tokens it covers, so the full
+  // 128 rows pay even where that leaves SMs without a tile.
+  return kWide;
 }
 
 template <bool W_MN>
