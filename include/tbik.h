@@ -275,19 +275,24 @@ int tbik_ar_trace(tbik_ar_t comm, uint64_t* out, int max_blocks, int* blocks);
 
 /* Stable grouping of M ids.  order[p] = index of the row that comes p-th when rows are sorted by id, rows of one id
  * in their own order; position = its inverse; offsets has groups + 1 entries.  Rows whose id is outside
- * [0, groups) belong to no group and come last, behind offsets[groups].  groups <= TBIK_MAX_GROUPS. */
+ * [0, groups) belong to no group and come last, behind offsets[groups].  groups <= TBIK_MAX_GROUPS.
+ * workspace: tbik_group_workspace_bytes(M, groups) bytes of device memory, 4-byte aligned, that no other call uses until
+ * this one is done; what it holds before and after means nothing. */
 #define TBIK_MAX_GROUPS 1024
+size_t tbik_group_workspace_bytes(int64_t M, int groups);
 int tbik_group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets,
-                    tbik_stream_t stream);
+                    void* workspace, size_t workspace_bytes, tbik_stream_t stream);
 
 /* Router: for each of T rows of logits [T, E] (row stride ld elements, any dtype code) the k largest values, largest
  * first, equal values by lower index, NaN above everything (ids [T, k]); their softmax weights in fp32 (weights
  * [T, k]): with `renormalize` over the k chosen, else over all E.  A row that holds nothing but -inf gets weights 0.
- * Then the grouping of the T * k entries of ids by expert, as tbik_group_rows(ids, T * k, E, ...).
+ * Then the grouping of the T * k entries of ids by expert, as tbik_group_rows(ids, T * k, E, ...); workspace:
+ * tbik_group_workspace_bytes(T * k, E) bytes.
  * 1 <= k <= min(E, TBIK_MAX_TOPK), E <= TBIK_MAX_GROUPS. */
 #define TBIK_MAX_TOPK 32
 int tbik_route_topk(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize, float* weights,
-                    int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, tbik_stream_t stream);
+                    int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                    tbik_stream_t stream);
 
 /* Gradient of the weights of tbik_route_topk with respect to the logits: dlogits [T, E] (row stride ldd, the dtype of
  * the logits), from the forward's weights and ids and dweights [T, k] (contiguous). */

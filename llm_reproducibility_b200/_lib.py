@@ -53,8 +53,9 @@ _PROTOTYPES = {
     "tbik_ar_graph_meta": (_i32, [_vp, _vp, ctypes.POINTER(_i64)]),
     "tbik_ar_register_graph_buffers": (_i32, [_vp, ctypes.POINTER(_vp), ctypes.POINTER(ctypes.POINTER(_i64))]),
     "tbik_ar_status": (_i32, [_vp, ctypes.POINTER(ctypes.c_uint32)]),
-    "tbik_group_rows": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp]),
-    "tbik_route_topk": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "tbik_group_workspace_bytes": (_sz, [_i64, _i32]),
+    "tbik_group_rows": (_i32, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "tbik_route_topk": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "tbik_route_topk_backward": (_i32, [_vp, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
     "tbik_grouped_gemm": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i32,
                                  _i32, _i32, _vp]),

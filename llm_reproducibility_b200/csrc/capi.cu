@@ -158,15 +158,18 @@ int tbik_ar_register_graph_buffers(tbik_ar_t comm, const void* const* handles, c
 
 int tbik_ar_status(tbik_ar_t comm, uint32_t out[8]) { return tbik::ar_status(comm, out); }
 
+size_t tbik_group_workspace_bytes(int64_t M, int groups) { return tbik::group_workspace_bytes(M, groups); }
+
 int tbik_group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets,
-                    tbik_stream_t stream) {
-  return tbik::group_rows(ids, M, groups, order, position, offsets, static_cast<cudaStream_t>(stream));
+                    void* workspace, size_t workspace_bytes, tbik_stream_t stream) {
+  return tbik::group_rows(ids, M, groups, order, position, offsets, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int tbik_route_topk(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize, float* weights,
-                    int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, tbik_stream_t stream) {
-  return tbik::route_topk(logits, ld, T, E, k, dtype, renormalize, weights, ids, order, position, offsets,
-                          static_cast<cudaStream_t>(stream));
+                    int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                    tbik_stream_t stream) {
+  return tbik::route_topk(logits, ld, T, E, k, dtype, renormalize, weights, ids, order, position, offsets, workspace,
+                          workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int tbik_route_topk_backward(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize,

@@ -4,12 +4,16 @@
 // largest key over the warp and, among equal keys, the lowest index (two warp-wide integer reductions).  A score's key
 // is its bit pattern made monotone, so the order is total and exact whatever the type.  Softmax statistics are fp32.
 //
-// Grouping: ONE cluster of up to 8 CTAs x 32 warps.  Warp w of the cluster owns the w-th contiguous run of rows, counts
-// its rows per group (lanes with the same id find each other with match.any, one of them adds), the counts are turned
-// into first places -- over the warps of a CTA in shared memory, over the CTAs through distributed shared memory, over
-// the groups with a scan -- and a second walk over the same rows hands out the places in row order.  No atomics: the
-// order is the stable one whatever the timing.  Both walks read the ids from L2; the bound is the latency of the
-// cluster's few SMs, not bytes.
+// Grouping: rows are dealt to warps in contiguous runs.  Every warp counts its rows per group, the counts are turned into
+// first places -- over the warps of a block, over the blocks, over the groups with a scan -- and a second walk over the same
+// rows hands out the places in row order: lanes with the same id find each other by ballots over the id's bits (a
+// match.any takes some 300 cycles for 32 different ids, eight ballots a third of that).  No global atomics and no waiting
+// between blocks: the order is the stable one whatever the timing.
+//   few rows    one launch of ONE cluster of up to 8 CTAs; the blocks exchange their counts through distributed shared
+//               memory.  What it takes is latency.
+//   many rows   a counting launch (the router itself, which has the ids in registers) leaves one row of counts per block in
+//               the workspace, and a second launch of as many blocks adds up the rows before its own.
+// 131072 rows of 128 groups: one cluster took 41 us, its 8 SMs bound by match.any and by scattered 4-byte stores.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -25,10 +29,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kGroupThreads = 1024;
-constexpr int kGroupWarps = kGroupThreads / 32;
+constexpr int kGroupThreads = 1024;  // of a CTA of the cluster form
+constexpr int kManyThreads = 512;    // of a block of the many-rows form
 constexpr int kMaxCluster = 8;
-constexpr int kRouteWarps = 8;  // tokens per block of the router's own launch
+constexpr int kRouteWarps = 16;      // of a block of the router's own launch
+constexpr int kBackWarps = 8;        // of a block of its gradient
+constexpr int kMaxBlocks = 256;      // of the many-rows form
+constexpr int kManyRows = 16384;     // rows from which it is taken
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -64,8 +71,9 @@ struct RouteParams {
 };
 
 // One token by one warp; V = ceil(E / 32) rounded up to a power of two.
+// Returns the lane's id (-1 from lane k on).
 template <typename T, int V>
-__device__ __forceinline__ void route_token(const RouteParams& p, int64_t t, int lane) {
+__device__ __forceinline__ int route_token(const RouteParams& p, int64_t t, int lane) {
   const T* row = static_cast<const T*>(p.logits) + t * p.ld;
   uint32_t key[V];
   uint32_t best = 0;
@@ -111,14 +119,9 @@ __device__ __forceinline__ void route_token(const RouteParams& p, int64_t t, int
   if (lane < p.k) {
     p.weights[t * p.k + lane] = empty ? 0.0f : w / total;
     p.ids[t * p.k + lane] = my_id;
+    return my_id;
   }
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + (threadIdx.x >> 5);
-  if (t < p.T) route_token<T, V>(p, t, threadIdx.x & 31);
+  return -1;
 }
 
 struct GroupParams {
@@ -126,29 +129,72 @@ struct GroupParams {
   int64_t M;
   int groups;
   int32_t *order, *position, *offsets;
+  // many-rows form: counts[block][groups + 1] of runs of rows_per_block rows
+  int32_t* counts;
+  int64_t rows_per_block;
+  int blocks;
 };
 
-// Places of the rows of one cluster's batch.  smem: [warps][G + 1] counts, then [G + 1] CTA totals, [G + 1] first
-// places, [32] warp sums of the scan.
-__device__ __forceinline__ void group_cluster(const GroupParams& p, int32_t* smem) {
+// Many tokens: the block routes a run of tokens and counts their experts.
+template <typename T, int V>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteParams p, const GroupParams g) {
+  __shared__ int32_t counts[TBIK_MAX_GROUPS];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int e = threadIdx.x; e < p.E; e += kRouteWarps * 32) counts[e] = 0;
+  __syncthreads();
+  const int64_t tokens = g.rows_per_block / p.k, t0 = static_cast<int64_t>(blockIdx.x) * tokens;
+  const int64_t t1 = t0 + tokens < p.T ? t0 + tokens : p.T;
+  for (int64_t t = t0 + (threadIdx.x >> 5); t < t1; t += kRouteWarps) {
+    const int id = route_token<T, V>(p, t, threadIdx.x & 31);
+    if (id >= 0) atomicAdd(&counts[id], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e <= p.E; e += kRouteWarps * 32)
+    g.counts[static_cast<int64_t>(blockIdx.x) * (p.E + 1) + e] = e < p.E ? counts[e] : 0;
+}
+
+// The same counts for ids that are given.
+__global__ void __launch_bounds__(kManyThreads) count_kernel(const GroupParams p) {
+  __shared__ int32_t counts[TBIK_MAX_GROUPS + 1];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int e = threadIdx.x; e <= p.groups; e += kManyThreads) counts[e] = 0;
+  __syncthreads();
+  const int64_t r0 = blockIdx.x * p.rows_per_block, r1 = r0 + p.rows_per_block < p.M ? r0 + p.rows_per_block : p.M;
+  for (int64_t i = r0 + threadIdx.x; i < r1; i += kManyThreads) {
+    const int id = p.ids[i];
+    atomicAdd(&counts[id < 0 || id >= p.groups ? p.groups : id], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e <= p.groups; e += kManyThreads) p.counts[static_cast<int64_t>(blockIdx.x) * (p.groups + 1) + e] = counts[e];
+}
+
+// Places of the rows of the batch.  smem: [warps][G + 1] counts, then [G + 1] totals of the block, [G + 1] rows before,
+// [G + 1] first places, [32] warp sums of the scan.
+template <bool MANY>
+__device__ __forceinline__ void group_block(const GroupParams& p, int32_t* smem) {
+  constexpr int THREADS = MANY ? kManyThreads : kGroupThreads, WARPS = THREADS / 32;
   cg::cluster_group cluster = cg::this_cluster();
-  const int nb = static_cast<int>(cluster.num_blocks());
-  const int rank = static_cast<int>(cluster.block_rank());
+  const int nb = MANY ? p.blocks : static_cast<int>(cluster.num_blocks());
+  const int rank = MANY ? static_cast<int>(blockIdx.x) : static_cast<int>(cluster.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int B = p.groups + 1;  // the last bucket: rows of no group
   int32_t* counts = smem;
-  int32_t* totals = smem + kGroupWarps * B;
-  int32_t* first = totals + B;
+  int32_t* totals = smem + WARPS * B;
+  int32_t* earlier = totals + B;
+  int32_t* first = earlier + B;
   int32_t* sums = first + B;
-  for (int i = threadIdx.x; i < kGroupWarps * B; i += kGroupThreads) counts[i] = 0;
+  for (int i = threadIdx.x; i < WARPS * B + 2 * B; i += THREADS) counts[i] = 0;
   __syncthreads();
 
-  const int64_t per_warp = ((p.M + nb * kGroupWarps - 1) / (nb * kGroupWarps) + 31) / 32 * 32;
-  const int64_t row0 = (static_cast<int64_t>(rank) * kGroupWarps + warp) * per_warp;
-  const int64_t row1 = row0 + per_warp < p.M ? row0 + per_warp : p.M;
+  const int64_t per_block = MANY ? p.rows_per_block : (p.M + nb - 1) / nb;
+  const int64_t per_warp = ((per_block + WARPS - 1) / WARPS + 31) / 32 * 32;
+  const int64_t run0 = MANY ? rank * per_block : rank * per_warp * WARPS;  // the block's run of rows
+  const int64_t run1 = MANY ? (run0 + per_block < p.M ? run0 + per_block : p.M) : p.M;
+  const int64_t row0 = run0 + warp * per_warp;
+  const int64_t row1 = row0 + per_warp < run1 ? row0 + per_warp : run1;
   int32_t* mine = counts + warp * B;
   constexpr int U = 4;  // steps whose ids are requested together
-  // walk(f): f(row, bucket, lanes of the step with the same bucket, lanes with a row) for every row of this warp, 32 at a time
+  // walk(f): f(row, bucket, whether the lane has a row), 32 rows at a time, by all lanes
   auto walk = [&](auto&& f) {
     for (int64_t r = row0; r < row1; r += 32 * U) {
       int32_t id[U];
@@ -160,43 +206,65 @@ __device__ __forceinline__ void group_cluster(const GroupParams& p, int32_t* sme
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int64_t i = r + u * 32 + lane;
-        const unsigned live = __ballot_sync(0xFFFFFFFFu, i < row1);
-        if (i < row1) {
-          const int b = (id[u] < 0 || id[u] >= p.groups) ? p.groups : id[u];
-          f(i, b, __match_any_sync(live, b), live);
-        }
-        __syncwarp();
+        if (r + u * 32 < row1) f(i, (id[u] < 0 || id[u] >= p.groups) ? p.groups : id[u], i < row1);
       }
     }
   };
-  walk([&](int64_t, int b, unsigned peers, unsigned) {
-    if (lane == __ffs(peers) - 1) mine[b] += __popc(peers);
+  walk([&](int64_t, int b, bool live) {
+    if (live) atomicAdd(&mine[b], 1);
   });
+  if constexpr (MANY) {
+    // counts of the other blocks: a warp adds up its share of the blocks, 32 groups at a time
+    for (int b0 = 0; b0 < B; b0 += 32) {
+      const int b = b0 + lane;
+      int all = 0, before = 0;
+      if (b < B) {
+#pragma unroll 8
+        for (int k = warp; k < nb; k += WARPS) {
+          const int v = __ldcg(p.counts + static_cast<int64_t>(k) * B + b);
+          all += v;
+          before += k < rank ? v : 0;
+        }
+        atomicAdd(&totals[b], all);
+        atomicAdd(&earlier[b], before);
+      }
+    }
+  }
   __syncthreads();
-  for (int b = threadIdx.x; b < B; b += kGroupThreads) {
+  const int64_t longest = min(MANY ? per_block : per_warp * WARPS, p.M);  // rows of a block at most
+  const int used = per_warp > 0 ? static_cast<int>((longest + per_warp - 1) / per_warp) : 0;  // warps that can have rows
+  for (int b = threadIdx.x; b < B; b += THREADS) {
     int32_t run = 0;
-    for (int w = 0; w < kGroupWarps; ++w) {
+    for (int w = 0; w < used; ++w) {
       const int32_t c = counts[w * B + b];
       counts[w * B + b] = run;
       run += c;
     }
-    totals[b] = run;
+    if constexpr (!MANY) totals[b] = run;
   }
-  cluster.sync();
-  // scan over the buckets: thread t holds buckets 2t and 2t + 1
-  int32_t all[2] = {0, 0}, before[2] = {0, 0};
+  if constexpr (MANY) __syncthreads(); else cluster.sync();
+  // scan over the buckets, PER of them per thread
+  constexpr int PER = (TBIK_MAX_GROUPS + 1 + THREADS - 1) / THREADS;
+  int32_t all[PER], before[PER], run = 0;
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int b = 2 * static_cast<int>(threadIdx.x) + u;
+  for (int u = 0; u < PER; ++u) {
+    const int b = PER * static_cast<int>(threadIdx.x) + u;
+    all[u] = before[u] = 0;
     if (b < B) {
-      for (int c = 0; c < nb; ++c) {
-        const int32_t v = cluster.map_shared_rank(totals, c)[b];
-        all[u] += v;
-        if (c < rank) before[u] += v;
+      if constexpr (MANY) {
+        all[u] = totals[b];
+        before[u] = earlier[b];
+      } else {
+        for (int c = 0; c < nb; ++c) {
+          const int32_t v = cluster.map_shared_rank(totals, c)[b];
+          all[u] += v;
+          if (c < rank) before[u] += v;
+        }
       }
     }
+    run += all[u];
   }
-  int32_t run = all[0] + all[1];
+  int32_t start = -run;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int32_t v = __shfl_up_sync(0xFFFFFFFFu, run, o);
@@ -204,51 +272,57 @@ __device__ __forceinline__ void group_cluster(const GroupParams& p, int32_t* sme
   }
   if (lane == 31) sums[warp] = run;
   __syncthreads();
-  if (warp == 0) {
-    int32_t s = sums[lane];
+  start += run;
+  for (int w = 0; w < warp; ++w) start += sums[w];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int32_t v = __shfl_up_sync(0xFFFFFFFFu, s, o);
-      if (lane >= o) s += v;
-    }
-    sums[lane] = s;
-  }
-  __syncthreads();
-  int32_t start = run - all[0] - all[1] + (warp > 0 ? sums[warp - 1] : 0);
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int b = 2 * static_cast<int>(threadIdx.x) + u;
+  for (int u = 0; u < PER; ++u) {
+    const int b = PER * static_cast<int>(threadIdx.x) + u;
     if (b < B) {
       first[b] = start + before[u];
       if (rank == 0) p.offsets[b] = start;
     }
     start += all[u];
   }
-  cluster.sync();  // nobody leaves while its totals may still be read; also publishes `first` to the block
-  walk([&](int64_t i, int b, unsigned peers, unsigned live) {
-    const int32_t at = first[b] + mine[b] + __popc(peers & ((1u << lane) - 1u));
-    __syncwarp(live);  // everyone has read the count before it moves on
-    if (lane == __ffs(peers) - 1) mine[b] += __popc(peers);
-    p.order[at] = static_cast<int32_t>(i);
-    p.position[i] = at;
+  if constexpr (MANY) __syncthreads(); else cluster.sync();  // nobody leaves while its totals may still be read
+  const int bits = 32 - __clz(p.groups);  // of a bucket's number
+  walk([&](int64_t i, int b, bool live) {
+    unsigned peers = __ballot_sync(0xFFFFFFFFu, live);
+    for (int k = 0; k < bits; ++k) {
+      const unsigned set = __ballot_sync(0xFFFFFFFFu, (b >> k) & 1);
+      peers &= (b >> k) & 1 ? set : ~set;
+    }
+    int at = 0;
+    if (live) at = first[b] + mine[b] + __popc(peers & ((1u << lane) - 1u));
+    __syncwarp();  // everyone has read the count before it moves on
+    if (live && lane == __ffs(peers) - 1) mine[b] += __popc(peers);
+    __syncwarp();
+    if (live) {
+      p.order[at] = static_cast<int32_t>(i);
+      p.position[i] = at;
+    }
   });
 }
 
 __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupParams p) {
   extern __shared__ int32_t group_smem[];
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the router's ids, when this launch follows it
-  group_cluster(p, group_smem);
+  group_block<false>(p, group_smem);
+}
+
+__global__ void __launch_bounds__(kManyThreads) group_many_kernel(const GroupParams p) {
+  extern __shared__ int32_t group_smem[];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the ids and counts of the launch before
+  group_block<true>(p, group_smem);
 }
 
 // Few tokens: router and grouping in one launch of one cluster.
 template <typename T, int V>
 __global__ void __launch_bounds__(kGroupThreads) route_group_kernel(const RouteParams r, const GroupParams p) {
   extern __shared__ int32_t group_smem[];
-  const int warps = gridDim.x * kGroupWarps;
-  for (int64_t t = blockIdx.x * kGroupWarps + (threadIdx.x >> 5); t < r.T; t += warps) route_token<T, V>(r, t, threadIdx.x & 31);
+  constexpr int WARPS = kGroupThreads / 32;
+  for (int64_t t = blockIdx.x * WARPS + (threadIdx.x >> 5); t < r.T; t += gridDim.x * WARPS) (void)route_token<T, V>(r, t, threadIdx.x & 31);
   __threadfence();
   cg::this_cluster().sync();
-  group_cluster(p, group_smem);
+  group_block<false>(p, group_smem);
 }
 
 struct RouteBackParams {
@@ -266,10 +340,10 @@ struct RouteBackParams {
 // is the weight, everything else gets 0) or all E.  One warp per token; the chosen experts' terms meet in a row of
 // shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_backward_kernel(const RouteBackParams p) {
-  __shared__ float rows[kRouteWarps][TBIK_MAX_GROUPS];
+__global__ void __launch_bounds__(kBackWarps * 32) route_backward_kernel(const RouteBackParams p) {
+  __shared__ float rows[kBackWarps][TBIK_MAX_GROUPS];
   const int lane = threadIdx.x & 31;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + (threadIdx.x >> 5);
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kBackWarps + (threadIdx.x >> 5);
   if (t >= p.T) return;
   float* s = rows[threadIdx.x >> 5];
   for (int e = lane; e < p.E; e += 32) s[e] = 0.0f;
@@ -302,41 +376,52 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_backward_kernel(const 
 }
 
 // ---------------------------------------------------------------- host side
-constexpr int kDevices = 64;
+size_t group_smem_bytes(int groups, int threads) { return (static_cast<size_t>(threads / 32 + 3) * (groups + 1) + 32) * sizeof(int32_t); }
 
-size_t group_smem_bytes(int groups) { return (static_cast<size_t>(kGroupWarps + 2) * (groups + 1) + 32) * sizeof(int32_t); }
-
-// CTAs of the cluster: one per 2048 rows, at most 8.  Few rows are done sooner without the cluster's barriers.
+// CTAs of the cluster: one per 1024 rows, at most 8.  Few rows are done sooner without the cluster's barriers.
 int cluster_size(int64_t M) {
   int c = 1;
-  while (c < kMaxCluster && M > 2048 * c) c *= 2;
+  while (c < kMaxCluster && M > 1024 * c) c *= 2;
   return c;
 }
 
+// Launches `kernel` on `blocks` blocks: as one cluster, or (after) as a plain grid that may start while the launch before
+// it still runs and waits for it itself.
 template <typename... Params>
-int launch_cluster(void (*kernel)(Params...), const char* what, int ctas, size_t smem, bool after, cudaStream_t stream,
-                   const Params&... params) {
-  // the attribute belongs to (kernel, device); setting it again is cheap and idempotent
+int launch_groups(void (*kernel)(Params...), const char* what, int blocks, int threads, size_t smem, bool after, cudaStream_t stream,
+                  const Params&... params) {
   if (smem > 48 * 1024) {
+    // belongs to (kernel, device); setting it again is cheap and idempotent
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return set_cuda_error(e, what);
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-  cfg.blockDim = dim3(kGroupThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[1];
+  if (after) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+  } else {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(blocks);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = after ? 2 : 1;
+  cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, params...);
   return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, what);
+}
+
+// Blocks of the many-rows form: runs of whole multiples of `unit` rows, at least 64, at most kMaxBlocks of them.
+void many_blocks(GroupParams* g, int64_t unit) {
+  int64_t per = (g->M + kMaxBlocks - 1) / kMaxBlocks;
+  if (per < 64) per = 64;
+  g->rows_per_block = (per + unit - 1) / unit * unit;
+  g->blocks = static_cast<int>((g->M + g->rows_per_block - 1) / g->rows_per_block);
 }
 
 int check_group(int64_t M, int groups, const void* ids, const void* order, const void* position, const void* offsets,
@@ -348,18 +433,20 @@ int check_group(int64_t M, int groups, const void* ids, const void* order, const
 }
 
 template <typename T, int V>
-int route_launch(const RouteParams& r, const GroupParams& g, cudaStream_t stream) {
-  const size_t smem = group_smem_bytes(g.groups);
-  // One launch while the cluster's 32 warps per CTA take at most two tokens each; beyond that the router gets the GPU.
-  const int ctas = cluster_size(g.M);
-  int fused = ctas;
-  while (fused < kMaxCluster && r.T > 2 * fused * kGroupWarps) fused *= 2;
-  if (r.T <= 2 * fused * kGroupWarps)
-    return launch_cluster(route_group_kernel<T, V>, "route_group_kernel launch", fused, smem, false, stream, r, g);
-  route_kernel<T, V><<<static_cast<unsigned>((r.T + kRouteWarps - 1) / kRouteWarps), kRouteWarps * 32, 0, stream>>>(r);
+int route_launch(const RouteParams& r, GroupParams g, cudaStream_t stream) {
+  if (g.M < kManyRows && r.T <= 4 * kMaxCluster * (kGroupThreads / 32)) {
+    // one launch: the cluster's warps take four tokens each at most
+    int ctas = cluster_size(g.M);
+    while (ctas < kMaxCluster && r.T > ctas * (kGroupThreads / 32)) ctas *= 2;
+    return launch_groups(route_group_kernel<T, V>, "route_group_kernel launch", ctas, kGroupThreads,
+                         group_smem_bytes(g.groups, kGroupThreads), false, stream, r, g);
+  }
+  many_blocks(&g, r.k);
+  route_kernel<T, V><<<static_cast<unsigned>(g.blocks), kRouteWarps * 32, 0, stream>>>(r, g);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "route_kernel launch");
-  return launch_cluster(group_kernel, "group_kernel launch", ctas, smem, true, stream, g);
+  return launch_groups(group_many_kernel, "group_many_kernel launch", g.blocks, kManyThreads, group_smem_bytes(g.groups, kManyThreads),
+                       true, stream, g);
 }
 
 template <typename T>
@@ -381,26 +468,56 @@ int check_route(int64_t T, int E, int k, int dtype) {
   return TBIK_OK;
 }
 
+int check_workspace(int64_t M, int groups, const void* workspace, size_t bytes) {
+  if (!workspace || bytes < group_workspace_bytes(M, groups) || (reinterpret_cast<uintptr_t>(workspace) & 3u))
+    return set_error(TBIK_ERR_ARG, "tbik_group_rows / tbik_route_topk: workspace of tbik_group_workspace_bytes() bytes needed");
+  return TBIK_OK;
+}
+
 }  // namespace
 
-int group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets,
-               cudaStream_t stream) {
+size_t group_workspace_bytes(int64_t M, int groups) {
+  // the router's runs are whole tokens and no shorter than these
+  if (M < 1 || groups < 1 || groups > TBIK_MAX_GROUPS) return 0;
+  GroupParams g{};
+  g.M = M;
+  many_blocks(&g, 1);
+  return static_cast<size_t>(g.blocks) * (groups + 1) * sizeof(int32_t);
+}
+
+int group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets, void* workspace,
+               size_t workspace_bytes, cudaStream_t stream) {
   const int rc = check_group(M, groups, ids, order, position, offsets,
                              "tbik_group_rows: 1 .. 1024 groups, 0 .. 2^31 - 1 rows, no null pointers");
   if (rc != TBIK_OK) return rc;
-  const GroupParams g{ids, M, groups, order, position, offsets};
-  return launch_cluster(group_kernel, "group_kernel launch", cluster_size(M), group_smem_bytes(groups), false, stream, g);
+  GroupParams g{ids, M, groups, order, position, offsets, static_cast<int32_t*>(workspace), 0, 0};
+  if (M < kManyRows)
+    return launch_groups(group_kernel, "group_kernel launch", cluster_size(M), kGroupThreads, group_smem_bytes(groups, kGroupThreads),
+                         false, stream, g);
+  const int rc2 = check_workspace(M, groups, workspace, workspace_bytes);
+  if (rc2 != TBIK_OK) return rc2;
+  many_blocks(&g, 1);
+  count_kernel<<<static_cast<unsigned>(g.blocks), kManyThreads, 0, stream>>>(g);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error(e, "count_kernel launch");
+  return launch_groups(group_many_kernel, "group_many_kernel launch", g.blocks, kManyThreads, group_smem_bytes(groups, kManyThreads),
+                       true, stream, g);
 }
 
 int route_topk(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize, float* weights,
-               int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, cudaStream_t stream) {
+               int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, void* workspace, size_t workspace_bytes,
+               cudaStream_t stream) {
   int rc = check_route(T, E, k, dtype);
   if (rc != TBIK_OK) return rc;
   rc = check_group(T * k, E, ids, order, position, offsets, "tbik_route_topk: null pointer");
   if (rc != TBIK_OK) return rc;
   if (T > 0 && (!logits || !weights)) return set_error(TBIK_ERR_ARG, "tbik_route_topk: null pointer");
+  if (T > 0) {
+    rc = check_workspace(T * k, E, workspace, workspace_bytes);
+    if (rc != TBIK_OK) return rc;
+  }
   const RouteParams r{logits, ld, T, E, k, renormalize, weights, ids};
-  const GroupParams g{ids, T * k, E, order, position, offsets};
+  const GroupParams g{ids, T * k, E, order, position, offsets, static_cast<int32_t*>(workspace), 0, 0};
   if (dtype == TBIK_DTYPE_BF16) return route_width<__nv_bfloat16>(r, g, stream);
   if (dtype == TBIK_DTYPE_FP16) return route_width<__half>(r, g, stream);
   return route_width<float>(r, g, stream);
@@ -413,10 +530,10 @@ int route_topk_backward(const void* logits, int64_t ld, int64_t T, int E, int k,
   if (rc != TBIK_OK || T == 0) return rc;
   if (!logits || !weights || !ids || !dweights || !dlogits) return set_error(TBIK_ERR_ARG, "tbik_route_topk_backward: null pointer");
   const RouteBackParams p{logits, ld, T, E, k, renormalize, weights, ids, dweights, dlogits, ldd};
-  const unsigned grid = static_cast<unsigned>((T + kRouteWarps - 1) / kRouteWarps);
-  if (dtype == TBIK_DTYPE_BF16) route_backward_kernel<__nv_bfloat16><<<grid, kRouteWarps * 32, 0, stream>>>(p);
-  else if (dtype == TBIK_DTYPE_FP16) route_backward_kernel<__half><<<grid, kRouteWarps * 32, 0, stream>>>(p);
-  else route_backward_kernel<float><<<grid, kRouteWarps * 32, 0, stream>>>(p);
+  const unsigned grid = static_cast<unsigned>((T + kBackWarps - 1) / kBackWarps);
+  if (dtype == TBIK_DTYPE_BF16) route_backward_kernel<__nv_bfloat16><<<grid, kBackWarps * 32, 0, stream>>>(p);
+  else if (dtype == TBIK_DTYPE_FP16) route_backward_kernel<__half><<<grid, kBackWarps * 32, 0, stream>>>(p);
+  else route_backward_kernel<float><<<grid, kBackWarps * 32, 0, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, "route_backward_kernel launch");
 }

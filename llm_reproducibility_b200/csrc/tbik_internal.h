@@ -49,10 +49,12 @@ int ar_graph_meta(tbik_ar_t h, void* handles_out, int64_t* offsets_out);
 int ar_register_graph_buffers(tbik_ar_t h, const void* const* handles, const int64_t* const* offsets);
 int ar_status(tbik_ar_t h, uint32_t out[8]);
 
-int group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets,
-               cudaStream_t stream);
+size_t group_workspace_bytes(int64_t M, int groups);
+int group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets, void* workspace,
+               size_t workspace_bytes, cudaStream_t stream);
 int route_topk(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize, float* weights,
-               int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, cudaStream_t stream);
+               int32_t* ids, int32_t* order, int32_t* position, int32_t* offsets, void* workspace, size_t workspace_bytes,
+               cudaStream_t stream);
 int route_topk_backward(const void* logits, int64_t ld, int64_t T, int E, int k, int dtype, int renormalize,
                         const float* weights, const int32_t* ids, const float* dweights, void* dlogits, int64_t ldd,
                         cudaStream_t stream);

@@ -67,11 +67,13 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
-def _empty_groups(M: int, groups: int, device: torch.device) -> RowGroups:
-    # one allocation; the three parts start on 16-byte boundaries
-    pad = (M + 3) // 4 * 4
-    buf = torch.empty(2 * pad + groups + 1, dtype=torch.int32, device=device)
-    return RowGroups(buf[:M], buf[pad:pad + M], buf[2 * pad:])
+def _empty_groups(M: int, groups: int, device: torch.device):
+    """An empty RowGroups and the kernels' workspace (pointer, bytes): one allocation, parts on 16-byte boundaries."""
+    pad, table = (M + 3) // 4 * 4, (groups + 4) // 4 * 4
+    nbytes = _lib.lib().tbik_group_workspace_bytes(M, groups)
+    buf = torch.empty(2 * pad + table + nbytes // 4, dtype=torch.int32, device=device)
+    g = RowGroups(buf[:M], buf[pad:pad + M], buf[2 * pad:2 * pad + groups + 1])
+    return g, buf.data_ptr() + 4 * (2 * pad + table), nbytes
 
 
 def _check_groups(num_groups: int) -> None:
@@ -89,9 +91,9 @@ def group_rows(ids: torch.Tensor, num_groups: int) -> RowGroups:
         raise ValueError("group_rows: fewer than 2^31 rows")
     dev = need_cuda("group_rows", ids)
     ids = ids.contiguous()
-    g = _empty_groups(ids.numel(), num_groups, dev)
+    g, ws, nbytes = _empty_groups(ids.numel(), num_groups, dev)
     rc = on_device(dev, lambda stream: _lib.lib().tbik_group_rows(
-        ids.data_ptr(), ids.numel(), num_groups, g.order.data_ptr(), g.position.data_ptr(), g.offsets.data_ptr(), stream))
+        ids.data_ptr(), ids.numel(), num_groups, g.order.data_ptr(), g.position.data_ptr(), g.offsets.data_ptr(), ws, nbytes, stream))
     if rc != 0:
         _lib.check(rc, "tbik_group_rows")
     return g
@@ -130,10 +132,10 @@ def _route(logits: torch.Tensor, k: int, renormalize: bool) -> Routing:
     dev = logits.device
     weights = torch.empty((T, k), dtype=torch.float32, device=dev)
     ids = torch.empty((T, k), dtype=torch.int32, device=dev)
-    g = _empty_groups(T * k, E, dev)
+    g, ws, nbytes = _empty_groups(T * k, E, dev)
     rc = on_device(dev, lambda stream: _lib.lib().tbik_route_topk(
         logits.data_ptr(), logits.stride(0), T, E, k, _LOGITS_CODE[logits.dtype], int(renormalize), weights.data_ptr(),
-        ids.data_ptr(), g.order.data_ptr(), g.position.data_ptr(), g.offsets.data_ptr(), stream))
+        ids.data_ptr(), g.order.data_ptr(), g.position.data_ptr(), g.offsets.data_ptr(), ws, nbytes, stream))
     if rc != 0:
         _lib.check(rc, "tbik_route_topk")
     return Routing(weights, ids, g)

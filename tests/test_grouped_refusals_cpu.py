@@ -153,11 +153,15 @@ def test_c_abi_refuses_before_any_launch():
     assert L.tbik_grouped_gemm_wgrad(p, p, p, p, 4, 8, 16, 2, 4, 16, 0, 0, 0, None) == -2
     assert L.tbik_grouped_gemm_wgrad(p, p, p, p, 4, 8, 16, 2, 8, 17, 0, 0, 0, None) == -4
     assert L.tbik_grouped_gemm_wgrad(p, p, p, p, 4, 8, 16, 2, 8, 16, 0, 1, 0, None) == -3
-    assert L.tbik_group_rows(p, 4, 0, p, p, p, None) == -2 and L.tbik_group_rows(None, 4, 2, p, p, p, None) == -1
-    assert L.tbik_group_rows(p, 4, 2, p, p, None, None) == -1 and L.tbik_group_rows(p, -1, 2, p, p, p, None) == -2
-    assert L.tbik_route_topk(p, 8, 4, 8, 9, 0, 1, p, p, p, p, p, None) == -2
-    assert L.tbik_route_topk(p, 8, 4, 8, 2, 7, 1, p, p, p, p, p, None) == -3
-    assert L.tbik_route_topk(None, 8, 4, 8, 2, 0, 1, p, p, p, p, p, None) == -1
+    assert L.tbik_group_rows(p, 4, 0, p, p, p, p, 99, None) == -2 and L.tbik_group_rows(None, 4, 2, p, p, p, p, 99, None) == -1
+    assert L.tbik_group_rows(p, 4, 2, p, p, None, p, 99, None) == -1 and L.tbik_group_rows(p, -1, 2, p, p, p, p, 99, None) == -2
+    need = L.tbik_group_workspace_bytes(1 << 20, 128)
+    assert need > 0 and L.tbik_group_rows(p, 1 << 20, 128, p, p, p, p, need - 1, None) == -1
+    assert L.tbik_group_rows(p, 1 << 20, 128, p, p, p, None, need, None) == -1 and "workspace" in _lib.last_error()
+    assert L.tbik_route_topk(p, 8, 4, 8, 2, 0, 1, p, p, p, p, p, None, 0, None) == -1
+    assert L.tbik_route_topk(p, 8, 4, 8, 9, 0, 1, p, p, p, p, p, p, 999, None) == -2
+    assert L.tbik_route_topk(p, 8, 4, 8, 2, 7, 1, p, p, p, p, p, p, 999, None) == -3
+    assert L.tbik_route_topk(None, 8, 4, 8, 2, 0, 1, p, p, p, p, p, p, 999, None) == -1
     assert L.tbik_route_topk_backward(p, 8, 4, 8, 2, 0, 1, p, p, None, p, 8, None) == -1
     assert L.tbik_route_topk_backward(p, 8, 0, 8, 2, 0, 1, None, None, None, None, 8, None) == 0
     base = [p, 64, p, 24, p, 24, p, p, p, None, p, p, 4, 24, 64, 8, 3, 0, 0, None]
