@@ -1,8 +1,15 @@
 // Rows grouped by id (a stable counting sort) and the router that produces the ids.
 //
-// Router: one warp per token.  The token's E scores sit in registers, element e in lane e % 32; each of k rounds takes the
-// largest key over the warp and, among equal keys, the lowest index (two warp-wide integer reductions).  A score's key
-// is its bit pattern made monotone, so the order is total and exact whatever the type.  Softmax statistics are fp32.
+// Router.  A score's key is its bit pattern made monotone, with the expert's number below it, so keys are all different,
+// larger score first, equal scores by lower number: one maximum gives value and expert, exact whatever the type.  16-bit
+// scores make 32-bit keys, fp32 scores 64-bit ones.
+//   k <= 8   up to 32 lanes per token, eight keys each at a time.  A lane sorts its eight in registers (a bitonic network),
+//            then lists meet pairwise: of two descending lists a, b the larger of a[i], b[7-i] are the best eight, in bitonic
+//            order.  No round depends on the one before.  The merges are a loop, not unrolled code: these are kernels of a
+//            few microseconds, and fetching a large body costs more than it saves (16384 tokens, 128 experts, k = 8: k rounds
+//            of a warp-wide maximum 18.6 us, sixteen keys per lane fully unrolled 12.1 us).
+//   else     one warp per token, k rounds of two warp-wide integer reductions.
+// Softmax statistics are fp32.
 //
 // Grouping: rows are dealt to warps in contiguous runs.  Every warp counts its rows per group, the counts are turned into
 // first places -- over the warps of a block, over the blocks, over the groups with a scan -- and a second walk over the same
@@ -32,9 +39,9 @@ namespace cg = cooperative_groups;
 constexpr int kGroupThreads = 1024;  // of a CTA of the cluster form
 constexpr int kManyThreads = 512;    // of a block of the many-rows form
 constexpr int kMaxCluster = 8;
-constexpr int kRouteWarps = 16;      // of a block of the router's own launch
+constexpr int kRouteWarps = 32;      // of a block of the router's own launch
 constexpr int kBackWarps = 8;        // of a block of its gradient
-constexpr int kMaxBlocks = 256;      // of the many-rows form
+constexpr int kMaxBlocks = 128;      // of the many-rows form: every block reads all blocks' counts
 constexpr int kManyRows = 16384;     // rows from which it is taken
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -56,6 +63,19 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
 
+// The same in 16 bits for 16-bit scores (their upper half of the fp32 pattern would not do for fp16).
+template <typename T> __device__ __forceinline__ uint32_t key16(float v) {
+  if (v != v) return 0xFFFFu;
+  const T h = from_float<T>(v + 0.0f);
+  const uint32_t u = *reinterpret_cast<const uint16_t*>(&h);
+  return (u & 0x8000u) ? (~u & 0xFFFFu) : (u | 0x8000u);
+}
+template <typename T> __device__ __forceinline__ float value16(uint32_t key) {
+  if (key == 0xFFFFu) return __uint_as_float(0x7FC00000u);
+  const uint16_t u = static_cast<uint16_t>((key & 0x8000u) ? (key & 0x7FFFu) : ~key);
+  return to_float(*reinterpret_cast<const T*>(&u));
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
@@ -68,6 +88,8 @@ struct RouteParams {
   int E, k, renormalize;
   float* weights;
   int32_t* ids;
+  int aligned;  // rows start on 16-byte boundaries and E is a multiple of 8
+  int lanes;    // k <= 8: lanes per token, a power of two
 };
 
 // One token by one warp; V = ceil(E / 32) rounded up to a power of two.
@@ -124,6 +146,164 @@ __device__ __forceinline__ int route_token(const RouteParams& p, int64_t t, int 
   return -1;
 }
 
+// ---- a few lanes per token
+template <typename T> struct Key { using type = uint32_t; };
+template <> struct Key<float> { using type = unsigned long long; };
+
+template <typename T>
+__device__ __forceinline__ typename Key<T>::type packed_key(float v, int e) {
+  if constexpr (sizeof(T) == 2) return (key16<T>(v) << 16) | static_cast<uint32_t>(0xFFFF - e);
+  else return (static_cast<unsigned long long>(key_of(v)) << 32) | static_cast<uint32_t>(~e);
+}
+
+template <typename K>
+__device__ __forceinline__ void order2(K& a, K& b) {  // larger first
+  const K hi = a > b ? a : b, lo = a > b ? b : a;
+  a = hi;
+  b = lo;
+}
+
+// Bitonic list of N to descending order.
+template <int N, typename K>
+__device__ __forceinline__ void bitonic_merge(K* v) {
+#pragma unroll
+  for (int d = N / 2; d > 0; d /= 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & d) == 0) order2(v[i], v[i + d]);
+  }
+}
+
+// Eight keys in any order to descending order.
+template <typename K>
+__device__ __forceinline__ void sort8(K* v) {
+#pragma unroll
+  for (int size = 2; size <= 8; size *= 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((i ^ (size - 1)) > i) order2(v[i], v[i ^ (size - 1)]);
+#pragma unroll
+    for (int d = size / 4; d > 0; d /= 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if ((i & d) == 0) order2(v[i], v[i + d]);
+    }
+  }
+}
+
+// One token by p.lanes neighbouring lanes, k <= 8; live: the token exists (dead lanes shuffle along).  Lane l holds the
+// experts 8 l .. 8 l + 7, and the same again 8 p.lanes further where there are more than 256.
+template <typename T>
+__device__ __forceinline__ void route_few(const RouteParams& p, int64_t t, bool live, int lane, int32_t* counts) {
+  using K = typename Key<T>::type;
+  const int l = lane & (p.lanes - 1), stride = 8 * p.lanes;
+  const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+  auto load = [&](int e, float (&x)[8]) {  // -inf where there is none
+    if (p.aligned) {                       // pieces of eight are whole and on 16-byte boundaries
+      alignas(16) T v[8];
+      if (live && e < p.E) {
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(sizeof(T)) / 2; ++j)
+          reinterpret_cast<uint4*>(v)[j] = __ldg(reinterpret_cast<const uint4*>(row + e) + j);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = live && e < p.E ? to_float(v[j]) : -INFINITY;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = live && e + j < p.E ? to_float(row[e + j]) : -INFINITY;
+    }
+  };
+  // the best eight of two descending lists
+  auto merge = [](K (&a)[8], const K (&b)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = a[i] > b[7 - i] ? a[i] : b[7 - i];
+    bitonic_merge<8>(a);
+  };
+  float x[8];
+  K best[8];
+#pragma unroll 1
+  for (int e0 = 0; e0 < p.E; e0 += stride) {
+    const int e = e0 + 8 * l;
+    load(e, x);
+    K key[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) key[j] = live && e + j < p.E ? packed_key<T>(x[j], e + j) : K(0);
+    sort8(key);
+    if (e0 == 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) best[j] = key[j];
+    } else {
+      merge(best, key);
+    }
+  }
+#pragma unroll 1
+  for (int d = 1; d < p.lanes; d *= 2) {
+    K other[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) other[i] = __shfl_xor_sync(0xFFFFFFFFu, best[i], d);
+    merge(best, other);
+  }
+  // every lane of the token holds the whole list
+  auto value = [](K k) {
+    if constexpr (sizeof(T) == 2) return value16<T>(k >> 16); else return value_of(static_cast<uint32_t>(k >> 32));
+  };
+  const float peak = value(best[0]);
+  const bool empty = peak == -INFINITY;  // every expert masked
+  float w[8], total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    w[i] = i < p.k && !empty ? expf(value(best[i]) - peak) : 0.0f;
+    total += w[i];
+  }
+  if (!p.renormalize) {
+    total = 0.0f;
+#pragma unroll 1
+    for (int e0 = 0; e0 < p.E; e0 += stride) {
+      const int e = e0 + 8 * l;
+      if (stride < p.E) load(e, x);  // else x still holds them
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (e + j < p.E) total += expf(x[j] - peak);
+    }
+    for (int d = 1; d < p.lanes; d *= 2) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+  }
+  if (!live) return;
+#pragma unroll 1
+  for (int i = l; i < p.k; i += p.lanes) {  // the lanes share the writing
+    K mine = best[0];
+    float wi = w[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) {
+      mine = i == j ? best[j] : mine;
+      wi = i == j ? w[j] : wi;
+    }
+    int e;
+    if constexpr (sizeof(T) == 2) e = static_cast<int>(0xFFFFu - (mine & 0xFFFFu)); else e = static_cast<int>(~static_cast<uint32_t>(mine));
+    p.weights[t * p.k + i] = empty ? 0.0f : wi / total;
+    p.ids[t * p.k + i] = e;
+    if (counts) atomicAdd(&counts[e], 1);
+  }
+}
+
+// The tokens t0 .. t1 - 1 by `warps` warps.  V = 0: k <= 8; else one warp per token with V keys per lane.
+template <typename T, int V>
+__device__ __forceinline__ void route_run(const RouteParams& p, int64_t t0, int64_t t1, int warp, int warps, int lane, int32_t* counts) {
+  if constexpr (V == 0) {
+    const int tokens = 32 / p.lanes;
+#pragma unroll 1
+    for (int64_t t = t0 + warp * tokens; t < t1; t += warps * tokens) {
+      const int64_t mine = t + lane / p.lanes;
+      route_few<T>(p, mine, mine < t1, lane, counts);
+    }
+  } else {
+#pragma unroll 1
+    for (int64_t t = t0 + warp; t < t1; t += warps) {
+      const int id = route_token<T, V>(p, t, lane);
+      if (counts && id >= 0) atomicAdd(&counts[id], 1);
+    }
+  }
+}
+
 struct GroupParams {
   const int32_t* ids;
   int64_t M;
@@ -144,10 +324,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RoutePara
   __syncthreads();
   const int64_t tokens = g.rows_per_block / p.k, t0 = static_cast<int64_t>(blockIdx.x) * tokens;
   const int64_t t1 = t0 + tokens < p.T ? t0 + tokens : p.T;
-  for (int64_t t = t0 + (threadIdx.x >> 5); t < t1; t += kRouteWarps) {
-    const int id = route_token<T, V>(p, t, threadIdx.x & 31);
-    if (id >= 0) atomicAdd(&counts[id], 1);
-  }
+  route_run<T, V>(p, t0, t1, threadIdx.x >> 5, kRouteWarps, threadIdx.x & 31, counts);
   __syncthreads();
   for (int e = threadIdx.x; e <= p.E; e += kRouteWarps * 32)
     g.counts[static_cast<int64_t>(blockIdx.x) * (p.E + 1) + e] = e < p.E ? counts[e] : 0;
@@ -214,16 +391,28 @@ __device__ __forceinline__ void group_block(const GroupParams& p, int32_t* smem)
     if (live) atomicAdd(&mine[b], 1);
   });
   if constexpr (MANY) {
-    // counts of the other blocks: a warp adds up its share of the blocks, 32 groups at a time
-    for (int b0 = 0; b0 < B; b0 += 32) {
-      const int b = b0 + lane;
+    // counts of the other blocks: a warp takes 32 groups and its share of the blocks, sixteen rows in flight
+    const int chunks = (B + 31) / 32, shares = chunks < WARPS ? WARPS / chunks : 1;
+    for (int c = warp; c < chunks * shares; c += WARPS) {
+      const int b = c / shares * 32 + lane;
       int all = 0, before = 0;
       if (b < B) {
-#pragma unroll 8
-        for (int k = warp; k < nb; k += WARPS) {
-          const int v = __ldcg(p.counts + static_cast<int64_t>(k) * B + b);
-          all += v;
-          before += k < rank ? v : 0;
+        const int32_t* from = p.counts + b;
+        // every block starts elsewhere: all of them want the same rows
+        const int share = c % shares, n = (nb - share + shares - 1) / shares, k0 = rank % n;
+        for (int i = 0; i < n; i += 16) {
+          int v[16];
+#pragma unroll
+          for (int u = 0; u < 16; ++u) {
+            const int k = i + u + k0 < n ? i + u + k0 : i + u + k0 - n;
+            v[u] = i + u < n ? __ldcg(from + static_cast<int64_t>(share + k * shares) * B) : 0;
+          }
+#pragma unroll
+          for (int u = 0; u < 16; ++u) {
+            const int k = i + u + k0 < n ? i + u + k0 : i + u + k0 - n;
+            all += v[u];
+            before += share + k * shares < rank ? v[u] : 0;
+          }
         }
         atomicAdd(&totals[b], all);
         atomicAdd(&earlier[b], before);
@@ -319,7 +508,7 @@ template <typename T, int V>
 __global__ void __launch_bounds__(kGroupThreads) route_group_kernel(const RouteParams r, const GroupParams p) {
   extern __shared__ int32_t group_smem[];
   constexpr int WARPS = kGroupThreads / 32;
-  for (int64_t t = blockIdx.x * WARPS + (threadIdx.x >> 5); t < r.T; t += gridDim.x * WARPS) (void)route_token<T, V>(r, t, threadIdx.x & 31);
+  route_run<T, V>(r, 0, r.T, blockIdx.x * WARPS + (threadIdx.x >> 5), gridDim.x * WARPS, threadIdx.x & 31, nullptr);
   __threadfence();
   cg::this_cluster().sync();
   group_block<false>(p, group_smem);
@@ -434,10 +623,12 @@ int check_group(int64_t M, int groups, const void* ids, const void* order, const
 
 template <typename T, int V>
 int route_launch(const RouteParams& r, GroupParams g, cudaStream_t stream) {
-  if (g.M < kManyRows && r.T <= 4 * kMaxCluster * (kGroupThreads / 32)) {
-    // one launch: the cluster's warps take four tokens each at most
+  constexpr int WARPS = kGroupThreads / 32;
+  const int tokens = V == 0 ? 32 / r.lanes : 1;  // of a warp at a time
+  if (g.M < kManyRows && r.T <= 4 * kMaxCluster * WARPS * tokens) {
+    // one launch: the cluster's warps go round four times at most
     int ctas = cluster_size(g.M);
-    while (ctas < kMaxCluster && r.T > ctas * (kGroupThreads / 32)) ctas *= 2;
+    while (ctas < kMaxCluster && r.T > ctas * WARPS * tokens) ctas *= 2;
     return launch_groups(route_group_kernel<T, V>, "route_group_kernel launch", ctas, kGroupThreads,
                          group_smem_bytes(g.groups, kGroupThreads), false, stream, r, g);
   }
@@ -451,10 +642,8 @@ int route_launch(const RouteParams& r, GroupParams g, cudaStream_t stream) {
 
 template <typename T>
 int route_width(const RouteParams& r, const GroupParams& g, cudaStream_t stream) {
-  if (r.E <= 32) return route_launch<T, 1>(r, g, stream);
-  if (r.E <= 64) return route_launch<T, 2>(r, g, stream);
+  if (r.k <= 8) return route_launch<T, 0>(r, g, stream);
   if (r.E <= 128) return route_launch<T, 4>(r, g, stream);
-  if (r.E <= 256) return route_launch<T, 8>(r, g, stream);
   if (r.E <= 512) return route_launch<T, 16>(r, g, stream);
   return route_launch<T, 32>(r, g, stream);
 }
@@ -516,7 +705,11 @@ int route_topk(const void* logits, int64_t ld, int64_t T, int E, int k, int dtyp
     rc = check_workspace(T * k, E, workspace, workspace_bytes);
     if (rc != TBIK_OK) return rc;
   }
-  const RouteParams r{logits, ld, T, E, k, renormalize, weights, ids};
+  const int es = dtype == TBIK_DTYPE_FP32 ? 4 : 2;
+  const int aligned = E % 8 == 0 && ld * es % 16 == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0;
+  int lanes = 1;
+  while (lanes < 32 && lanes * 8 < E) lanes *= 2;
+  const RouteParams r{logits, ld, T, E, k, renormalize, weights, ids, aligned, lanes};
   const GroupParams g{ids, T * k, E, order, position, offsets, static_cast<int32_t*>(workspace), 0, 0};
   if (dtype == TBIK_DTYPE_BF16) return route_width<__nv_bfloat16>(r, g, stream);
   if (dtype == TBIK_DTYPE_FP16) return route_width<__half>(r, g, stream);
