@@ -34,10 +34,8 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kLeaves = 8;
-constexpr uint32_t kStageBytes = 49152;  // one of the two buffers of a staged leaf
-constexpr uint64_t kWaitNs = 2000000000ull;
-
-__device__ uint32_t g_adapters_status[4];
+// One of the two buffers of a staged leaf: four CTAs per SM for the usual ranks, more columns at a time for the large ones.
+__host__ __device__ constexpr uint32_t stage_bytes(int R) { return R <= 32 ? 24576 : 49152; }
 
 struct Params {
   const void *x, *y, *A, *B;
@@ -50,6 +48,9 @@ struct Params {
   int cluster;     // CTAs per item
   int rest;        // rows of no adapter have work to do too (copy y, or zero h)
 };
+
+template <bool B> struct Bool { static constexpr bool value = B; };
+template <int I> struct Int { static constexpr int value = I; };
 
 template <typename T> struct Half;
 template <> struct Half<__nv_bfloat16> {
@@ -74,17 +75,18 @@ template <> struct Half<__half> {
   }
 };
 
-TBIK_DEVICE void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar) : "memory");
+TBIK_DEVICE void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)) : "memory");
 }
+TBIK_DEVICE void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> TBIK_DEVICE void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 TBIK_DEVICE void prefetch_l2(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(src)), "r"(bytes) : "memory");
 }
 
 TBIK_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Shared memory: [rows TM][item 4][barriers 2][abort][row factors TM] | leaf sums [8 / cluster][TM][R] | h [TM][R] |
+// Shared memory: [rows TM][item 4][row factors TM] | leaf sums [8 / cluster][TM][R] | h [TM][R] |
 // h as operand [MT][ceil(R / 16)][32 lanes] x 32 bytes | two staging buffers
 struct Layout {
   uint32_t sums, h, frags, stage, total;
@@ -97,20 +99,18 @@ __host__ __device__ inline Layout layout(int R, int cluster) {
   l.h = l.sums + (kLeaves / cluster) * TM * R * 4;
   l.frags = l.h + TM * R * 4;
   l.stage = (l.frags + MT * ((R + 15) / 16) * 1024 + 127) / 128 * 128;
-  l.total = l.stage + (STAGED ? 2 * kStageBytes : 0);
+  l.total = l.stage + (STAGED ? 2 * stage_bytes(R) : 0);
   return l;
 }
 
 template <typename T, int MT, bool STAGED>
-__global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(const Params p) {
   constexpr int TM = MT * 16;
   extern __shared__ __align__(128) uint8_t smem[];
   const Layout lay = layout<MT, STAGED>(p.R, p.cluster);
   int* rows = reinterpret_cast<int*>(smem);                 // row index or -1
   int* item = rows + TM;                                    // adapter, first place, rows
   float* factor = reinterpret_cast<float*>(smem + 256);     // what a row of h was divided by (fp16)
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + 240);
-  const uint32_t bars = smem_u32(smem + 224);
   float* sums = reinterpret_cast<float*>(smem + lay.sums);
   float* hs = reinterpret_cast<float*>(smem + lay.h);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -118,11 +118,7 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
   const int R = p.R, K = p.K;
 
   if (tid == 0) {
-    *abort_flag = 0u;
     item[0] = -2;
-    mbar_init(bars, 1);
-    mbar_init(bars + 8, 1);
-    fence_mbar_init();
   }
   // ---- which adapter and rows: tiles of the groups in order, then tiles of the rows of no adapter
   {
@@ -219,46 +215,64 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
     const T* x = static_cast<const T*>(p.x);
     const int own = kLeaves / C;  // leaves of this CTA
     const int ntiles = R / 8;
+    if (STAGED && expand && warp == 1) {
+      // this CTA's share of B and of the rows of y is wanted right after: on its way to L2 meanwhile
+      const int per = ceil_div(nblocks, C) * 32, n0 = min(rank * per, p.N), n1 = min(n0 + per, p.N);
+      if (lane == 0 && n1 > n0) prefetch_l2(B + static_cast<int64_t>(n0) * R, static_cast<uint32_t>(n1 - n0) * R * 2);
+      if (lane < TM && n1 > n0 && rows[lane] >= 0)
+        prefetch_l2(static_cast<const T*>(p.y) + static_cast<int64_t>(rows[lane]) * p.ldy + n0, static_cast<uint32_t>(n1 - n0) * 2);
+    }
     if constexpr (STAGED) {
-      // columns per buffer, a multiple of 32; a row's pitch is 64 bytes off a multiple of 128, so that the 16-byte pieces
-      // that 8 lanes read together lie in different banks
-      const int cols = min(static_cast<int>((kStageBytes / (R + TM) - 64) / 128 * 64), (p.leaf + 63) / 64 * 64);
-      const uint32_t pitch = static_cast<uint32_t>(cols) * 2 + 64;
-      const int per_leaf = ceil_div(p.leaf, cols), steps = own * per_leaf;
-      if (expand && warp == 1) {
-        // this CTA's share of B and of the rows of y is wanted right after: on its way to L2 meanwhile
-        const int per = ceil_div(nblocks, C) * 32, n0 = min(rank * per, p.N), n1 = min(n0 + per, p.N);
-        if (lane == 0 && n1 > n0) prefetch_l2(B + static_cast<int64_t>(n0) * R, static_cast<uint32_t>(n1 - n0) * R * 2);
-        if (lane < TM && n1 > n0 && rows[lane] >= 0)
-          prefetch_l2(static_cast<const T*>(p.y) + static_cast<int64_t>(rows[lane]) * p.ldy + n0, static_cast<uint32_t>(n1 - n0) * 2);
-      }
+      // A buffer holds `cols` columns of the adapter's R rows and of the tile's `count` rows: the whole leaf where it fits in
+      // both buffers together, else alternating halves.  A row's pitch is 64 bytes off a multiple of 128, so that the
+      // 16-byte pieces that 8 lanes read together lie in different banks.
+      const uint32_t stage = stage_bytes(R), lines = static_cast<uint32_t>(R + count);
+      const int whole = (p.leaf + 63) / 64 * 64;
+      const bool once = lines * (static_cast<uint32_t>(whole) * 2 + 64) <= 2 * stage;
+      const int cols = once ? whole : static_cast<int>((stage / lines - 64) / 128 * 64);
+      const uint32_t pitch = static_cast<uint32_t>(cols) * 2 + 64, second = once ? 0u : stage;
+      const int per_leaf = ceil_div(p.leaf, cols), steps = own * per_leaf, ahead = once ? 1 : 2;
       auto range = [&](int s, int& k0, int& k1) {
         const int l = rank * own + s / per_leaf;
         const int64_t b = static_cast<int64_t>(l) * p.leaf, e = min(b + p.leaf, static_cast<int64_t>(K));
         const int64_t f = min(b + static_cast<int64_t>(s % per_leaf) * cols, e);
         k0 = static_cast<int>(f);
-        k1 = static_cast<int>(min(f + cols, e));
+        k1 = max(static_cast<int>(min(f + cols, e)), k0);
       };
-      auto load = [&](int s) {  // warp 0
+      // A warp per row, 16 bytes per lane; one group of asynchronous copies per step, empty or not.
+      auto load = [&](int s) {
         int k0, k1;
         range(s, k0, k1);
-        if (k1 <= k0) return;
-        const uint32_t bytes = static_cast<uint32_t>(k1 - k0) * 2, buf = smem_u32(smem + lay.stage) + (s & 1) * kStageBytes, bar = bars + 8 * (s & 1);
-        int live = 0;
-        for (int i = 0; i < TM; ++i) live += rows[i] >= 0 ? 1 : 0;
-        if (lane == 0) mbar_arrive_expect_tx(bar, bytes * static_cast<uint32_t>(R + live));
-        __syncwarp();
-        for (int r = lane; r < R; r += 32) bulk_load(buf + r * pitch, A + static_cast<int64_t>(r) * K + k0, bytes, bar);
-        if (lane < TM && rows[lane] >= 0)
-          bulk_load(buf + (R + lane) * pitch, x + static_cast<int64_t>(rows[lane]) * p.ldx + k0, bytes, bar);
+        const uint32_t buf = smem_u32(smem + lay.stage) + (s & 1) * second;
+        for (int i = warp; i < R + count; i += kWarps) {
+          const int t = i < R ? 0 : rows[i - R];
+          if (t < 0) continue;
+          const T* src = (i < R ? A + static_cast<int64_t>(i) * K : x + static_cast<int64_t>(t) * p.ldx) + k0;
+          for (int k = lane * 8; k < k1 - k0; k += 256) copy16(buf + i * pitch + k * 2, src + k);
+        }
+        copy_commit();
       };
-      if (warp == 0) {
-        load(0);
-        if (steps > 1) load(1);
-      }
+      load(0);
+      if (ahead == 2 && steps > 1) load(1);
+      // Rows of the instruction beyond the tile repeat its last one: a row's results depend on no other row, and theirs are
+      // not read.  Columns between the end of K and the next multiple of 32 are cleared below.
+      const int row0 = R + min(g, count - 1), row1 = R + min(g + 8, count - 1);
       float acc[2][4];  // this warp's column tiles: warp, warp + 8
-      uint32_t used[2] = {0u, 0u};
-      bool dead = false;
+      auto chain = [&](const uint8_t* buf, int n, auto two) {
+        const uint8_t *x0 = buf + row0 * pitch + c * 16, *x1 = buf + row1 * pitch + c * 16, *b0 = buf + (warp * 8 + g) * pitch + c * 16;
+#pragma unroll 4
+        for (int k = 0; k < n; k += 32) {
+          const uint4 a0 = *reinterpret_cast<const uint4*>(x0 + k * 2), a1 = *reinterpret_cast<const uint4*>(x1 + k * 2);
+          const uint4 b = *reinterpret_cast<const uint4*>(b0 + k * 2);
+          Half<T>::mma(acc[0], make_uint4(a0.x, a1.x, a0.y, a1.y), b.x, b.y);
+          Half<T>::mma(acc[0], make_uint4(a0.z, a1.z, a0.w, a1.w), b.z, b.w);
+          if constexpr (decltype(two)::value) {
+            const uint4 d = *reinterpret_cast<const uint4*>(b0 + 64 * pitch + k * 2);
+            Half<T>::mma(acc[1], make_uint4(a0.x, a1.x, a0.y, a1.y), d.x, d.y);
+            Half<T>::mma(acc[1], make_uint4(a0.z, a1.z, a0.w, a1.w), d.z, d.w);
+          }
+        }
+      };
       for (int s = 0; s < steps; ++s) {
         int k0, k1;
         range(s, k0, k1);
@@ -268,53 +282,29 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
         }
-        if (k1 > k0) {
-          // after a wait that ran out the warp keeps step with the barriers and computes on what is there
-          if (!dead && !mbar_wait_bounded(bars + 8 * (s & 1), used[s & 1] & 1u, abort_flag, kWaitNs)) dead = true;
-          ++used[s & 1];
-          const uint8_t* buf = smem + lay.stage + (s & 1) * kStageBytes;
-          const uint8_t* x0 = buf + (R + g) * pitch + c * 16;
-          const bool r0 = rows[g] >= 0, r1 = rows[g + 8] >= 0;
-          const int n = k1 - k0;
-          if (warp < ntiles) {
-#pragma unroll 4
-            for (int k = 0; k < n; k += 32) {
-              const bool in = k + c * 8 < n;
-              const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-              const uint4 a0 = in && r0 ? *reinterpret_cast<const uint4*>(x0 + k * 2) : zero;
-              const uint4 a1 = in && r1 ? *reinterpret_cast<const uint4*>(x0 + 8 * pitch + k * 2) : zero;
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                if (warp + 8 * i < ntiles) {
-                  const uint4 b = in ? *reinterpret_cast<const uint4*>(buf + ((warp + 8 * i) * 8 + g) * pitch + c * 16 + k * 2) : zero;
-                  Half<T>::mma(acc[i], make_uint4(a0.x, a1.x, a0.y, a1.y), b.x, b.y);
-                  Half<T>::mma(acc[i], make_uint4(a0.z, a1.z, a0.w, a1.w), b.z, b.w);
-                }
-              }
-            }
-          }
-        }
+        if (ahead == 2 && s + 1 < steps) copy_wait<1>(); else copy_wait<0>();
+        uint8_t* buf = smem + lay.stage + (s & 1) * second;
+        const int n = k1 - k0, pad = (32 - n % 32) % 32 / 8;  // 16-byte pieces to clear per row
+        if (pad > 0)
+          for (int i = tid; i < (R + count) * pad; i += kThreads)
+            *reinterpret_cast<uint4*>(buf + i / pad * pitch + n * 2 + i % pad * 16) = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+        if (warp + 8 < ntiles) chain(buf, n, Bool<true>{});
+        else if (warp < ntiles) chain(buf, n, Bool<false>{});
         if ((s + 1) % per_leaf == 0) {
           float* out = sums + (s / per_leaf) * TM * R;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int n = (warp + 8 * i) * 8 + c * 2;
+            const int n8 = (warp + 8 * i) * 8 + c * 2;
             if (warp + 8 * i < ntiles) {
-              *reinterpret_cast<float2*>(out + g * R + n) = make_float2(acc[i][0], acc[i][1]);
-              *reinterpret_cast<float2*>(out + (g + 8) * R + n) = make_float2(acc[i][2], acc[i][3]);
+              *reinterpret_cast<float2*>(out + g * R + n8) = make_float2(acc[i][0], acc[i][1]);
+              *reinterpret_cast<float2*>(out + (g + 8) * R + n8) = make_float2(acc[i][2], acc[i][3]);
             }
           }
         }
-        if (s + 2 < steps) {
+        if (s + ahead < steps) {
           __syncthreads();  // everyone is done with the buffer
-          if (warp == 0 && !dead) load(s + 2);
-        }
-      }
-      if (dead) {
-        g_adapters_status[1] = blockIdx.x;
-        g_adapters_status[0] = 1u;
-        const uint64_t t0 = global_timer_ns();  // copies in flight get time to land
-        while (global_timer_ns() - t0 < 200000ull) {
+          load(s + ahead);
         }
       }
     } else {
@@ -322,12 +312,10 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
       const int leaf = rank * own + warp / C, part = warp % C;
       const int64_t kb = min(static_cast<int64_t>(leaf) * p.leaf, static_cast<int64_t>(K));
       const int k0 = static_cast<int>(kb), k1 = static_cast<int>(min(kb + p.leaf, static_cast<int64_t>(K)));
+      // rows and column tiles beyond what there is repeat the last one; their results are not read
       const T* xr[2 * MT];
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) {
-        const int t = rows[i * 8 + g];
-        xr[i] = t >= 0 ? x + static_cast<int64_t>(t) * p.ldx + c * 8 : nullptr;
-      }
+      for (int i = 0; i < 2 * MT; ++i) xr[i] = x + static_cast<int64_t>(max(rows[min(i * 8 + g, count - 1)], 0)) * p.ldx + c * 8;
       float* out = sums + (warp / C) * TM * R;
       for (int n0 = part; n0 < ntiles; n0 += 4 * C) {
         float acc[MT][4][4];
@@ -337,27 +325,28 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
           for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
-        const T* ar = A + static_cast<int64_t>(n0 * 8 + g) * K + c * 8;
-        const int64_t a_step = static_cast<int64_t>(C) * 8 * K;
-#pragma unroll 2
-        for (int k = k0; k < k1; k += 32) {
-          const bool in = k + c * 8 < k1;
-          const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        const T* ar[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ar[i] = A + static_cast<int64_t>(min(n0 + i * C, ntiles - 1) * 8 + g) * K + c * 8;
+        auto step = [&](int k, bool in) {
           uint4 a[2 * MT], b[4];
 #pragma unroll
-          for (int i = 0; i < 2 * MT; ++i) a[i] = in && xr[i] ? __ldg(reinterpret_cast<const uint4*>(xr[i] + k)) : zero;
+          for (int i = 0; i < 2 * MT; ++i) a[i] = in ? __ldg(reinterpret_cast<const uint4*>(xr[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            b[i] = in && n0 + i * C < ntiles ? __ldg(reinterpret_cast<const uint4*>(ar + i * a_step + k)) : zero;
+          for (int i = 0; i < 4; ++i) b[i] = in ? __ldg(reinterpret_cast<const uint4*>(ar[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              Half<T>::mma(acc[m][i], make_uint4(a[2 * m].x, a[2 * m + 1].x, a[2 * m].y, a[2 * m + 1].y), b[i].x, b[i].y);
-              Half<T>::mma(acc[m][i], make_uint4(a[2 * m].z, a[2 * m + 1].z, a[2 * m].w, a[2 * m + 1].w), b[i].z, b[i].w);
-            }
-          }
-        }
+            for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].x, a[2 * m + 1].x, a[2 * m].y, a[2 * m + 1].y), b[i].x, b[i].y);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].z, a[2 * m + 1].z, a[2 * m].w, a[2 * m + 1].w), b[i].z, b[i].w);
+        };
+        const int whole = k0 + (k1 - k0) / 32 * 32;
+#pragma unroll 2
+        for (int k = k0; k < whole; k += 32) step(k, true);
+        if (whole < k1) step(whole, whole + c * 8 < k1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (n0 + i * C < ntiles) {
@@ -370,6 +359,11 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
           }
         }
       }
+    }
+    if (!STAGED && expand && warp == 0 && lane < count && rows[lane] >= 0) {
+      // the rows of y are wanted next: on their way to L2 while the sums are joined
+      const int per = ceil_div(nblocks, C) * 32, n0 = min(rank * per, p.N), n1 = min(n0 + per, p.N);
+      if (n1 > n0) prefetch_l2(static_cast<const T*>(p.y) + static_cast<int64_t>(rows[lane]) * p.ldy + n0, static_cast<uint32_t>(n1 - n0) * 2);
     }
     // ---- the leaves' sums, from wherever in the cluster they are
     cg::cluster_group cluster = cg::this_cluster();
@@ -421,11 +415,15 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
     }
     __syncthreads();
   }
+  // Instruction s of a run of 16 columns of h: lane c's four columns.  Where R is a multiple of 32 the lane's columns of two
+  // instructions are 8 neighbours, so that its piece of a row of B is 16 bytes; else it is 8.
+  const bool wide = R % 32 == 0;
+  auto column = [&](int s, int at) { return wide ? 32 * (s >> 1) + 8 * at + 4 * (s & 1) : 16 * s + 4 * at; };
   uint4* frags = reinterpret_cast<uint4*>(smem + lay.frags);
   const int ksteps = (R + 15) / 16;
   for (int i = tid; i < MT * ksteps * 32; i += kThreads) {
     const int ln = i & 31, s = (i >> 5) % ksteps, m = (i >> 5) / ksteps;
-    const int r = 16 * s + 4 * (ln & 3);
+    const int r = column(s, ln & 3);
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {  // rows ln / 4 and + 8
@@ -455,59 +453,102 @@ __global__ void __launch_bounds__(kThreads, 2) adapters_kernel(const Params p) {
   const T* y = static_cast<const T*>(p.y);
   T* out = static_cast<T*>(p.out);
   const int per = ceil_div(nblocks, C), b1 = min((rank + 1) * per, nblocks);
-  for (int blk = rank * per + warp; blk < b1; blk += kWarps) {
-    const int col = blk * 32 + c * 8;  // the lane's 8 columns
-    const bool in = col < p.N;
-    uint4 yv[2 * MT];
+  int row[2 * MT];
+  [[maybe_unused]] float s_row[kScaled ? 2 * MT : 1];
 #pragma unroll
-    for (int i = 0; i < 2 * MT; ++i) {
-      const int t = rows[i * 8 + g];
-      if (in && t >= 0) yv[i] = *reinterpret_cast<const uint4*>(y + static_cast<int64_t>(t) * p.ldy + col);
-    }
-    float acc[MT][4][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
-    // column of B that this lane brings for instruction j: 8 (g / 2) + 2 j + g % 2
-    const int n0 = blk * 32 + 8 * (g >> 1) + (g & 1);
-    const T* br = B + static_cast<int64_t>(n0) * R + 4 * c;
-#pragma unroll 2
-    for (int s = 0; s < ksteps; ++s) {
-      uint2 b[4];
-      const bool ok = n0 < p.N && 16 * s + 4 * c < R;  // N is a multiple of 8: all four columns are in or out
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = ok ? __ldg(reinterpret_cast<const uint2*>(br + 2 * j * R + 16 * s)) : make_uint2(0u, 0u);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint4 hi = frags[2 * ((m * ksteps + s) * 32 + lane)], lo = frags[2 * ((m * ksteps + s) * 32 + lane) + 1];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          Half<T>::mma(acc[m][j], hi, b[j].x, b[j].y);
-          Half<T>::mma(acc[m][j], lo, b[j].x, b[j].y);
-        }
-      }
-    }
-    if (in) {
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) {
-        const int t = rows[i * 8 + g];
-        if (t < 0) continue;
-        float s = scale;
-        if constexpr (kScaled) s = scale / factor[i * 8 + g];  // a power of two: exact
-        const uint32_t yw[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
-        uint32_t o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float d0 = acc[i >> 1][j][2 * (i & 1)], d1 = acc[i >> 1][j][2 * (i & 1) + 1];
-          o[j] = Half<T>::pack(fmaf(s, d0, Half<T>::f32(yw[j], 0)), fmaf(s, d1, Half<T>::f32(yw[j], 1)));
-        }
-        *reinterpret_cast<uint4*>(out + static_cast<int64_t>(t) * p.ldo + col) = make_uint4(o[0], o[1], o[2], o[3]);
-      }
-    }
+  for (int i = 0; i < 2 * MT; ++i) {
+    row[i] = i * 8 + g < count ? rows[i * 8 + g] : -1;
+    if constexpr (kScaled) s_row[i] = scale / factor[i * 8 + g];  // a power of two: exact
   }
+  // KS > 0: h has KS runs of 16 columns and stays in registers; 0: any number, read from shared memory.  WIDE as above.
+  auto product = [&](auto ks_, auto wide_) {
+    constexpr int KS = decltype(ks_)::value;
+    constexpr bool WIDE = decltype(wide_)::value;
+    uint4 hi[KS > 0 ? MT * KS : 1], lo[KS > 0 ? MT * KS : 1];
+    if constexpr (KS > 0) {
+#pragma unroll
+      for (int i = 0; i < MT * KS; ++i) {
+        hi[i] = frags[2 * (i * 32 + lane)];
+        lo[i] = frags[2 * (i * 32 + lane) + 1];
+      }
+    }
+    for (int blk = rank * per + warp; blk < b1; blk += kWarps) {
+      const int col = blk * 32 + c * 8;  // the lane's 8 columns
+      uint4 yv[2 * MT];
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i)
+        if (col < p.N && row[i] >= 0) yv[i] = *reinterpret_cast<const uint4*>(y + row[i] * p.ldy + col);
+      float acc[MT][4][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
+      // column of B that this lane brings for instruction j: 8 (g / 2) + 2 j + g % 2
+      const int n0 = blk * 32 + 8 * (g >> 1) + (g & 1);
+      const bool live = n0 < p.N;  // N is a multiple of 8: all four columns are in or out
+      const T* br = B + static_cast<int64_t>(live ? n0 : 0) * R;
+      auto multiply = [&](int s, const uint2 (&b)[4]) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int f = KS > 0 ? m * KS + s : 0;
+          uint4 h = hi[f], l = lo[f];
+          if constexpr (KS == 0) {
+            h = frags[2 * ((m * ksteps + s) * 32 + lane)];
+            l = frags[2 * ((m * ksteps + s) * 32 + lane) + 1];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) Half<T>::mma(acc[m][j], h, b[j].x, b[j].y);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) Half<T>::mma(acc[m][j], l, b[j].x, b[j].y);
+        }
+      };
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int s2 = 0; s2 < (KS > 0 ? KS / 2 : TBIK_MAX_RANK / 32); ++s2) {
+          if (KS == 0 && 2 * s2 >= ksteps) break;
+          uint4 w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(br + 2 * j * R + 32 * s2 + 8 * c));
+          const uint2 b0[4] = {{w[0].x, w[0].y}, {w[1].x, w[1].y}, {w[2].x, w[2].y}, {w[3].x, w[3].y}};
+          const uint2 b1_[4] = {{w[0].z, w[0].w}, {w[1].z, w[1].w}, {w[2].z, w[2].w}, {w[3].z, w[3].w}};
+          multiply(2 * s2, b0);
+          multiply(2 * s2 + 1, b1_);
+        }
+      } else {
+        constexpr int STEPS = KS > 0 ? KS : (TBIK_MAX_RANK + 15) / 16;
+#pragma unroll 2
+        for (int s = 0; s < STEPS; ++s) {
+          if (KS == 0 && s >= ksteps) break;
+          uint2 b[4];
+          const bool ok = 16 * s + 4 * c < R;  // R may end inside the run
+#pragma unroll
+          for (int j = 0; j < 4; ++j) b[j] = ok ? __ldg(reinterpret_cast<const uint2*>(br + 2 * j * R + 16 * s + 4 * c)) : make_uint2(0u, 0u);
+          multiply(s, b);
+        }
+      }
+      if (col < p.N) {
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) {
+          if (row[i] < 0) continue;
+          const float s = kScaled ? s_row[kScaled ? i : 0] : scale;
+          const uint32_t yw[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float d0 = acc[i >> 1][j][2 * (i & 1)], d1 = acc[i >> 1][j][2 * (i & 1) + 1];
+            o[j] = Half<T>::pack(fmaf(s, d0, Half<T>::f32(yw[j], 0)), fmaf(s, d1, Half<T>::f32(yw[j], 1)));
+          }
+          *reinterpret_cast<uint4*>(out + row[i] * p.ldo + col) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+    }
+  };
+  if (R == 32) product(Int<2>{}, Bool<true>{});
+  else if (wide) product(Int<0>{}, Bool<true>{});
+  else if (R <= 16) product(Int<1>{}, Bool<false>{});
+  else product(Int<0>{}, Bool<false>{});
 }
 
 // ---------------------------------------------------------------- host side
@@ -573,16 +614,6 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
   if (dtype == TBIK_DTYPE_BF16)
     return few ? launch<__nv_bfloat16, 1, true>(p, items, stream) : launch<__nv_bfloat16, 2, false>(p, items, stream);
   return few ? launch<__half, 1, true>(p, items, stream) : launch<__half, 2, false>(p, items, stream);
-}
-
-int adapters_status(uint32_t out[4]) {
-  cudaError_t e = cudaMemcpyFromSymbol(out, g_adapters_status, sizeof(uint32_t) * 4);
-  if (e != cudaSuccess) return set_cuda_error(e, "cudaMemcpyFromSymbol(g_adapters_status)");
-  if (out[0] != 0) {
-    const uint32_t zero[4] = {0, 0, 0, 0};
-    cudaMemcpyToSymbol(g_adapters_status, zero, sizeof(zero));
-  }
-  return TBIK_OK;
 }
 
 }  // namespace tbik

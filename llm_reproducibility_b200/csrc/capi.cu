@@ -2,8 +2,6 @@
 #include <stdio.h>
 #include <string.h>
 
-#include <initializer_list>
-
 #include "tbik_internal.h"
 
 namespace tbik {
@@ -87,12 +85,11 @@ int tbik_gemm_static(const void* A, const void* W, void* C, int M, int N, int K,
 int tbik_gemm_status(uint32_t out[4]) {
   if (!out) return tbik::set_error(TBIK_ERR_ARG, "tbik_gemm_status: null output pointer");
   int rc = tbik::gemm_status(out);
-  for (auto more : {tbik::grouped_status, tbik::adapters_status}) {
-    uint32_t words[4];
-    if (rc != TBIK_OK || out[0] != 0) break;
-    rc = more(words);
-    if (rc == TBIK_OK && words[0] != 0)
-      for (int i = 0; i < 3; ++i) out[i] = words[i];
+  if (rc == TBIK_OK && out[0] == 0) {
+    uint32_t grouped[4];
+    rc = tbik::grouped_status(grouped);
+    if (rc == TBIK_OK && grouped[0] != 0)
+      for (int i = 0; i < 3; ++i) out[i] = grouped[i];
   }
   return rc;
 }

@@ -64,7 +64,6 @@ int grouped_gemm(const void* A, const void* W, void* C, const int32_t* offsets, 
 int grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* offsets, int64_t M, int N, int K, int groups,
                        int64_t lddc, int64_t lda, int dtype, int out_dtype, int max_ctas, cudaStream_t stream);
 int grouped_status(uint32_t out[4]);
-int adapters_status(uint32_t out[4]);
 int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, const void* A, const void* B,
              const float* scales, float* h, const int32_t* order, const int32_t* offsets, int64_t T, int N, int K, int R,
              int adapters, int dtype, int leaf, cudaStream_t stream);
