@@ -50,7 +50,7 @@ struct Params {
 };
 
 template <bool B> struct Bool { static constexpr bool value = B; };
-template <int I> struct Int { static constexpr int value = I; };
+template <typename V> struct Four { V v[4]; };
 
 template <typename T> struct Half;
 template <> struct Half<__nv_bfloat16> {
@@ -58,7 +58,7 @@ template <> struct Half<__nv_bfloat16> {
   TBIK_DEVICE static uint32_t pack(float lo, float hi) { return Pack16<__nv_bfloat16>::from_f32(lo, hi); }
   TBIK_DEVICE static float round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
   TBIK_DEVICE static void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
   }
 };
@@ -70,7 +70,7 @@ template <> struct Half<__half> {
   TBIK_DEVICE static uint32_t pack(float lo, float hi) { return Pack16<__half>::from_f32(lo, hi); }
   TBIK_DEVICE static float round(float v) { return __half2float(__float2half_rn(v)); }
   TBIK_DEVICE static void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
   }
 };
@@ -80,6 +80,12 @@ TBIK_DEVICE void copy16(uint32_t dst, const void* src) {
 }
 TBIK_DEVICE void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> TBIK_DEVICE void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// A row is read 64 bytes at a time by lanes of eight rows: L2 is asked for the 256 bytes around at once.
+TBIK_DEVICE uint4 load_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 TBIK_DEVICE void prefetch_l2(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(src)), "r"(bytes) : "memory");
 }
@@ -91,26 +97,27 @@ TBIK_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
 struct Layout {
   uint32_t sums, h, frags, stage, total;
 };
-template <int MT, bool STAGED>
+template <int MT, int RG, bool STAGED>
 __host__ __device__ inline Layout layout(int R, int cluster) {
-  constexpr int TM = MT * 16;
+  constexpr int TM = RG * MT * 16;
   Layout l;
-  l.sums = 512;
+  l.sums = 1024;
   l.h = l.sums + (kLeaves / cluster) * TM * R * 4;
   l.frags = l.h + TM * R * 4;
-  l.stage = (l.frags + MT * ((R + 15) / 16) * 1024 + 127) / 128 * 128;
+  l.stage = (l.frags + RG * MT * ((R + 15) / 16) * 1024 + 127) / 128 * 128;
   l.total = l.stage + (STAGED ? 2 * stage_bytes(R) : 0);
   return l;
 }
 
-template <typename T, int MT, bool STAGED>
+// RG groups of warps, each with MT x 16 rows of the tile.
+template <typename T, int MT, int RG, bool STAGED>
 __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(const Params p) {
-  constexpr int TM = MT * 16;
+  constexpr int TM = RG * MT * 16, W = kWarps / RG;  // rows of the tile, warps of a group
   extern __shared__ __align__(128) uint8_t smem[];
-  const Layout lay = layout<MT, STAGED>(p.R, p.cluster);
+  const Layout lay = layout<MT, RG, STAGED>(p.R, p.cluster);
   int* rows = reinterpret_cast<int*>(smem);                 // row index or -1
   int* item = rows + TM;                                    // adapter, first place, rows
-  float* factor = reinterpret_cast<float*>(smem + 256);     // what a row of h was divided by (fp16)
+  float* factor = reinterpret_cast<float*>(smem + 512);     // what a row of h was divided by (fp16)
   float* sums = reinterpret_cast<float*>(smem + lay.sums);
   float* hs = reinterpret_cast<float*>(smem + lay.h);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -197,7 +204,15 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
       if (expand) {
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.y) + static_cast<int64_t>(t) * p.ldy);
         uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<int64_t>(t) * p.ldo);
-        for (int c = lane; c < p.N / 8; c += 32) dst[c] = src[c];
+        for (int c0 = lane; c0 < p.N / 8; c0 += 32 * 8) {  // eight pieces in flight
+          uint4 v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (c0 + u * 32 < p.N / 8) v[u] = src[c0 + u * 32];
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (c0 + u * 32 < p.N / 8) dst[c0 + u * 32] = v[u];
+        }
       } else {
         for (int r = lane; r < R; r += 32) p.h[static_cast<int64_t>(t) * R + r] = 0.0f;
       }
@@ -206,6 +221,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   }
 
   const int g = lane >> 2, c = lane & 3;  // the lane's row (and row + 8) and its place in a row
+  const int first_row = warp / W * (MT * 16), w = warp % W;  // of the warp's group of rows; its number there
   const int nblocks = ceil_div(p.N, 32);
   const T* B = static_cast<const T*>(p.B) + static_cast<int64_t>(adapter) * p.N * R;
 
@@ -308,16 +324,19 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
         }
       }
     } else {
-      // one leaf per C warps; a warp's column tiles are part, part + C, ... in runs of four
-      const int leaf = rank * own + warp / C, part = warp % C;
+      // A group's W warps take a leaf each, in turns, or share the column tiles of a leaf where the CTA has fewer leaves.  Two
+      // groups read the same rows of A at about the same time: the second finds them in L1.
+      const int parts = own < W ? W / own : 1, part = w % parts;
+      for (int slot = w / parts; slot < own; slot += W / parts) {
+      const int leaf = rank * own + slot;
       const int64_t kb = min(static_cast<int64_t>(leaf) * p.leaf, static_cast<int64_t>(K));
       const int k0 = static_cast<int>(kb), k1 = static_cast<int>(min(kb + p.leaf, static_cast<int64_t>(K)));
       // rows and column tiles beyond what there is repeat the last one; their results are not read
       const T* xr[2 * MT];
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) xr[i] = x + static_cast<int64_t>(max(rows[min(i * 8 + g, count - 1)], 0)) * p.ldx + c * 8;
-      float* out = sums + (warp / C) * TM * R;
-      for (int n0 = part; n0 < ntiles; n0 += 4 * C) {
+      for (int i = 0; i < 2 * MT; ++i) xr[i] = x + static_cast<int64_t>(max(rows[min(first_row + i * 8 + g, count - 1)], 0)) * p.ldx + c * 8;
+      float* out = sums + (slot * TM + first_row) * R;
+      for (int n0 = part; n0 < ntiles; n0 += 4 * parts) {
         float acc[MT][4][4];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -327,13 +346,15 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
             for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
         const T* ar[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ar[i] = A + static_cast<int64_t>(min(n0 + i * C, ntiles - 1) * 8 + g) * K + c * 8;
-        auto step = [&](int k, bool in) {
-          uint4 a[2 * MT], b[4];
+        for (int i = 0; i < 4; ++i) ar[i] = A + static_cast<int64_t>(min(n0 + i * parts, ntiles - 1) * 8 + g) * K + c * 8;
+        // `in`: the lane's piece of the run of 32 columns exists
+        auto load = [&](int k, bool in, uint4 (&a)[2 * MT], uint4 (&b)[4]) {
 #pragma unroll
-          for (int i = 0; i < 2 * MT; ++i) a[i] = in ? __ldg(reinterpret_cast<const uint4*>(xr[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
+          for (int i = 0; i < 2 * MT; ++i) a[i] = in ? load_stream(xr[i] + k) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
           for (int i = 0; i < 4; ++i) b[i] = in ? __ldg(reinterpret_cast<const uint4*>(ar[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        auto multiply = [&](const uint4 (&a)[2 * MT], const uint4 (&b)[4]) {
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -343,14 +364,22 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
 #pragma unroll
             for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].z, a[2 * m + 1].z, a[2 * m].w, a[2 * m + 1].w), b[i].z, b[i].w);
         };
-        const int whole = k0 + (k1 - k0) / 32 * 32;
-#pragma unroll 2
-        for (int k = k0; k < whole; k += 32) step(k, true);
-        if (whole < k1) step(whole, whole + c * 8 < k1);
+        // the next run is on its way while one is multiplied
+        uint4 a[2][2 * MT], b[2][4];
+        load(k0, k0 + c * 8 < k1, a[0], b[0]);
+#pragma unroll 1
+        for (int k = k0; k < k1; k += 64) {
+          if (k + 32 < k1) load(k + 32, k + 32 + c * 8 < k1, a[1], b[1]);
+          multiply(a[0], b[0]);
+          if (k + 32 < k1) {
+            if (k + 64 < k1) load(k + 64, k + 64 + c * 8 < k1, a[0], b[0]);
+            multiply(a[1], b[1]);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (n0 + i * C < ntiles) {
-            const int n = (n0 + i * C) * 8 + c * 2;
+          if (n0 + i * parts < ntiles) {
+            const int n = (n0 + i * parts) * 8 + c * 2;
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
               *reinterpret_cast<float2*>(out + (m * 16 + g) * R + n) = make_float2(acc[m][i][0], acc[m][i][1]);
@@ -359,11 +388,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
           }
         }
       }
-    }
-    if (!STAGED && expand && warp == 0 && lane < count && rows[lane] >= 0) {
-      // the rows of y are wanted next: on their way to L2 while the sums are joined
-      const int per = ceil_div(nblocks, C) * 32, n0 = min(rank * per, p.N), n1 = min(n0 + per, p.N);
-      if (n1 > n0) prefetch_l2(static_cast<const T*>(p.y) + static_cast<int64_t>(rows[lane]) * p.ldy + n0, static_cast<uint32_t>(n1 - n0) * 2);
+      }
     }
     // ---- the leaves' sums, from wherever in the cluster they are
     cg::cluster_group cluster = cg::this_cluster();
@@ -421,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   auto column = [&](int s, int at) { return wide ? 32 * (s >> 1) + 8 * at + 4 * (s & 1) : 16 * s + 4 * at; };
   uint4* frags = reinterpret_cast<uint4*>(smem + lay.frags);
   const int ksteps = (R + 15) / 16;
-  for (int i = tid; i < MT * ksteps * 32; i += kThreads) {
+  for (int i = tid; i < RG * MT * ksteps * 32; i += kThreads) {
     const int ln = i & 31, s = (i >> 5) % ksteps, m = (i >> 5) / ksteps;
     const int r = column(s, ln & 3);
     uint32_t hi[4], lo[4];
@@ -457,106 +482,155 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   [[maybe_unused]] float s_row[kScaled ? 2 * MT : 1];
 #pragma unroll
   for (int i = 0; i < 2 * MT; ++i) {
-    row[i] = i * 8 + g < count ? rows[i * 8 + g] : -1;
-    if constexpr (kScaled) s_row[i] = scale / factor[i * 8 + g];  // a power of two: exact
+    row[i] = first_row + i * 8 + g < count ? rows[first_row + i * 8 + g] : -1;
+    if constexpr (kScaled) s_row[i] = scale / factor[first_row + i * 8 + g];  // a power of two: exact
   }
-  // KS > 0: h has KS runs of 16 columns and stays in registers; 0: any number, read from shared memory.  WIDE as above.
-  auto product = [&](auto ks_, auto wide_) {
-    constexpr int KS = decltype(ks_)::value;
-    constexpr bool WIDE = decltype(wide_)::value;
-    uint4 hi[KS > 0 ? MT * KS : 1], lo[KS > 0 ? MT * KS : 1];
-    if constexpr (KS > 0) {
+  const uint4* mine = frags + 2 * (first_row / 16) * ksteps * 32;
+  auto load_y = [&](int blk, uint4 (&v)[2 * MT]) {
+    const int col = blk * 32 + c * 8;  // the lane's 8 columns
 #pragma unroll
-      for (int i = 0; i < MT * KS; ++i) {
-        hi[i] = frags[2 * (i * 32 + lane)];
-        lo[i] = frags[2 * (i * 32 + lane) + 1];
-      }
-    }
-    for (int blk = rank * per + warp; blk < b1; blk += kWarps) {
-      const int col = blk * 32 + c * 8;  // the lane's 8 columns
-      uint4 yv[2 * MT];
+    for (int i = 0; i < 2 * MT; ++i)
+      if (col < p.N && row[i] >= 0) v[i] = *reinterpret_cast<const uint4*>(y + row[i] * p.ldy + col);
+  };
+  // row of B, i.e. column of the result, that this lane brings for instruction j: 8 (g / 2) + 2 j + g % 2 (N is a multiple of 8:
+  // all four are in or out, and where they are out their results are not stored)
+  auto row_of_b = [&](int blk) {
+    const int n0 = blk * 32 + 8 * (g >> 1) + (g & 1);
+    return B + static_cast<int64_t>(n0 < p.N ? n0 : 0) * R;
+  };
+  auto load_wide = [&](int blk, int s2, uint4 (&v)[4]) {
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i)
-        if (col < p.N && row[i] >= 0) yv[i] = *reinterpret_cast<const uint4*>(y + row[i] * p.ldy + col);
-      float acc[MT][4][4];
+    for (int j = 0; j < 4; ++j) v[j] = __ldg(reinterpret_cast<const uint4*>(row_of_b(blk) + 2 * j * R + 32 * s2 + 8 * c));
+  };
+  auto load_narrow = [&](int blk, int s, uint2 (&v)[4]) {
+    const bool ok = 16 * s + 4 * c < R;  // R may end inside the run
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+    for (int j = 0; j < 4; ++j) v[j] = ok ? __ldg(reinterpret_cast<const uint2*>(row_of_b(blk) + 2 * j * R + 16 * s + 4 * c)) : make_uint2(0u, 0u);
+  };
+  // acc += rows 16 m .. of h, run s, times the four instructions' operands
+  auto multiply = [&](int m, int s, const uint2 (&v)[4], float (&acc)[4][4]) {
+    const uint4 hi = mine[2 * ((m * ksteps + s) * 32 + lane)], lo = mine[2 * ((m * ksteps + s) * 32 + lane) + 1];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j) Half<T>::mma(acc[j], hi, v[j].x, v[j].y);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
-      // column of B that this lane brings for instruction j: 8 (g / 2) + 2 j + g % 2
-      const int n0 = blk * 32 + 8 * (g >> 1) + (g & 1);
-      const bool live = n0 < p.N;  // N is a multiple of 8: all four columns are in or out
-      const T* br = B + static_cast<int64_t>(live ? n0 : 0) * R;
-      auto multiply = [&](int s, const uint2 (&b)[4]) {
+    for (int j = 0; j < 4; ++j) Half<T>::mma(acc[j], lo, v[j].x, v[j].y);
+  };
+  auto multiply_wide = [&](int m, int s2, const uint4 (&v)[4], float (&acc)[4][4]) {
+    const uint2 lo8[4] = {{v[0].x, v[0].y}, {v[1].x, v[1].y}, {v[2].x, v[2].y}, {v[3].x, v[3].y}};
+    const uint2 hi8[4] = {{v[0].z, v[0].w}, {v[1].z, v[1].w}, {v[2].z, v[2].w}, {v[3].z, v[3].w}};
+    multiply(m, 2 * s2, lo8, acc);
+    multiply(m, 2 * s2 + 1, hi8, acc);
+  };
+  auto finish = [&](int blk, int m, const uint4 (&yv)[2 * MT], const float (&acc)[4][4]) {
+    const int col = blk * 32 + c * 8;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const int f = KS > 0 ? m * KS + s : 0;
-          uint4 h = hi[f], l = lo[f];
-          if constexpr (KS == 0) {
-            h = frags[2 * ((m * ksteps + s) * 32 + lane)];
-            l = frags[2 * ((m * ksteps + s) * 32 + lane) + 1];
-          }
+    for (int u = 0; u < 2; ++u) {
+      const int i = 2 * m + u;
+      if (col >= p.N || row[i] < 0) continue;
+      const float s = kScaled ? s_row[kScaled ? i : 0] : scale;
+      const uint32_t yw[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
+      uint32_t o[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) Half<T>::mma(acc[m][j], h, b[j].x, b[j].y);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) Half<T>::mma(acc[m][j], l, b[j].x, b[j].y);
-        }
-      };
-      if constexpr (WIDE) {
-#pragma unroll
-        for (int s2 = 0; s2 < (KS > 0 ? KS / 2 : TBIK_MAX_RANK / 32); ++s2) {
-          if (KS == 0 && 2 * s2 >= ksteps) break;
-          uint4 w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(br + 2 * j * R + 32 * s2 + 8 * c));
-          const uint2 b0[4] = {{w[0].x, w[0].y}, {w[1].x, w[1].y}, {w[2].x, w[2].y}, {w[3].x, w[3].y}};
-          const uint2 b1_[4] = {{w[0].z, w[0].w}, {w[1].z, w[1].w}, {w[2].z, w[2].w}, {w[3].z, w[3].w}};
-          multiply(2 * s2, b0);
-          multiply(2 * s2 + 1, b1_);
-        }
-      } else {
-        constexpr int STEPS = KS > 0 ? KS : (TBIK_MAX_RANK + 15) / 16;
-#pragma unroll 2
-        for (int s = 0; s < STEPS; ++s) {
-          if (KS == 0 && s >= ksteps) break;
-          uint2 b[4];
-          const bool ok = 16 * s + 4 * c < R;  // R may end inside the run
-#pragma unroll
-          for (int j = 0; j < 4; ++j) b[j] = ok ? __ldg(reinterpret_cast<const uint2*>(br + 2 * j * R + 16 * s + 4 * c)) : make_uint2(0u, 0u);
-          multiply(s, b);
-        }
-      }
-      if (col < p.N) {
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-          if (row[i] < 0) continue;
-          const float s = kScaled ? s_row[kScaled ? i : 0] : scale;
-          const uint32_t yw[4] = {yv[i].x, yv[i].y, yv[i].z, yv[i].w};
-          uint32_t o[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float d0 = acc[i >> 1][j][2 * (i & 1)], d1 = acc[i >> 1][j][2 * (i & 1) + 1];
-            o[j] = Half<T>::pack(fmaf(s, d0, Half<T>::f32(yw[j], 0)), fmaf(s, d1, Half<T>::f32(yw[j], 1)));
-          }
-          *reinterpret_cast<uint4*>(out + row[i] * p.ldo + col) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
-      }
+      for (int j = 0; j < 4; ++j)
+        o[j] = Half<T>::pack(fmaf(s, acc[j][2 * u], Half<T>::f32(yw[j], 0)), fmaf(s, acc[j][2 * u + 1], Half<T>::f32(yw[j], 1)));
+      *reinterpret_cast<uint4*>(out + row[i] * p.ldo + col) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   };
-  if (R == 32) product(Int<2>{}, Bool<true>{});
-  else if (wide) product(Int<0>{}, Bool<true>{});
-  else if (R <= 16) product(Int<1>{}, Bool<false>{});
-  else product(Int<0>{}, Bool<false>{});
+  auto clear = [](float (&acc)[4][4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+  };
+  const int b0 = rank * per + w;
+  bool done = false;
+  if constexpr (!STAGED) {
+    if (R <= 16 || R == 32) {
+    // h in one load of B per trip: the next trip's y and B are on their way while one is multiplied
+    auto run = [&](auto load_b, auto times, auto sample) {
+      uint4 yv[2][2 * MT];
+      decltype(sample) bv[2];
+      auto trip = [&](int blk, int at) {
+        if (blk + W < b1) {
+          load_y(blk + W, yv[1 - at]);
+          load_b(blk + W, bv[1 - at].v);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          float acc[4][4];
+          clear(acc);
+          times(m, bv[at].v, acc);
+          finish(blk, m, yv[at], acc);
+        }
+      };
+      if (b0 < b1) {
+        load_y(b0, yv[0]);
+        load_b(b0, bv[0].v);
+      }
+#pragma unroll 1
+      for (int blk = b0; blk < b1; blk += 2 * W) {
+        trip(blk, 0);
+        if (blk + W < b1) trip(blk + W, 1);
+      }
+    };
+    if (R == 32) run([&](int blk, uint4 (&v)[4]) { load_wide(blk, 0, v); }, [&](int m, const uint4 (&v)[4], float (&acc)[4][4]) { multiply_wide(m, 0, v, acc); }, Four<uint4>{});
+    else run([&](int blk, uint2 (&v)[4]) { load_narrow(blk, 0, v); }, [&](int m, const uint2 (&v)[4], float (&acc)[4][4]) { multiply(m, 0, v, acc); }, Four<uint2>{});
+    done = true;
+    }
+  } else if (R <= 16) {  // a trip or two: nothing to run ahead of
+#pragma unroll 1
+    for (int blk = b0; blk < b1; blk += W) {
+      uint4 yv[2 * MT];
+      uint2 v[4];
+      load_y(blk, yv);
+      load_narrow(blk, 0, v);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float acc[4][4];
+        clear(acc);
+        multiply(m, 0, v, acc);
+        finish(blk, m, yv, acc);
+      }
+    }
+    done = true;
+  }
+  if (!done) {
+#pragma unroll 1
+    for (int blk = b0; blk < b1; blk += W) {
+      uint4 yv[2 * MT];
+      load_y(blk, yv);
+      float acc[MT][4][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) clear(acc[m]);
+      if (wide) {
+#pragma unroll 2
+        for (int s2 = 0; s2 < ksteps / 2; ++s2) {
+          uint4 v[4];
+          load_wide(blk, s2, v);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) multiply_wide(m, s2, v, acc[m]);
+        }
+      } else {
+#pragma unroll 2
+        for (int s = 0; s < ksteps; ++s) {
+          uint2 v[4];
+          load_narrow(blk, s, v);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) multiply(m, s, v, acc[m]);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) finish(blk, m, yv, acc[m]);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- host side
 constexpr int kMaxDevices = 64;
 
-template <typename T, int MT, bool STAGED>
+template <typename T, int MT, int RG, bool STAGED>
 int launch(const Params& p, int64_t items, cudaStream_t stream) {
-  auto kernel = adapters_kernel<T, MT, STAGED>;
+  auto kernel = adapters_kernel<T, MT, RG, STAGED>;
   static std::atomic<bool> configured[kMaxDevices];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -568,7 +642,7 @@ int launch(const Params& p, int64_t items, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(items * p.cluster));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = layout<MT, STAGED>(p.R, p.cluster).total;
+  cfg.dynamicSmemBytes = layout<MT, RG, STAGED>(p.R, p.cluster).total;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -606,14 +680,15 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
     return set_error(TBIK_ERR_ALIGN, "tbik_adapters: pointers must be 16-byte aligned, row strides multiples of 8 elements");
   Params p{x, y, A, B, out, scales, h, order, offsets, T, ldx, ldy, ldo, N, K, R, adapters, leaf, 1, 0};
   p.rest = (expand ? out != y : 1) ? 1 : 0;
-  // Few rows: 16-row tiles.  CTAs per tile: as many as keep the grid near two CTAs per SM.
+  // Few rows: 16-row tiles.  CTAs per tile: as many as keep the grid near two CTAs per SM; with large ranks enough for the
+  // leaves' sums of 64 rows to fit.
   const bool few = T <= 1024;
-  const int rows = few ? 16 : 32;
+  const int rows = few ? 16 : 64;
   const int64_t items = T / rows + (T < adapters ? T : adapters) + (p.rest ? 1 : 0);
-  while (p.cluster < kLeaves && items * p.cluster * 2 <= 2 * 148 + 148) p.cluster *= 2;
+  while (p.cluster < kLeaves && (items * p.cluster * 2 <= 2 * 148 + 148 || (!few && kLeaves / p.cluster * R > 256))) p.cluster *= 2;
   if (dtype == TBIK_DTYPE_BF16)
-    return few ? launch<__nv_bfloat16, 1, true>(p, items, stream) : launch<__nv_bfloat16, 2, false>(p, items, stream);
-  return few ? launch<__half, 1, true>(p, items, stream) : launch<__half, 2, false>(p, items, stream);
+    return few ? launch<__nv_bfloat16, 1, 1, true>(p, items, stream) : launch<__nv_bfloat16, 2, 2, false>(p, items, stream);
+  return few ? launch<__half, 1, 1, true>(p, items, stream) : launch<__half, 2, 2, false>(p, items, stream);
 }
 
 }  // namespace tbik
