@@ -34,8 +34,9 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kLeaves = 8;
-// One of the two buffers of a staged leaf: four CTAs per SM for the usual ranks, more columns at a time for the large ones.
-__host__ __device__ constexpr uint32_t stage_bytes(int R) { return R <= 32 ? 24576 : 49152; }
+// One of the two buffers of a staged leaf.  Three CTAs per SM for the usual ranks, whose leaf then comes in one piece (96 rows of 48
+// adapters, rank 16, K = 12288: 24 KiB 18.5 us, 30 KiB 17.4 us, 36 KiB and two CTAs 22.6 us); more columns at a time for the large ones.
+__host__ __device__ constexpr uint32_t stage_bytes(int R) { return R <= 32 ? 30720 : 49152; }
 
 struct Params {
   const void *x, *y, *A, *B;

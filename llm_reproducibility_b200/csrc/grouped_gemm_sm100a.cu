@@ -933,9 +933,18 @@ int make_map(CUtensorMap* tm, int dtype, const void* base, int rank, const int64
   cuuint32_t box[3] = {BK, static_cast<cuuint32_t>(box_rows), 1}, one[3] = {1, 1, 1};
   for (int i = 0; i < rank; ++i) d[i] = static_cast<cuuint64_t>(dims[i]);
   for (int i = 0; i + 1 < rank; ++i) s[i] = static_cast<cuuint64_t>(strides[i]) * 2;
-  const CUresult r = fn(tm, dtype == TBIK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                        static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&]() {
+    return fn(tm, dtype == TBIK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+              static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+    // The first CUDA call of a host thread (a backward pass runs in one of its own): the runtime binds the device's
+    // context when it is told the device, the driver call above does not.
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   if (r != CUDA_SUCCESS) {
     char msg[160];
     snprintf(msg, sizeof(msg), "cuTensorMapEncodeTiled failed with CUresult %d (%lld x %lld, stride %lld)", static_cast<int>(r),

@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .row_groups import RowGroups, need_cuda, on_device, overlap, refuse_grad
+from .row_groups import RowGroups, empty, launch, need_cuda, overlap, refuse_grad
 from .tree_based_matmul import _DTYPE_CODE
 
 
@@ -34,7 +34,8 @@ def leaf_for_adapters(K_total: int, max_tp: int = 8) -> int:
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """Rows of contiguous elements on 16-byte boundaries; anything else is copied once."""
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 and t.stride(0) >= t.shape[1]:
+    step, one = t.stride()
+    if one == 1 and step % 8 == 0 and step >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -49,19 +50,23 @@ def _check(what, rows, groups: RowGroups, adapters: int, rank: int, widths, *ten
         raise ValueError(f"{what}: the rank must be a multiple of 8 up to {_lib.MAX_RANK} (pad with zeros), got {rank}")
     if not 1 <= adapters <= _lib.MAX_GROUPS:
         raise ValueError(f"{what}: 1 .. {_lib.MAX_GROUPS} adapters, got {adapters}")
-    if any(w < 8 or w % 8 for w in widths):
-        raise ValueError(f"{what}: widths must be positive multiples of 8, got {widths}")
-    for name, t, n in (("order", groups.order, rows), ("offsets", groups.offsets, adapters + 1)):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n:
-            raise ValueError(f"{what}: groups.{name} must be {n} int32 values, got {tuple(t.shape)} of {t.dtype}")
-    return need_cuda(what, *tensors, groups.order, groups.offsets)
+    for w in widths:
+        if w < 8 or w % 8:
+            raise ValueError(f"{what}: widths must be positive multiples of 8, got {widths}")
+    order, _, offsets = groups
+    if order.dtype != torch.int32 or order.shape != (rows,):
+        raise ValueError(f"{what}: groups.order must be {rows} int32 values, got {tuple(order.shape)} of {order.dtype}")
+    if offsets.dtype != torch.int32 or offsets.shape != (adapters + 1,):
+        raise ValueError(f"{what}: groups.offsets must be {adapters + 1} int32 values, got {tuple(offsets.shape)} of {offsets.dtype}")
+    return need_cuda(what, *tensors, order, offsets)
 
 
 def _types(what, first, *others) -> None:
     if first.dtype not in _DTYPE_CODE:
         raise NotImplementedError(f"{what}: dtype {first.dtype} is not supported")
-    if any(t.dtype != first.dtype for t in others):
-        raise ValueError(f"{what}: operands of {first.dtype} and {[t.dtype for t in others]}")
+    for t in others:
+        if t.dtype != first.dtype:
+            raise ValueError(f"{what}: operands of {first.dtype} and {t.dtype}")
 
 
 def _check_leaf(what, K: int, leaf: Optional[int]) -> int:
@@ -75,7 +80,7 @@ def _check_leaf(what, K: int, leaf: Optional[int]) -> int:
 def _check_out(what, y, out, *others):
     """The result's tensor.  It is written while the operands are read: it may be y itself, and else overlaps nothing."""
     if out is None:
-        return torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        return empty(y.shape[0], y.shape[1], y.dtype, y.device)
     same = out.data_ptr() == y.data_ptr() and out.stride() == y.stride()
     if any(overlap(out, t) for t in others + (() if same else (y,))):
         raise ValueError(f"{what}: out overlaps an operand")
@@ -86,14 +91,15 @@ def _check_out(what, y, out, *others):
 
 
 def _launch(what, dev, x, y, out, A, B, scales, h, groups, T, N, K, R, adapters, dtype, leaf):
-    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-    ld = lambda t: max(t.stride(0), t.shape[1]) if t is not None else 0  # noqa: E731
     order, offsets = groups.order.contiguous(), groups.offsets.contiguous()
-    rc = on_device(dev, lambda stream: _lib.lib().tbik_adapters(
-        ptr(x), ld(x), ptr(y), ld(y), ptr(out), ld(out), ptr(A), ptr(B), ptr(scales), ptr(h), order.data_ptr(),
-        offsets.data_ptr(), T, N, K, R, adapters, _DTYPE_CODE[dtype], leaf, stream))
-    if rc != 0:
-        _lib.check(rc, "tbik_adapters")
+    px = ldx = py = ldy = po = ldo = 0
+    if x is not None:
+        px, ldx = x.data_ptr(), max(x.stride(0), K)
+    if y is not None:
+        py, ldy, po, ldo = y.data_ptr(), max(y.stride(0), N), out.data_ptr(), max(out.stride(0), N)
+    launch("tbik_adapters", dev, px, ldx, py, ldy, po, ldo, A.data_ptr() if A is not None else 0, B.data_ptr() if B is not None else 0,
+           scales.data_ptr() if scales is not None else 0, h.data_ptr() if h is not None else 0, order.data_ptr(), offsets.data_ptr(),
+           T, N, K, R, adapters, _DTYPE_CODE[dtype], leaf)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, groups: RowGroups, scales: torch.Tensor, *,
@@ -135,7 +141,7 @@ def lora_shrink(x: torch.Tensor, A: torch.Tensor, groups: RowGroups, *, leaf: Op
     (T, K), (L, R, _) = x.shape, A.shape
     leaf = _check_leaf(what, K, leaf)
     dev = _check(what, T, groups, L, R, (K,), x, A)
-    h = torch.empty((T, R), dtype=torch.float32, device=dev)
+    h = empty(T, R, torch.float32, dev)
     if T:
         _launch(what, dev, _rows16(x), None, None, _weights16(A), None, None, h, groups, T, 8, K, R, L, x.dtype, leaf)
     return h

@@ -20,7 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .grouped_matmul import _grouped, _weight_gradient
-from .row_groups import Routing, RowGroups, _route, _route_backward
+from .row_groups import Routing, _route, _route_backward
 from .tree_based_matmul import _LEAF, matmul_tp_persistent
 
 
@@ -93,22 +93,25 @@ def tree_grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Te
 
 
 class _TreeRouteTopk(torch.autograd.Function):
+    """The weights are the one output that autograd knows: the integers go past it, in `found`."""
+
     @staticmethod
-    def forward(ctx, logits, k, renormalize):
+    def forward(ctx, logits, k, renormalize, found):
         r = _route(logits, k, renormalize)
         ctx.save_for_backward(logits, r.weights, r.ids)
         ctx.renormalize = renormalize
-        ctx.mark_non_differentiable(r.ids, *r.groups)
-        return (r.weights, r.ids) + tuple(r.groups)
+        found.append(r)
+        return r.weights
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dweights, *_):
+    def backward(ctx, dweights):
         logits, weights, ids = ctx.saved_tensors
-        return _route_backward(logits, weights, ids, dweights, ctx.renormalize), None, None
+        return _route_backward(logits, weights, ids, dweights, ctx.renormalize), None, None, None
 
 
 def tree_route_topk(logits: torch.Tensor, k: int, *, renormalize: bool = True) -> Routing:
     """`route_topk` whose weights carry a gradient to the logits (through the softmax; the choice itself has none)."""
-    weights, ids, order, position, offsets = _TreeRouteTopk.apply(logits, k, renormalize)
-    return Routing(weights, ids, RowGroups(order, position, offsets))
+    found = []
+    weights = _TreeRouteTopk.apply(logits, k, renormalize, found)
+    return Routing(weights, found[0].ids, found[0].groups)

@@ -13,19 +13,21 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .row_groups import need_cuda, on_device, overlap, refuse_grad
+from .row_groups import empty, launch, need_cuda, overlap, refuse_grad
 from .tree_based_matmul import _DTYPE_CODE
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """t [.., rows, cols] with contiguous elements in a row, 16-byte aligned rows; anything else is copied once."""
     cols = t.shape[-1]
-    ok = (t.stride(-1) == 1 or cols == 1) and t.data_ptr() % 16 == 0
-    # a stride that is never stepped says nothing, but the kernel's tensor maps read it all the same
-    for d in range(t.dim() - 1):
-        ok = ok and t.stride(d) % 8 == 0 and t.stride(d) >= cols
-    if ok:
-        return t
+    *steps, last = t.stride()
+    # (a stride that is never stepped says nothing, but the kernel's tensor maps read it all the same)
+    if (last == 1 or cols == 1) and t.data_ptr() % 16 == 0:
+        for s in steps:
+            if s % 8 or s < cols:
+                break
+        else:
+            return t
     pad = (cols + 7) // 8 * 8
     buf = torch.empty(t.shape[:-1] + (pad,), dtype=t.dtype, device=t.device)
     buf[..., :cols].copy_(t)
@@ -82,7 +84,7 @@ def _grouped(A, W, offsets, leaf=None, out=None, out_dtype=None, max_ctas=0):
     dev = need_cuda(what, A, W, offsets)
     c_dtype = out_dtype or A.dtype
     if out is None:
-        C = torch.empty((M, N), dtype=c_dtype, device=dev)
+        C = empty(M, N, c_dtype, dev)
     else:
         C = out
         if C.shape != (M, N) or C.dtype != c_dtype or C.device != dev or (N > 1 and C.stride(1) != 1) or \
@@ -99,12 +101,11 @@ def _grouped(A, W, offsets, leaf=None, out=None, out_dtype=None, max_ctas=0):
         layout = _lib.W_N_CONTIGUOUS
         W = W.transpose(1, 2)
     W = _aligned_rows(W)
-    rc = on_device(dev, lambda stream: _lib.lib().tbik_grouped_gemm(
-        A.data_ptr(), W.data_ptr(), C.data_ptr(), offsets.data_ptr(), M, N, K, G, A.stride(0), W.stride(1), W.stride(0),
-        max(C.stride(0), N), layout, _DTYPE_CODE[A.dtype], _lib.DTYPE_FP32 if c_dtype == torch.float32 else _DTYPE_CODE[A.dtype],
-        leaf or 0, int(out is None), max_ctas, stream))
-    if rc != 0:
-        _lib.check(rc, "tbik_grouped_gemm")
+    step_w, ldw, _ = W.stride()
+    code = _DTYPE_CODE[A.dtype]
+    launch("tbik_grouped_gemm", dev, A.data_ptr(), W.data_ptr(), C.data_ptr(), offsets.data_ptr(), M, N, K, G, A.stride(0), ldw,
+           step_w, max(C.stride(0), N), layout, code, _lib.DTYPE_FP32 if c_dtype == torch.float32 else code, leaf or 0, out is None,
+           max_ctas)
     return C
 
 
@@ -135,9 +136,7 @@ def _weight_gradient(dC, A, offsets, out_dtype=None, max_ctas=0):
     if M == 0:
         return dW.zero_()
     A, dC = _aligned_rows(A), _aligned_rows(dC)
-    rc = on_device(dev, lambda stream: _lib.lib().tbik_grouped_gemm_wgrad(
-        dC.data_ptr(), A.data_ptr(), dW.data_ptr(), offsets.data_ptr(), M, N, K, groups, dC.stride(0), A.stride(0),
-        _DTYPE_CODE[A.dtype], _lib.DTYPE_FP32 if dW.dtype == torch.float32 else _DTYPE_CODE[A.dtype], max_ctas, stream))
-    if rc != 0:
-        _lib.check(rc, "tbik_grouped_gemm_wgrad")
+    code = _DTYPE_CODE[A.dtype]
+    launch("tbik_grouped_gemm_wgrad", dev, dC.data_ptr(), A.data_ptr(), dW.data_ptr(), offsets.data_ptr(), M, N, K, groups,
+           dC.stride(0), A.stride(0), code, _lib.DTYPE_FP32 if dW.dtype == torch.float32 else code, max_ctas)
     return dW

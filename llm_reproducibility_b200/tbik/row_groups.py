@@ -32,28 +32,42 @@ class Routing(NamedTuple):
     groups: RowGroups      # of the T * k flat entries of ids: row i is token i // k
 
 
-def on_device(device: torch.device, call) -> int:
-    """Run `call(stream)` with `device` current; the kernels go to that device's current stream."""
-    if torch.cuda.current_device() == device.index:
-        return call(_raw_stream(device.index))
-    with torch.cuda.device(device):
-        return call(_raw_stream(device.index))
+def launch(name: str, device: torch.device, *args) -> None:
+    """Call the library's function `name` with `args` and, as its last argument, the current stream of `device`, which is
+    made the current device for the call."""
+    fn = getattr(_lib.lib(), name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(index))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+def empty(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """torch.empty((rows, cols)) by the quicker of its ways: a microsecond of a decode step's few."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
 def need_cuda(what: str, *tensors: torch.Tensor) -> torch.device:
     """The tensors' one CUDA device."""
+    device = tensors[0].device
     for t in tensors:
         if not t.is_cuda:
             raise RuntimeError(f"{what} needs CUDA tensors (there is no CPU fallback)")
-        if t.device != tensors[0].device:
-            raise RuntimeError(f"{what}: tensors on {tensors[0].device} and {t.device}")
-    return tensors[0].device
+        if t.device != device:
+            raise RuntimeError(f"{what}: tensors on {device} and {t.device}")
+    return device
 
 
 def refuse_grad(what: str, instead: str, *tensors) -> None:
     """A call that records no gradient must not swallow one."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} records no gradient: {instead}")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{what} records no gradient: {instead}")
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -68,12 +82,12 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _empty_groups(M: int, groups: int, device: torch.device):
-    """An empty RowGroups and the kernels' workspace (pointer, bytes): one allocation, parts on 16-byte boundaries."""
-    pad, table = (M + 3) // 4 * 4, (groups + 4) // 4 * 4
+    """An empty RowGroups and the kernels' workspace (pointer, bytes), in one allocation."""
     nbytes = _lib.lib().tbik_group_workspace_bytes(M, groups)
-    buf = torch.empty(2 * pad + table + nbytes // 4, dtype=torch.int32, device=device)
-    g = RowGroups(buf[:M], buf[pad:pad + M], buf[2 * pad:2 * pad + groups + 1])
-    return g, buf.data_ptr() + 4 * (2 * pad + table), nbytes
+    sizes = [M, M, groups + 1, nbytes // 4]
+    buf = torch.empty_strided((sum(sizes),), (1,), dtype=torch.int32, device=device)
+    order, position, offsets, ws = buf.split_with_sizes(sizes)
+    return RowGroups(order, position, offsets), ws.data_ptr(), nbytes
 
 
 def _check_groups(num_groups: int) -> None:
@@ -92,10 +106,8 @@ def group_rows(ids: torch.Tensor, num_groups: int) -> RowGroups:
     dev = need_cuda("group_rows", ids)
     ids = ids.contiguous()
     g, ws, nbytes = _empty_groups(ids.numel(), num_groups, dev)
-    rc = on_device(dev, lambda stream: _lib.lib().tbik_group_rows(
-        ids.data_ptr(), ids.numel(), num_groups, g.order.data_ptr(), g.position.data_ptr(), g.offsets.data_ptr(), ws, nbytes, stream))
-    if rc != 0:
-        _lib.check(rc, "tbik_group_rows")
+    launch("tbik_group_rows", dev, ids.data_ptr(), ids.numel(), num_groups, g.order.data_ptr(), g.position.data_ptr(),
+           g.offsets.data_ptr(), ws, nbytes)
     return g
 
 
@@ -111,7 +123,8 @@ def _check_logits(logits: torch.Tensor, k: int) -> torch.Tensor:
         raise ValueError(f"route_topk: k must be in 1 .. {min(E, _lib.MAX_TOPK)}, got {k}")
     if T * k >= 1 << 31:
         raise ValueError("route_topk: fewer than 2^31 (token, slot) rows")
-    need_cuda("route_topk", logits)
+    if not logits.is_cuda:
+        need_cuda("route_topk", logits)
     # rows may be strided or broadcast; the experts of a row must be contiguous
     return logits if logits.stride(1) == 1 or E == 1 else logits.contiguous()
 
@@ -130,25 +143,19 @@ def _route(logits: torch.Tensor, k: int, renormalize: bool) -> Routing:
     logits = _check_logits(logits, k)
     T, E = logits.shape
     dev = logits.device
-    weights = torch.empty((T, k), dtype=torch.float32, device=dev)
-    ids = torch.empty((T, k), dtype=torch.int32, device=dev)
+    weights, ids = empty(T, k, torch.float32, dev), empty(T, k, torch.int32, dev)
     g, ws, nbytes = _empty_groups(T * k, E, dev)
-    rc = on_device(dev, lambda stream: _lib.lib().tbik_route_topk(
-        logits.data_ptr(), logits.stride(0), T, E, k, _LOGITS_CODE[logits.dtype], int(renormalize), weights.data_ptr(),
-        ids.data_ptr(), g.order.data_ptr(), g.position.data_ptr(), g.offsets.data_ptr(), ws, nbytes, stream))
-    if rc != 0:
-        _lib.check(rc, "tbik_route_topk")
+    launch("tbik_route_topk", dev, logits.data_ptr(), logits.stride(0), T, E, k, _LOGITS_CODE[logits.dtype], renormalize,
+           weights.data_ptr(), ids.data_ptr(), g.order.data_ptr(), g.position.data_ptr(), g.offsets.data_ptr(), ws, nbytes)
     return Routing(weights, ids, g)
 
 
 def _route_backward(logits, weights, ids, dweights, renormalize: bool) -> torch.Tensor:
     logits = _check_logits(logits, ids.shape[1])
     T, E = logits.shape
-    dweights = dweights.to(torch.float32).contiguous()
-    dlogits = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-    rc = on_device(logits.device, lambda stream: _lib.lib().tbik_route_topk_backward(
-        logits.data_ptr(), logits.stride(0), T, E, ids.shape[1], _LOGITS_CODE[logits.dtype], int(renormalize),
-        weights.data_ptr(), ids.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), E, stream))
-    if rc != 0:
-        _lib.check(rc, "tbik_route_topk_backward")
+    if dweights.dtype != torch.float32 or not dweights.is_contiguous():
+        dweights = dweights.to(torch.float32).contiguous()
+    dlogits = empty(T, E, logits.dtype, logits.device)
+    launch("tbik_route_topk_backward", logits.device, logits.data_ptr(), logits.stride(0), T, E, ids.shape[1],
+           _LOGITS_CODE[logits.dtype], renormalize, weights.data_ptr(), ids.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), E)
     return dlogits

@@ -323,3 +323,30 @@ def test_device_status_stays_clean():
     from llm_reproducibility_b200.tbik.tree_based_matmul import gemm_device_status
     torch.cuda.synchronize()
     assert gemm_device_status()[0] == 0
+
+
+def test_first_cuda_call_of_a_host_thread():
+    """A backward pass runs in a thread of its own, whose first CUDA call may be this one: nothing before it may have
+    bound a context there (the allocator serves the result from its cache)."""
+    import threading
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent, grouped_weight_gradient
+    off = offsets_of([20, 30]).cuda()
+    A, W, D = make((50, 64), torch.bfloat16, "int", 1), make((2, 72, 64), torch.bfloat16, "int", 2), make((50, 72), torch.bfloat16, "int", 3)
+    want, dwant = grouped_matmul_tp_persistent(A, W, off), grouped_weight_gradient(D, A, off)
+    spare = [torch.empty_like(want), torch.empty_like(dwant)]
+    del spare
+    torch.cuda.synchronize()
+    for call, expected in ((lambda: grouped_matmul_tp_persistent(A, W, off), want), (lambda: grouped_weight_gradient(D, A, off), dwant)):
+        got = []
+
+        def work():
+            try:
+                got.append(call())
+            except Exception as e:  # noqa: BLE001
+                got.append(e)
+
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert torch.is_tensor(got[0]) and torch.equal(got[0], expected), got[0]
