@@ -230,6 +230,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
 
   int role_failed = 0;
 
+  // The tree's epilogue holds a node and a whole leaf in registers: with 128 tokens per tile it takes registers from the
+  // warps that issue.
+  constexpr bool SPLIT = TREE && C_::CHUNKS > 1;
+  if (warp < EPI_WARP0) {
+  if constexpr (SPLIT) setmaxnreg_dec<56>();
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (elect_one()) {
@@ -389,8 +394,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
         }
       }
     }
-  } else if (warp >= EPI_WARP0) {
+  }
+  } else {
     // ------------------------------------------------------------ epilogue: lanes are weight rows, columns are tokens
+    if constexpr (SPLIT) setmaxnreg_inc<224>();
     const int q = warp & 3;                 // tensor-memory lane quadrant of this warp
     const int h = (warp - EPI_WARP0) >> 2;  // it drains every second chunk of tokens
     const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
@@ -451,7 +458,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
           }
         }
       };
-      [[maybe_unused]] float node[TREE ? C_::CHUNKS * CHUNK : 1];
+      // the open level-0 group, then the node that climbs the tree: fp32 in the registers that tcgen05.ld fills
+      [[maybe_unused]] uint32_t node[TREE ? C_::CHUNKS : 1][CHUNK];
       int in_group = 0;
       uint32_t closed = 0;
       for (int l = 0; ok && l < p.T; ++l, ++chain) {
@@ -490,38 +498,40 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
           }
         } else {
           tmem_wait_st();  // stack stores of earlier leaves have landed
-          uint32_t raw[C_::CHUNKS][CHUNK];
+          // one fp32 add per node (commutative: which side is the earlier one does not matter)
+          auto add = [&](uint32_t (&x)[CHUNK], const uint32_t (&y)[CHUNK]) {
 #pragma unroll
-          for (int c = 0; c < C_::CHUNKS; ++c)
-            if (c < have) tmem_ld32(tacc + c * C_::EPI_HALVES * CHUNK, raw[c]);
-          tmem_wait_ld();
-          release();
+            for (int j = 0; j < CHUNK; ++j) x[j] = __float_as_uint(__fadd_rn(__uint_as_float(x[j]), __uint_as_float(y[j])));
+          };
+          // 32 columns per chunk from tensor memory, all chunks requested before the first is waited for
+          auto fetch = [&](uint32_t (&v)[C_::CHUNKS][CHUNK], uint32_t col) {
 #pragma unroll
-          for (int c = 0; c < C_::CHUNKS; ++c) {
+            for (int c = 0; c < C_::CHUNKS; ++c)
+              if (c < have) tmem_ld32(col + c * C_::EPI_HALVES * CHUNK, v[c]);
+            tmem_wait_ld();
+          };
+          if (in_group == 0) {
+            fetch(node, tacc);
+            release();
+          } else {
+            uint32_t raw[C_::CHUNKS][CHUNK];
+            fetch(raw, tacc);
+            release();
 #pragma unroll
-            for (int j = 0; j < CHUNK; ++j) {
-              const float v = __uint_as_float(raw[c][j]);
-              node[c * CHUNK + j] = in_group > 0 ? __fadd_rn(node[c * CHUNK + j], v) : v;  // level 0: F leaves left to right
-            }
+            for (int c = 0; c < C_::CHUNKS; ++c)
+              if (c < have) add(node[c], raw[c]);  // level 0: F leaves left to right
           }
           if (++in_group < p.F) continue;
           in_group = 0;
           uint32_t gb = closed++;
           int lvl = 1;
-          auto stack_col = [&](int level, int c) -> uint32_t {
-            return tmem_base + lane_off + (1 + level) * TN + (c * C_::EPI_HALVES + h) * CHUNK;
-          };
+          auto stack_col = [&](int level) -> uint32_t { return tmem_base + lane_off + (1 + level) * TN + h * CHUNK; };
           while (lvl < p.L && (gb & 1u)) {
+            uint32_t raw[C_::CHUNKS][CHUNK];
+            fetch(raw, stack_col(lvl));
 #pragma unroll
-            for (int c = 0; c < C_::CHUNKS; ++c) {
-              if (c < have) {
-                uint32_t s[CHUNK];
-                tmem_ld32(stack_col(lvl, c), s);
-                tmem_wait_ld();
-#pragma unroll
-                for (int j = 0; j < CHUNK; ++j) node[c * CHUNK + j] = __fadd_rn(__uint_as_float(s[j]), node[c * CHUNK + j]);
-              }
-            }
+            for (int c = 0; c < C_::CHUNKS; ++c)
+              if (c < have) add(node[c], raw[c]);
             gb >>= 1;
             ++lvl;
           }
@@ -529,14 +539,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
           for (int c = 0; c < C_::CHUNKS; ++c) {
             if (c < have) {
               if (lvl < p.L) {
-                uint32_t s[CHUNK];
-#pragma unroll
-                for (int j = 0; j < CHUNK; ++j) s[j] = __float_as_uint(node[c * CHUNK + j]);
-                tmem_st32(stack_col(lvl, c), s);
+                tmem_st32(stack_col(lvl) + c * C_::EPI_HALVES * CHUNK, node[c]);
               } else {
                 float v[CHUNK];
 #pragma unroll
-                for (int j = 0; j < CHUNK; ++j) v[j] = node[c * CHUNK + j];
+                for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(node[c][j]);
                 store_chunk(v, (c * C_::EPI_HALVES + h) * CHUNK);
               }
             }
