@@ -279,18 +279,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
           }
           return true;
         };
-        for (int l = 0; ok && l < p.T; ++l) {
-          const int x0 = l * p.blocks_per_leaf * BK;
-          if (SUB == 1 && (p.blocks_per_leaf & 3) == 0) {
-            // straight-line code for four blocks: a taken branch per block costs more than issuing its loads
-            for (int b = 0; ok && b < p.blocks_per_leaf; b += 4) {
+        if constexpr (SUB == 1) {
+          // straight-line code for four blocks: a taken branch per block costs more than issuing its loads.  Leaves follow
+          // each other in K, so they do not matter here.
+          const int blocks = p.T * p.blocks_per_leaf;
+          int b = 0;
+          for (; ok && b + 4 <= blocks; b += 4) {
 #pragma unroll
-              for (int u = 0; u < 4; ++u)
-                if (!load(x0 + (b + u) * BK, 1)) break;
-            }
-          } else {
+            for (int u = 0; u < 4; ++u)
+              if (!load((b + u) * BK, 1)) break;
+          }
+          for (; ok && b < blocks; ++b)
+            if (!load(b * BK, 1)) break;
+        } else {
+          for (int l = 0; ok && l < p.T; ++l) {
             for (int b = 0; b < p.blocks_per_leaf; b += SUB)
-              if (!load(x0 + b * BK, min(SUB, p.blocks_per_leaf - b))) break;
+              if (!load((l * p.blocks_per_leaf + b) * BK, min(SUB, p.blocks_per_leaf - b))) break;
           }
         }
       }
@@ -380,12 +384,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
             }
             return true;
           };
-          if (SUB == 1 && (p.blocks_per_leaf & 3) == 0) {
-            for (int b = 0; ok && b < p.blocks_per_leaf; b += 4) {
+          if constexpr (SUB == 1) {
+            int b = 0;
+            for (; ok && b + 4 <= p.blocks_per_leaf; b += 4) {
 #pragma unroll
               for (int u = 0; u < 4; ++u)
                 if (!stage_of(b + u, 1)) break;
             }
+#pragma unroll
+            for (int u = 0; u < 3; ++u)
+              if (ok && b + u < p.blocks_per_leaf) stage_of(b + u, 1);
           } else {
             for (int b = 0; b < p.blocks_per_leaf; b += SUB)
               if (!stage_of(b, min(SUB, p.blocks_per_leaf - b))) break;
