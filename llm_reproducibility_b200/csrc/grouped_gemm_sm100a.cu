@@ -50,13 +50,13 @@ constexpr int NUM_EPI_WARPS = 8;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int CHUNK = 32;  // accumulator columns per tcgen05.ld
 constexpr uint64_t WAIT_LIMIT_NS = 2000000000ull;
-constexpr uint32_t STAGING_BYTES_PER_WARP = 2048;
+constexpr uint32_t STAGING_BYTES_PER_WARP = 4096;  // weight gradient: 32 rows of 128 bytes
 constexpr int GROUP_M = 8;  // row tiles that share a sweep over the columns
 
 __device__ uint32_t g_grouped_status[4];  // [0] a bounded wait ran out, [1] block, [2] role
 
 struct Maps {
-  CUtensorMap a[4];  // forward: A with boxes of 16, 32, 64, 128 rows; weight gradient: a[0] = dC
+  CUtensorMap a[4];  // forward: A with boxes of 16, 32, 64, 128 rows; weight gradient: a[0] = dC, a[1] = dW
   CUtensorMap b;     // W; weight gradient: A
 };
 
@@ -583,6 +583,7 @@ struct WgradParams {
   int rows, cols;        // N, K: dW[g] is [N, K]
   int tiles_r, tiles_c;
   int half, out32;
+  int tma_store;         // dW leaves through tensor map a[1]
 };
 
 template <int BN, int STAGES_, bool PAIR>
@@ -862,6 +863,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
       }
     };
 
+    // 128 bytes of each of this warp's 32 rows (64 columns, or 32 of fp32) to shared memory in the tensor map's swizzle, and
+    // from there as one tiled store, which stops at the edges of the group's matrix.  (Pieces of 64 bytes stored by the
+    // threads themselves wrote an all-zero gradient of 268 MB in 64 us.)
+    const uint32_t stage_addr = smem_u32(staging);
+    auto staging_free = [&]() {  // the store before has read the staging buffer
+      if (lane == 0) bulk_wait_read_all();
+      __syncwarp();
+    };
+    auto put = [&](int j, const uint4& w) {  // piece j of this lane's row
+      *reinterpret_cast<uint4*>(staging + lane * 128 + ((j ^ (lane & 7)) << 4)) = w;
+    };
+    auto send = [&](const Tile& t, int row0, int col) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(&maps.a[1], stage_addr, col, row0, t.g);
+        bulk_commit_group();
+      }
+    };
+
     uint32_t chain = 0;
     for (int tile = unit; ok && tile < num_tiles; tile += num_units) {
       const Tile t = tile_at(tile);
@@ -869,6 +890,19 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
       const int rows_left = p.rows - row0;
       uint8_t* c_row0 = static_cast<uint8_t*>(p.C) + (static_cast<int64_t>(t.g) * p.rows + row0) * p.cols * es;
       const int col0 = t.col + h * C_::CW;
+      const bool here = rows_left > 0 && col0 < p.cols;  // this warp has something to write
+      if (t.count == 0 && p.tma_store) {
+        if (here) {
+          staging_free();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) put(j, make_uint4(0u, 0u, 0u, 0u));
+          const int step = p.out32 ? 32 : 64;
+          fence_proxy_async_smem();
+          __syncwarp();
+          for (int c = col0; c < min(col0 + C_::CW, p.cols); c += step) send(t, row0, c);
+        }
+        continue;
+      }
       if (t.count == 0) {
         float zero[CHUNK];
 #pragma unroll
@@ -890,8 +924,40 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * a);
       };
-      if (rows_left <= 0 || col0 >= p.cols) {
+      if (!here) {
         release();
+        continue;
+      }
+      if (p.tma_store) {
+#pragma unroll
+        for (int c = 0; c < C_::NCH; c += 2) {  // 64 columns at a time
+          uint32_t raw[2][CHUNK];
+          tmem_ld32(tacc + c * CHUNK, raw[0]);
+          tmem_ld32(tacc + (c + 1) * CHUNK, raw[1]);
+          tmem_wait_ld();
+          if (c + 2 >= C_::NCH) release();
+          const int col = col0 + c * CHUNK;
+          if (p.out32) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              staging_free();
+#pragma unroll
+              for (int j = 0; j < 8; ++j) put(j, make_uint4(raw[u][4 * j], raw[u][4 * j + 1], raw[u][4 * j + 2], raw[u][4 * j + 3]));
+              if (col + u * CHUNK < p.cols) send(t, row0, col + u * CHUNK);
+            }
+          } else {
+            uint32_t w[CHUNK];
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) {
+              const float lo = __uint_as_float(raw[j / 16][2 * (j % 16)]), hi = __uint_as_float(raw[j / 16][2 * (j % 16) + 1]);
+              w[j] = p.half ? Pack16<__nv_bfloat16>::from_f32(lo, hi) : Pack16<__half>::from_f32(lo, hi);
+            }
+            staging_free();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) put(j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
+            if (col < p.cols) send(t, row0, col);
+          }
+        }
         continue;
       }
       uint32_t raw[2][CHUNK];
@@ -909,6 +975,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
   }
 
   // ---------------------------------------------------------------- tear-down
+  if (warp >= EPI_WARP0 && lane == 0) bulk_wait_read_all();  // staged stores have left shared memory
   tc_fence_before_sync();
   __syncwarp();
   if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
@@ -940,16 +1007,17 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// `rank` 2 or 3 dimensions of a 16-bit tensor, innermost first, strides in elements; box 64 wide, `box_rows` high.
+// `rank` 2 or 3 dimensions of a tensor, innermost first, strides in elements; box 128 bytes wide, `box_rows` high.
 int make_map(CUtensorMap* tm, int dtype, const void* base, int rank, const int64_t* dims, const int64_t* strides, int box_rows) {
+  const bool f32 = dtype == TBIK_DTYPE_FP32;  // (results only) 32 wide: 128 bytes either way
   EncodeTiledFn fn = encode_fn();
   if (!fn) return set_error(TBIK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   cuuint64_t d[3], s[2];
-  cuuint32_t box[3] = {BK, static_cast<cuuint32_t>(box_rows), 1}, one[3] = {1, 1, 1};
+  cuuint32_t box[3] = {f32 ? 32u : 64u, static_cast<cuuint32_t>(box_rows), 1}, one[3] = {1, 1, 1};
   for (int i = 0; i < rank; ++i) d[i] = static_cast<cuuint64_t>(dims[i]);
-  for (int i = 0; i + 1 < rank; ++i) s[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+  for (int i = 0; i + 1 < rank; ++i) s[i] = static_cast<cuuint64_t>(strides[i]) * (f32 ? 4 : 2);
   auto encode = [&]() {
-    return fn(tm, dtype == TBIK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+    return fn(tm, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == TBIK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
               static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
@@ -1156,6 +1224,13 @@ int grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* o
   rc = make_map(&maps.a[0], dtype, dC, 2, dd, sd, BK);
   if (rc != TBIK_OK) return rc;
   for (int i = 1; i < 4; ++i) maps.a[i] = maps.a[0];
+  const int es = out_dtype == TBIK_DTYPE_FP32 ? 4 : 2;
+  const bool tma_store = !bad_align(dW) && static_cast<int64_t>(K) * es % 16 == 0;
+  if (tma_store) {
+    const int64_t dw[3] = {K, N, groups}, sw[2] = {K, static_cast<int64_t>(N) * K};
+    rc = make_map(&maps.a[1], out_dtype, dW, 3, dw, sw, 32);
+    if (rc != TBIK_OK) return rc;
+  }
   rc = make_map(&maps.b, dtype, A, 2, da, sa, BK);
   if (rc != TBIK_OK) return rc;
   const bool pair = N > BM && K > BM;
@@ -1171,9 +1246,10 @@ int grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* o
   p.tiles_c = (K + bn - 1) / bn;
   p.half = dtype == TBIK_DTYPE_BF16 ? 1 : 0;
   p.out32 = out_dtype == TBIK_DTYPE_FP32 ? 1 : 0;
+  p.tma_store = tma_store ? 1 : 0;
   const int64_t most = static_cast<int64_t>(groups) * p.tiles_r * p.tiles_c;
   if (most >= (int64_t(1) << 31)) return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm_wgrad: too many tiles");
-  return pair ? launch_wgrad<256, 6, true>(maps, p, most, max_ctas, stream) : launch_wgrad<128, 6, false>(maps, p, most, max_ctas, stream);
+  return pair ? launch_wgrad<256, 5, true>(maps, p, most, max_ctas, stream) : launch_wgrad<128, 5, false>(maps, p, most, max_ctas, stream);
 }
 
 int grouped_status(uint32_t out[4]) {

@@ -162,6 +162,11 @@ TBIK_DEVICE void tma_store_2d(const void* tmap, uint32_t smem_src, int32_t x, in
                ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_src), "r"(x), "r"(y)
                : "memory");
 }
+TBIK_DEVICE void tma_store_3d(const void* tmap, uint32_t smem_src, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_src), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 TBIK_DEVICE void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // All bulk stores committed by this thread have finished READING shared memory.
 TBIK_DEVICE void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
