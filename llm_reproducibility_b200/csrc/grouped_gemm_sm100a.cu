@@ -60,42 +60,84 @@ struct Maps {
   CUtensorMap b;     // W; weight gradient: A
 };
 
-// The groups' rows and tiles in shared memory: first[g], last[g] and before[g] = tiles of the groups before g (G + 1
-// entries), tiles_of(rows) tiles each.  Whatever `offsets` holds, the running maximum keeps the groups' rows inside
-// [0, M) and disjoint.  Called by all threads; one more barrier has to follow before the table is read.
+// What every role has to know of the groups, in shared memory: rows first[g] .. last[g] - 1, tiles of `per[g]` rows
+// (forward), before[g] tiles in the groups before g (G + 1 entries).
+struct Table {
+  int *first, *last, *before, *per;
+  int* warps;  // 3 x 16 words of scratch
+  static constexpr uint32_t bytes(int groups) { return 4u * (4 * groups + 1 + 48); }
+  TBIK_DEVICE Table(uint8_t* at, int groups) {
+    first = reinterpret_cast<int*>(at);
+    last = first + groups;
+    per = last + groups;
+    before = per + groups;
+    warps = before + groups + 1;
+  }
+};
+
+TBIK_DEVICE int scan_max(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v = max(v, u);
+  }
+  return v;
+}
+TBIK_DEVICE int scan_sum(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Fills the table; all threads of the block, a thread per group.  tiles_of(rows, per) gives a group's tiles and writes the
+// rows of one.  Whatever `offsets` holds, the running maximum keeps the groups' rows inside [0, M) and disjoint.  One more
+// barrier has to follow before the table is read.
 template <typename TilesOf>
-TBIK_DEVICE void build_table(const int32_t* offsets, int groups, int M, int* first, int* last, int* before, TilesOf tiles_of) {
-  for (int g = threadIdx.x; g < groups; g += NUM_THREADS) last[g] = min(max(offsets[g + 1], 0), M);
-  const int lane = threadIdx.x & 31;
-  int run = 0, end = threadIdx.x < 32 ? min(max(offsets[0], 0), M) : 0;
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  for (int g0 = 0; g0 < groups; g0 += 32) {
-    const int g = g0 + lane;
-    int hi = g < groups ? max(last[g], end) : end;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xFFFFFFFFu, hi, o);
-      if (lane >= o) hi = max(hi, v);
-    }
+TBIK_DEVICE void build_table(const int32_t* offsets, int groups, int M, const Table& t, TilesOf tiles_of) {
+  constexpr int WARPS = NUM_THREADS / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int end = min(max(offsets[0], 0), M), run = 0;  // rows and tiles of the passes before
+  for (int g0 = 0; g0 < groups; g0 += NUM_THREADS) {
+    const int g = g0 + static_cast<int>(threadIdx.x);
+    int hi = scan_max(g < groups ? min(max(offsets[g + 1], 0), M) : 0, lane);
+    if (lane == 31) t.warps[warp] = hi;
+    __syncthreads();
+    int before_warp = end;
+    for (int w = 0; w < warp; ++w) before_warp = max(before_warp, t.warps[w]);
+    hi = max(hi, before_warp);
     int lo = __shfl_up_sync(0xFFFFFFFFu, hi, 1);
-    if (lane == 0) lo = end;
-    const int t = g < groups ? tiles_of(hi - lo) : 0;
-    int s = t;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xFFFFFFFFu, s, o);
-      if (lane >= o) s += v;
+    if (lane == 0) lo = before_warp;
+    int per = 1;
+    const int tiles = g < groups ? tiles_of(hi - lo, per) : 0;
+    const int sum = scan_sum(tiles, lane);
+    if (lane == 31) {
+      t.warps[16 + warp] = sum;
+      t.warps[32 + warp] = hi;
+    }
+    __syncthreads();
+    int at = run;
+    for (int w = 0; w < WARPS; ++w) {
+      if (w < warp) at += t.warps[16 + w];
+      run += t.warps[16 + w];
+      end = max(end, t.warps[32 + w]);
     }
     if (g < groups) {
-      first[g] = lo;
-      last[g] = hi;
-      before[g] = run + s - t;
+      t.first[g] = lo;
+      t.last[g] = hi;
+      t.per[g] = per;
+      t.before[g] = at + sum - tiles;
+      if (g == groups - 1) t.before[groups] = at + sum;
     }
-    run += __shfl_sync(0xFFFFFFFFu, s, 31);
-    end = __shfl_sync(0xFFFFFFFFu, hi, 31);
   }
-  if (lane == 0) before[groups] = run;
+}
+
+// a / b for a >= 0, b > 0, small numbers without the long integer division: (a + 0.5) / b is at least 0.5 / b away from a
+// whole number, 2^-21 of itself for a < 2^20, and __fdividef is off by 2 units, 2^-22, at most.
+TBIK_DEVICE int quotient(int a, int b) {
+  return a < (1 << 20) ? static_cast<int>(__fdividef(static_cast<float>(a) + 0.5f, static_cast<float>(b))) : a / b;
 }
 
 // The group that a tile belongs to: before[g] <= tile < before[g + 1].
@@ -143,13 +185,13 @@ struct ForwardCfg {
   static constexpr uint32_t OFF_TEMPTY = OFF_TFULL + 16;
   static constexpr uint32_t OFF_TMEM_PTR = OFF_TEMPTY + 16;
   static constexpr uint32_t OFF_ABORT = OFF_TMEM_PTR + 4;
-  static constexpr uint32_t OFF_TABLE = OFF_ABORT + 8;  // first[G], last[G], tiles before[G + 1]
-  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + 4 * (3 * groups + 1) + 1024; }
+  static constexpr uint32_t OFF_TABLE = OFF_ABORT + 8;
+  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + Table::bytes(groups) + 1024; }
   static_assert(smem_bytes(TBIK_MAX_GROUPS) <= 232448, "shared memory budget");
   // tokens per tile of a group of m rows: as few tiles as TN allows, evenly filled
   static TBIK_DEVICE int tokens(int m) {
     const int tiles = (m + TN - 1) / TN;
-    return tiles == 0 ? STEP : ((m + tiles - 1) / tiles + STEP - 1) / STEP * STEP;
+    return tiles == 0 ? STEP : (quotient(m + tiles - 1, tiles) + STEP - 1) / STEP * STEP;
   }
 };
 
@@ -173,9 +215,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
   auto empty_bar = [&](int s) { return smem_base + C_::OFF_EMPTY + 8u * s; };
   auto tfull_bar = [&](int a) { return smem_base + C_::OFF_TFULL + 8u * a; };
   auto tempty_bar = [&](int a) { return smem_base + C_::OFF_TEMPTY + 8u * a; };
-  int* first = reinterpret_cast<int*>(smem_gen + C_::OFF_TABLE);
-  int* last = first + p.groups;
-  int* before = last + p.groups;
+  const Table table(smem_gen + C_::OFF_TABLE, p.groups);
 
   if constexpr (PAIR) cluster_sync_all();
   if (threadIdx.x == 0) {
@@ -199,30 +239,34 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
       tmem_relinquish();
     }
   }
-  build_table(p.offsets, p.groups, p.M, first, last, before,
-              [&](int m) { const int n = C_::tokens(m); return (m + n - 1) / n * p.tiles_w; });
+  build_table(p.offsets, p.groups, p.M, table, [&](int m, int& per) {
+    per = C_::tokens(m);
+    return quotient(m + per - 1, per) * p.tiles_w;
+  });
   tc_fence_before_sync();
   if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_ptr_smem;
-  const int num_tiles = before[p.groups];
+  const int num_tiles = table.before[p.groups];
 
   struct Tile {
     int g, t0, tokens, w0;  // group; first token row and number of rows; first weight row
   };
   auto tile_at = [&](int tile) {
-    const int g = group_of(before, p.groups, tile);
-    const int local = tile - before[g], m = last[g] - first[g], n = C_::tokens(m), tiles_t = (m + n - 1) / n;
-    // GROUP_M token tiles share a sweep over the weight's rows
-    const int block = local / (GROUP_M * p.tiles_w);
-    const int in = local - block * GROUP_M * p.tiles_w;
-    const int height = min(tiles_t - block * GROUP_M, GROUP_M);
-    const int tt = block * GROUP_M + in % height;
+    const int g = group_of(table.before, p.groups, tile);
+    const int n = table.per[g], lo = table.first[g], hi = table.last[g];
+    int in = tile - table.before[g], first_tt = 0, height = quotient(hi - lo + n - 1, n);
+    if (height > GROUP_M) {  // GROUP_M token tiles share a sweep over the weight's rows
+      first_tt = quotient(in, GROUP_M * p.tiles_w) * GROUP_M;
+      in -= first_tt * p.tiles_w;
+      height = min(height - first_tt, GROUP_M);
+    }
+    const int tw = quotient(in, height);
     Tile t;
     t.g = g;
-    t.t0 = first[g] + tt * n;
-    t.tokens = min(n, last[g] - t.t0);
-    t.w0 = in / height * C_::W_TILE;
+    t.t0 = lo + (first_tt + in - tw * height) * n;
+    t.tokens = min(n, hi - t.t0);
+    t.w0 = tw * C_::W_TILE;
     return t;
   };
   // token count of the instructions: whole steps
@@ -417,7 +461,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
     if (p.zero_outside) {
       // rows of no group, before the first and behind the last: one warp per row
       const bool vec = (p.ldc * es) % 16 == 0 && (static_cast<int64_t>(p.N) * es) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.C) & 15u) == 0;
-      const int lo = first[0], hi = last[p.groups - 1];
+      const int lo = table.first[0], hi = table.last[p.groups - 1];
       for (int64_t i = static_cast<int64_t>(blockIdx.x) * NUM_EPI_WARPS + warp - EPI_WARP0; i < static_cast<int64_t>(lo) + (p.M - hi);
            i += static_cast<int64_t>(gridDim.x) * NUM_EPI_WARPS) {
         const int64_t row = i < lo ? i : hi + (i - lo);
@@ -603,7 +647,7 @@ struct WgradCfg {
   static constexpr uint32_t OFF_TMEM_PTR = OFF_TEMPTY + 16;
   static constexpr uint32_t OFF_ABORT = OFF_TMEM_PTR + 4;
   static constexpr uint32_t OFF_TABLE = OFF_ABORT + 8;
-  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + 4 * (3 * groups + 1) + 1024; }
+  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + Table::bytes(groups) + 1024; }
   static_assert(smem_bytes(TBIK_MAX_GROUPS) <= 232448, "shared memory budget");
 };
 
@@ -628,9 +672,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
   auto empty_bar = [&](int s) { return smem_base + C_::OFF_EMPTY + 8u * s; };
   auto tfull_bar = [&](int a) { return smem_base + C_::OFF_TFULL + 8u * a; };
   auto tempty_bar = [&](int a) { return smem_base + C_::OFF_TEMPTY + 8u * a; };
-  int* first = reinterpret_cast<int*>(smem_gen + C_::OFF_TABLE);
-  int* last = first + p.groups;
-  int* before = last + p.groups;
+  const Table table(smem_gen + C_::OFF_TABLE, p.groups);
 
   if constexpr (PAIR) cluster_sync_all();
   if (threadIdx.x == 0) {
@@ -654,7 +696,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
       tmem_relinquish();
     }
   }
-  build_table(p.offsets, p.groups, p.M, first, last, before, [&](int) { return p.tiles_r * p.tiles_c; });
+  build_table(p.offsets, p.groups, p.M, table, [&](int, int&) { return 0; });
   tc_fence_before_sync();
   if constexpr (PAIR) cluster_sync_all(); else __syncthreads();
   tc_fence_after_sync();
@@ -666,11 +708,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
   };
   auto tile_at = [&](int tile) {
     const int per = p.tiles_r * p.tiles_c;
-    const int g = tile / per, local = tile - g * per;
-    const int block = local / (GROUP_M * p.tiles_c);
-    const int in = local - block * GROUP_M * p.tiles_c;
-    const int height = min(p.tiles_r - block * GROUP_M, GROUP_M);
-    return Tile{g, first[g], last[g] - first[g], (block * GROUP_M + in % height) * TILE_M, in / height * BN};
+    const int g = quotient(tile, per);
+    int in = tile - g * per, first_row = 0, height = p.tiles_r;
+    if (height > GROUP_M) {
+      first_row = quotient(in, GROUP_M * p.tiles_c) * GROUP_M;
+      in -= first_row * p.tiles_c;
+      height = min(height - first_row, GROUP_M);
+    }
+    const int col = quotient(in, height);
+    return Tile{g, table.first[g], table.last[g] - table.first[g], (first_row + in - col * height) * TILE_M, col * BN};
   };
 
   int role_failed = 0;
