@@ -535,18 +535,18 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
           continue;
         }
         if constexpr (!TREE) {
-          uint32_t raw[2][CHUNK];
-          tmem_ld32(tacc, raw[0]);
+          // A loop, not unrolled code: with few tiles per SM this runs once or twice, and fetching four copies of the body
+          // took longer than draining (one 256-token tile per SM, N = 1000: 13000 cycles).
+#pragma unroll 1
+          for (int c = 0; c < have; ++c) {
+            uint32_t raw[CHUNK];
+            tmem_ld32(tacc + c * C_::EPI_HALVES * CHUNK, raw);
+            tmem_wait_ld();
+            if (c + 1 == have) release();
+            float v[CHUNK];
 #pragma unroll
-          for (int c = 0; c < C_::CHUNKS; ++c) {
-            if (c < have) {
-              tmem_wait_ld();
-              if (c + 1 < C_::CHUNKS && c + 1 < have) tmem_ld32(tacc + (c + 1) * C_::EPI_HALVES * CHUNK, raw[(c + 1) & 1]); else release();
-              float v[CHUNK];
-#pragma unroll
-              for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(raw[c & 1][j]);
-              store_chunk(v, (c * C_::EPI_HALVES + h) * CHUNK);
-            }
+            for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(raw[j]);
+            store_chunk(v, (c * C_::EPI_HALVES + h) * CHUNK);
           }
         } else {
           tmem_wait_st();  // stack stores of earlier leaves have landed
