@@ -41,7 +41,7 @@ constexpr int kManyThreads = 512;    // of a block of the many-rows form
 constexpr int kMaxCluster = 8;
 constexpr int kRouteWarps = 32;      // of a block of the router's own launch
 constexpr int kBackWarps = 8;        // of a block of its gradient
-constexpr int kMaxBlocks = 128;      // of the many-rows form: every block reads all blocks' counts
+constexpr int kMaxBlocks = 128;      // of the many-rows form
 constexpr int kManyRows = 16384;     // rows from which it is taken
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -51,6 +51,9 @@ template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+template <typename T> struct Exponent { static constexpr bool kBf16 = false; };
+template <> struct Exponent<__nv_bfloat16> { static constexpr bool kBf16 = true; };
 
 // Monotone key of a score: larger score, larger key; -0 equals +0; every NaN is the largest key; 0 is below them all.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -63,12 +66,12 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
 }
 
-// The same in 16 bits for 16-bit scores (their upper half of the fp32 pattern would not do for fp16).
-template <typename T> __device__ __forceinline__ uint32_t key16(float v) {
-  if (v != v) return 0xFFFFu;
-  const T h = from_float<T>(v + 0.0f);
-  const uint32_t u = *reinterpret_cast<const uint16_t*>(&h);
-  return (u & 0x8000u) ? (~u & 0xFFFFu) : (u | 0x8000u);
+// The same from a 16-bit score's own bits (u < 2^16), in 16 bits.
+template <typename T> __device__ __forceinline__ uint32_t key16(uint32_t u) {
+  constexpr uint32_t kInf = sizeof(T) == 2 && Exponent<T>::kBf16 ? 0x7F80u : 0x7C00u;
+  const uint32_t size = u & 0x7FFFu;
+  const uint32_t key = (u & 0x8000u) && size != 0u ? (~u & 0xFFFFu) : (size | 0x8000u);
+  return size > kInf ? 0xFFFFu : key;
 }
 template <typename T> __device__ __forceinline__ float value16(uint32_t key) {
   if (key == 0xFFFFu) return __uint_as_float(0x7FC00000u);
@@ -150,10 +153,19 @@ __device__ __forceinline__ int route_token(const RouteParams& p, int64_t t, int 
 template <typename T> struct Key { using type = uint32_t; };
 template <> struct Key<float> { using type = unsigned long long; };
 
+// `raw`: the score's bits
 template <typename T>
-__device__ __forceinline__ typename Key<T>::type packed_key(float v, int e) {
-  if constexpr (sizeof(T) == 2) return (key16<T>(v) << 16) | static_cast<uint32_t>(0xFFFF - e);
-  else return (static_cast<unsigned long long>(key_of(v)) << 32) | static_cast<uint32_t>(~e);
+__device__ __forceinline__ typename Key<T>::type packed_key(uint32_t raw, int e) {
+  if constexpr (sizeof(T) == 2) return (key16<T>(raw) << 16) | static_cast<uint32_t>(0xFFFF - e);
+  else return (static_cast<unsigned long long>(key_of(__uint_as_float(raw))) << 32) | static_cast<uint32_t>(~e);
+}
+template <typename T>
+__device__ __forceinline__ float raw_value(uint32_t raw) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(raw);
+  else {
+    const uint16_t u = static_cast<uint16_t>(raw);
+    return to_float(*reinterpret_cast<const T*>(&u));
+  }
 }
 
 template <typename K>
@@ -198,19 +210,31 @@ __device__ __forceinline__ void route_few(const RouteParams& p, int64_t t, bool 
   using K = typename Key<T>::type;
   const int l = lane & (p.lanes - 1), stride = 8 * p.lanes;
   const T* row = static_cast<const T*>(p.logits) + t * p.ld;
-  auto load = [&](int e, float (&x)[8]) {  // -inf where there is none
-    if (p.aligned) {                       // pieces of eight are whole and on 16-byte boundaries
-      alignas(16) T v[8];
-      if (live && e < p.E) {
+  auto load = [&](int e, uint32_t (&x)[8]) {  // the scores' bits, 0 where there is none
+    if (p.aligned) {                          // pieces of eight are whole and on 16-byte boundaries
+      uint4 v[sizeof(T) / 2];
 #pragma unroll
-        for (int j = 0; j < static_cast<int>(sizeof(T)) / 2; ++j)
-          reinterpret_cast<uint4*>(v)[j] = __ldg(reinterpret_cast<const uint4*>(row + e) + j);
+      for (int j = 0; j < static_cast<int>(sizeof(T)) / 2; ++j)
+        v[j] = live && e < p.E ? __ldg(reinterpret_cast<const uint4*>(row + e) + j) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          const uint4 q = v[j / 4];
+          x[j] = j % 4 == 0 ? q.x : j % 4 == 1 ? q.y : j % 4 == 2 ? q.z : q.w;
+        } else {
+          const uint32_t w = j / 2 == 0 ? v[0].x : j / 2 == 1 ? v[0].y : j / 2 == 2 ? v[0].z : v[0].w;
+          x[j] = j % 2 ? w >> 16 : w & 0xFFFFu;
+        }
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = live && e < p.E ? to_float(v[j]) : -INFINITY;
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = live && e + j < p.E ? to_float(row[e + j]) : -INFINITY;
+      for (int j = 0; j < 8; ++j) {
+        x[j] = 0u;
+        if (live && e + j < p.E) {
+          if constexpr (sizeof(T) == 4) x[j] = __float_as_uint(row[e + j]);
+          else x[j] = *reinterpret_cast<const uint16_t*>(row + e + j);
+        }
+      }
     }
   };
   // the best eight of two descending lists
@@ -219,7 +243,7 @@ __device__ __forceinline__ void route_few(const RouteParams& p, int64_t t, bool 
     for (int i = 0; i < 8; ++i) a[i] = a[i] > b[7 - i] ? a[i] : b[7 - i];
     bitonic_merge<8>(a);
   };
-  float x[8];
+  uint32_t x[8];
   K best[8];
 #pragma unroll 1
   for (int e0 = 0; e0 < p.E; e0 += stride) {
@@ -249,37 +273,38 @@ __device__ __forceinline__ void route_few(const RouteParams& p, int64_t t, bool 
   };
   const float peak = value(best[0]);
   const bool empty = peak == -INFINITY;  // every expert masked
-  float w[8], total = 0.0f;
+  // entry i of the list and its exponential: lane l's first is entry l, with fewer than eight lanes more follow
+  auto entry = [&](int i) {
+    K k = best[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    w[i] = i < p.k && !empty ? expf(value(best[i]) - peak) : 0.0f;
-    total += w[i];
-  }
-  if (!p.renormalize) {
-    total = 0.0f;
+    for (int j = 1; j < 8; ++j) k = i == j ? best[j] : k;
+    return k;
+  };
+  auto weight = [&](int i, K k) { return i < p.k && !empty ? expf(value(k) - peak) : 0.0f; };
+  const K mine = entry(l & 7);
+  const float w = weight(l, mine);
+  float total = 0.0f;
+  if (p.renormalize) {
+    total = w;
+    for (int i = l + p.lanes; i < p.k; i += p.lanes) total += weight(i, entry(i));
+  } else {
 #pragma unroll 1
     for (int e0 = 0; e0 < p.E; e0 += stride) {
       const int e = e0 + 8 * l;
       if (stride < p.E) load(e, x);  // else x still holds them
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (e + j < p.E) total += expf(x[j] - peak);
+        if (e + j < p.E) total += expf(raw_value<T>(x[j]) - peak);
     }
-    for (int d = 1; d < p.lanes; d *= 2) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
   }
+  for (int d = 1; d < p.lanes; d *= 2) total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
   if (!live) return;
 #pragma unroll 1
   for (int i = l; i < p.k; i += p.lanes) {  // the lanes share the writing
-    K mine = best[0];
-    float wi = w[0];
-#pragma unroll
-    for (int j = 1; j < 8; ++j) {
-      mine = i == j ? best[j] : mine;
-      wi = i == j ? w[j] : wi;
-    }
+    const K k = i == l ? mine : entry(i);
     int e;
-    if constexpr (sizeof(T) == 2) e = static_cast<int>(0xFFFFu - (mine & 0xFFFFu)); else e = static_cast<int>(~static_cast<uint32_t>(mine));
-    p.weights[t * p.k + i] = empty ? 0.0f : wi / total;
+    if constexpr (sizeof(T) == 2) e = static_cast<int>(0xFFFFu - (k & 0xFFFFu)); else e = static_cast<int>(~static_cast<uint32_t>(k));
+    p.weights[t * p.k + i] = empty ? 0.0f : (i == l ? w : weight(i, k)) / total;
     p.ids[t * p.k + i] = e;
     if (counts) atomicAdd(&counts[e], 1);
   }
@@ -391,31 +416,35 @@ __device__ __forceinline__ void group_block(const GroupParams& p, int32_t* smem)
     if (live) atomicAdd(&mine[b], 1);
   });
   if constexpr (MANY) {
-    // counts of the other blocks: a warp takes 32 groups and its share of the blocks, sixteen rows in flight
-    const int chunks = (B + 31) / 32, shares = chunks < WARPS ? WARPS / chunks : 1;
-    for (int c = warp; c < chunks * shares; c += WARPS) {
-      const int b = c / shares * 32 + lane;
-      int all = 0, before = 0;
+    // Counts of the other blocks.  Eight neighbours share the reading: each adds up an eighth of the rows -- all of them, and
+    // those before the cluster -- and leaves the sums to the others; what the neighbours before it have it reads itself.
+    // (Every block reading all rows took 6.6k cycles, most of it waiting for the same lines as everyone else.)
+    const int in_cluster = rank % kMaxCluster, first_block = rank - in_cluster;
+    const int chunks = (B + 31) / 32;
+    for (int c = warp; c < chunks; c += WARPS) {
+      const int b = c * 32 + lane;
       if (b < B) {
+        int all = 0, before = 0, near = 0;
         const int32_t* from = p.counts + b;
-        // every block starts elsewhere: all of them want the same rows
-        const int share = c % shares, n = (nb - share + shares - 1) / shares, k0 = rank % n;
-        for (int i = 0; i < n; i += 16) {
-          int v[16];
+        int v[kMaxBlocks / kMaxCluster], u[kMaxCluster - 1];
 #pragma unroll
-          for (int u = 0; u < 16; ++u) {
-            const int k = i + u + k0 < n ? i + u + k0 : i + u + k0 - n;
-            v[u] = i + u < n ? __ldcg(from + static_cast<int64_t>(share + k * shares) * B) : 0;
-          }
-#pragma unroll
-          for (int u = 0; u < 16; ++u) {
-            const int k = i + u + k0 < n ? i + u + k0 : i + u + k0 - n;
-            all += v[u];
-            before += share + k * shares < rank ? v[u] : 0;
-          }
+        for (int i = 0; i < kMaxBlocks / kMaxCluster; ++i) {
+          const int k = i * kMaxCluster + in_cluster;
+          v[i] = k < nb ? __ldcg(from + static_cast<int64_t>(k) * B) : 0;
         }
-        atomicAdd(&totals[b], all);
-        atomicAdd(&earlier[b], before);
+#pragma unroll
+        for (int i = 0; i < kMaxCluster - 1; ++i)
+          u[i] = i < in_cluster && first_block + i < nb ? __ldcg(from + static_cast<int64_t>(first_block + i) * B) : 0;
+#pragma unroll
+        for (int i = 0; i < kMaxBlocks / kMaxCluster; ++i) {
+          all += v[i];
+          before += i * kMaxCluster + in_cluster < first_block ? v[i] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kMaxCluster - 1; ++i) near += u[i];
+        totals[b] = all;
+        earlier[b] = before;
+        first[b] = near;
       }
     }
   }
@@ -431,18 +460,25 @@ __device__ __forceinline__ void group_block(const GroupParams& p, int32_t* smem)
     }
     if constexpr (!MANY) totals[b] = run;
   }
-  if constexpr (MANY) __syncthreads(); else cluster.sync();
-  // scan over the buckets, PER of them per thread
+  if (MANY || nb > 1) cluster.sync(); else __syncthreads();
+  // scan over the buckets, `width` neighbours per thread
   constexpr int PER = (TBIK_MAX_GROUPS + 1 + THREADS - 1) / THREADS;
+  const int width = (B + THREADS - 1) / THREADS;
   int32_t all[PER], before[PER], run = 0;
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const int b = PER * static_cast<int>(threadIdx.x) + u;
+    const int b = width * static_cast<int>(threadIdx.x) + u;
     all[u] = before[u] = 0;
-    if (b < B) {
+    if (u < width && b < B) {
       if constexpr (MANY) {
+        before[u] = first[b];  // (this thread's alone)
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) {
+          all[u] += cluster.map_shared_rank(totals, c)[b];
+          before[u] += cluster.map_shared_rank(earlier, c)[b];
+        }
+      } else if (nb == 1) {
         all[u] = totals[b];
-        before[u] = earlier[b];
       } else {
         for (int c = 0; c < nb; ++c) {
           const int32_t v = cluster.map_shared_rank(totals, c)[b];
@@ -465,14 +501,14 @@ __device__ __forceinline__ void group_block(const GroupParams& p, int32_t* smem)
   for (int w = 0; w < warp; ++w) start += sums[w];
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
-    const int b = PER * static_cast<int>(threadIdx.x) + u;
-    if (b < B) {
+    const int b = width * static_cast<int>(threadIdx.x) + u;
+    if (u < width && b < B) {
       first[b] = start + before[u];
       if (rank == 0) p.offsets[b] = start;
     }
     start += all[u];
   }
-  if constexpr (MANY) __syncthreads(); else cluster.sync();  // nobody leaves while its totals may still be read
+  if (MANY || nb > 1) cluster.sync(); else __syncthreads();  // nobody leaves while its totals may still be read
   const int bits = 32 - __clz(p.groups);  // of a bucket's number
   walk([&](int64_t i, int b, bool live) {
     unsigned peers = __ballot_sync(0xFFFFFFFFu, live);
@@ -510,7 +546,7 @@ __global__ void __launch_bounds__(kGroupThreads) route_group_kernel(const RouteP
   constexpr int WARPS = kGroupThreads / 32;
   route_run<T, V>(r, 0, r.T, blockIdx.x * WARPS + (threadIdx.x >> 5), gridDim.x * WARPS, threadIdx.x & 31, nullptr);
   __threadfence();
-  cg::this_cluster().sync();
+  if (gridDim.x > 1) cg::this_cluster().sync(); else __syncthreads();
   group_block<false>(p, group_smem);
 }
 
@@ -574,8 +610,8 @@ int cluster_size(int64_t M) {
   return c;
 }
 
-// Launches `kernel` on `blocks` blocks: as one cluster, or (after) as a plain grid that may start while the launch before
-// it still runs and waits for it itself.
+// Launches `kernel` on `blocks` blocks: as one cluster, or (after) in clusters of eight that may start while the launch
+// before them still runs and wait for it themselves.
 template <typename... Params>
 int launch_groups(void (*kernel)(Params...), const char* what, int blocks, int threads, size_t smem, bool after, cudaStream_t stream,
                   const Params&... params) {
@@ -589,18 +625,15 @@ int launch_groups(void (*kernel)(Params...), const char* what, int blocks, int t
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  if (after) {
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-  } else {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(blocks);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-  }
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(after ? kMaxCluster : blocks);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = after ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, params...);
   return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, what);
 }
@@ -636,7 +669,7 @@ int route_launch(const RouteParams& r, GroupParams g, cudaStream_t stream) {
   route_kernel<T, V><<<static_cast<unsigned>(g.blocks), kRouteWarps * 32, 0, stream>>>(r, g);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "route_kernel launch");
-  return launch_groups(group_many_kernel, "group_many_kernel launch", g.blocks, kManyThreads, group_smem_bytes(g.groups, kManyThreads),
+  return launch_groups(group_many_kernel, "group_many_kernel launch", (g.blocks + kMaxCluster - 1) / kMaxCluster * kMaxCluster, kManyThreads, group_smem_bytes(g.groups, kManyThreads),
                        true, stream, g);
 }
 
@@ -689,7 +722,7 @@ int group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_
   count_kernel<<<static_cast<unsigned>(g.blocks), kManyThreads, 0, stream>>>(g);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "count_kernel launch");
-  return launch_groups(group_many_kernel, "group_many_kernel launch", g.blocks, kManyThreads, group_smem_bytes(groups, kManyThreads),
+  return launch_groups(group_many_kernel, "group_many_kernel launch", (g.blocks + kMaxCluster - 1) / kMaxCluster * kMaxCluster, kManyThreads, group_smem_bytes(groups, kManyThreads),
                        true, stream, g);
 }
 
