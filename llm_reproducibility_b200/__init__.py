@@ -3,6 +3,10 @@
 Sub-packages mirror the reference project's importable surface:
   tbik.tree_based_matmul       matmul_tp_persistent
   tbik.tree_based_all_reduce   tree_all_reduce_sum, tree_all_reduce_sum_native
+  tbik.autograd                tree_matmul, tree_linear, tree_grouped_linear, tree_route_topk (differentiable)
+  tbik.grouped_matmul          grouped_matmul_tp_persistent, grouped_weight_gradient (products by expert)
+  tbik.row_groups              route_topk, group_rows (router, rows grouped by id)
+  tbik.adapters                lora_add, lora_shrink, lora_expand_add (low-rank adapters of many requests)
   mini_allreduce               CustomAllreduce, CustomTreeAllreduce, custom_all_reduce_ops
   patch                        apply_patches, patch_tp_invariant
   utils                        environment switches

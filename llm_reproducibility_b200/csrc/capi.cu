@@ -24,7 +24,7 @@ extern "C" {
 
 const char* tbik_last_error(void) { return tbik::g_last_error; }
 
-int tbik_version(void) { return 1000; }
+int tbik_version(void) { return 1001; }
 
 int tbik_tree_shape(int64_t K, int leaf, int* T, int* F, int* L) {
   if (!T || !F || !L) return tbik::set_error(TBIK_ERR_ARG, "tbik_tree_shape: null output pointer");

@@ -100,12 +100,15 @@ def test_shards_of_k_add_up_to_the_unsharded_bits(K, tp):
     assert torch.equal(parts[0], lora_shrink(x, A, groups))
 
 
-def test_a_row_has_the_same_bits_in_every_batch():
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R", [8, 16, 24, 32, 40, 64, 128])
+def test_a_row_has_the_same_bits_in_every_batch(R, dtype):
+    """One row, a decode batch, prompts: tiles and their work differ, the bits do not."""
     from llm_reproducibility_b200.tbik.adapters import lora_add
     from llm_reproducibility_b200.tbik.row_groups import group_rows
-    y, x, A, B, ids, s = case(3000, 6, 16, 1032, 328, torch.bfloat16, "normal", none=0.1)
+    y, x, A, B, ids, s = case(3000, 6, R, 1032, 328, dtype, "normal", none=0.1)
     full = lora_add(y, x, A, B, group_rows(ids, 6), s)
-    for rows in (slice(0, 1), slice(5, 9), slice(100, 140), slice(700, 1900)):
+    for rows in (slice(0, 1), slice(5, 9), slice(100, 140), slice(500, 1524), slice(700, 1725)):
         part = lora_add(y[rows], x[rows], A, B, group_rows(ids[rows], 6), s)
         assert torch.equal(part, full[rows])
 
@@ -200,3 +203,34 @@ def test_streams_and_a_graph_that_follows_new_ids():
         ids.copy_((torch.arange(64, device="cuda") * shift) % 7 - 1)
         graph.replay()
         assert torch.equal(out, ref(y, x, A, B, torch.where(ids < 5, ids, -1), s)[0].to(torch.bfloat16))
+
+
+def test_rows_beyond_32_bit_offsets():
+    """More than 2^31 elements in y: rows at the end of a long batch."""
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    T, N, K, R = 140000, 16384, 64, 16
+    ids = (torch.arange(T, device="cuda") % 3 - 1).to(torch.int32)
+    x, A, B = make((T, K), torch.bfloat16, "int", 1), make((2, R, K), torch.bfloat16, "int", 2), make((2, N, R), torch.bfloat16, "int", 3)
+    y = torch.ones(T, N, dtype=torch.bfloat16, device="cuda")
+    assert y.numel() > 1 << 31
+    s = torch.tensor([1.0, 2.0], device="cuda")
+    lora_add(y, x, A, B, group_rows(ids, 2), s, out=y)
+    for rows in (slice(0, 50), slice(131060, 131100), slice(T - 50, T)):
+        want = ref(torch.ones(rows.stop - rows.start, N, dtype=torch.bfloat16, device="cuda"), x[rows], A, B, ids[rows], s)[0]
+        assert torch.equal(y[rows], want.to(torch.bfloat16))
+
+
+def test_refusals_on_the_device():
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    y, x, A, B, ids, s = case(20, 3, 16, 64, 64, torch.bfloat16, "int")
+    g = group_rows(ids, 3)
+    buf = torch.zeros(21, 64, dtype=torch.bfloat16, device="cuda")
+    for bad_y, out in ((y, x), (buf[:20], buf[1:]), (y, torch.empty(20, 64, device="cuda")), (y, torch.empty(20, 68, dtype=torch.bfloat16, device="cuda")[:, 4:])):
+        with pytest.raises(ValueError, match="out"):
+            lora_add(bad_y, x, A, B, g, s, out=out)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        lora_add(y, x, A, B, g, s.cpu())
+    with pytest.raises(ValueError, match="offsets"):
+        lora_add(y, x, A, B, group_rows(ids, 4), s)

@@ -138,13 +138,16 @@ def test_a_group_with_nan_leaves_the_others_alone():
         assert torch.equal(dW[[0, 2, 3, 4]], grad[[0, 2, 3, 4]])
 
 
-@pytest.mark.parametrize("K,leaf", [(512, 64), (768, 192), (4096, 512), (1536, 256), (64, 64), (2048, 128)])
-def test_tree_over_k(K, leaf):
+@pytest.mark.parametrize("w_n_contiguous", [False, True])
+@pytest.mark.parametrize("K,leaf", [(512, 64), (768, 192), (4096, 512), (1536, 256), (64, 64), (2048, 128), (16384, 64)])
+def test_tree_over_k(K, leaf, w_n_contiguous):
     """The leaves' sums are joined in the framework's tree: same value, and shards of K add up to the unsharded bits."""
     from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent
     from llm_reproducibility_b200.tbik.tree_based_matmul import tree_shape
     M, G, N = 300, 4, 200
     A, W = make((M, K), torch.bfloat16, "normal", 11), make((G, N, K), torch.bfloat16, "normal", 12, 0.1)
+    if w_n_contiguous:
+        W = W.transpose(1, 2).contiguous().transpose(1, 2)
     off = offsets_of(ragged(M, G, 5)).cuda()
     value, size = forward_ref(A, W, off)
     full = grouped_matmul_tp_persistent(A, W, off, leaf=leaf)
@@ -350,3 +353,73 @@ def test_first_cuda_call_of_a_host_thread():
         t.join()
         torch.cuda.synchronize()
         assert torch.is_tensor(got[0]) and torch.equal(got[0], expected), got[0]
+
+
+def test_results_beyond_32_bit_offsets():
+    """More than 2^31 elements in C and in dW."""
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent, grouped_weight_gradient
+    M, N, K = 270000, 8192, 16
+    A, W = make((M, K), torch.bfloat16, "int", 1), make((3, N, K), torch.bfloat16, "int", 2)
+    off = torch.tensor([0, 100000, 262200, M - 5], dtype=torch.int32, device="cuda")
+    C = grouped_matmul_tp_persistent(A, W, off)
+    for g, rows in ((0, slice(0, 40)), (1, slice(262144, 262200)), (2, slice(M - 60, M - 5))):
+        assert torch.equal(C[rows], (A[rows].double() @ W[g].double().t()).to(torch.bfloat16))
+    assert (C[M - 5:] == 0).all()
+    del C
+    D, X = make((64, 33000), torch.bfloat16, "int", 3), make((64, 33000), torch.bfloat16, "int", 4)
+    dW = grouped_weight_gradient(D, X, torch.tensor([0, 10, 64], dtype=torch.int32, device="cuda"))
+    assert dW.numel() > 1 << 31
+    for g, (lo, hi) in enumerate(((0, 10), (10, 64))):
+        for n in (0, 32999):
+            assert torch.equal(dW[g, n], (D[lo:hi, n].double() @ X[lo:hi].double()).to(torch.bfloat16))
+
+
+def test_forward_and_gradients_captured_in_a_graph():
+    from llm_reproducibility_b200.tbik.autograd import tree_grouped_linear
+    off = offsets_of([70, 0, 130]).cuda()
+    x, w = make((200, 128), torch.bfloat16, "int", 1).requires_grad_(True), make((3, 256, 128), torch.bfloat16, "int", 2).requires_grad_(True)
+    dy = make((200, 256), torch.bfloat16, "int", 3)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(tree_grouped_linear(x, w, off), (x, w), dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = tree_grouped_linear(x, w, off)
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+    with torch.no_grad():
+        x.copy_(make((200, 128), torch.bfloat16, "int", 7))
+        off.copy_(torch.tensor([0, 33, 150, 199], dtype=torch.int32))
+    graph.replay()
+    assert torch.equal(y, forward_ref(x.detach(), w.detach(), off)[0].to(torch.bfloat16))
+    assert torch.equal(dw, wgrad_ref(dy, x.detach(), off)[0].to(torch.bfloat16))
+    at = off.tolist()
+    for g, (lo, hi) in enumerate(zip(at, at[1:])):
+        assert torch.equal(dx[lo:hi], (dy[lo:hi].double() @ w[g].detach().double()).to(torch.bfloat16))
+    assert (dx[199:] == 0).all()
+
+
+def test_no_rows_at_all_and_second_derivatives():
+    from llm_reproducibility_b200.tbik.autograd import tree_grouped_linear
+    w = make((2, 16, 8), torch.bfloat16, "int", 1).requires_grad_(True)
+    x = torch.zeros(0, 8, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    tree_grouped_linear(x, w, torch.zeros(3, dtype=torch.int32, device="cuda")).sum().backward()
+    assert x.grad.shape == (0, 8) and (w.grad == 0).all()
+    x = make((4, 8), torch.bfloat16, "int", 2).requires_grad_(True)
+    (g,) = torch.autograd.grad(tree_grouped_linear(x, w, offsets_of([2, 2]).cuda()).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_refusals_on_the_device():
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent as f
+    A, W, off = make((8, 64), torch.bfloat16, "int", 1), make((2, 64, 64), torch.bfloat16, "int", 2), offsets_of([4, 4]).cuda()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        f(A, W, off.cpu())
+    for out in (torch.empty(8, 63, dtype=torch.bfloat16, device="cuda"), torch.empty(8, 64, device="cuda"),
+                torch.empty(64, 8, dtype=torch.bfloat16, device="cuda").t(), torch.empty(1, 64, dtype=torch.bfloat16, device="cuda").expand(8, 64)):
+        with pytest.raises(ValueError, match="out must"):
+            f(A, W, off, out=out)
+    with pytest.raises(ValueError, match="overlaps"):
+        f(A, W, off, out=A)

@@ -57,7 +57,8 @@ def route_ref(x, k, renormalize):
 
 
 CASES = [(1, 1, 1), (1, 128, 8), (3, 2, 2), (5, 33, 32), (64, 64, 6), (512, 128, 8), (513, 128, 8), (777, 60, 4), (9, 257, 16),
-         (40, 1024, 32), (2000, 512, 10), (4099, 8, 2)]
+         (40, 1024, 32), (2000, 512, 10), (4099, 8, 2),
+         (0, 4, 2), (40, 1024, 8), (7, 300, 8), (5, 8, 8), (3, 5, 3), (2000, 16, 2), (64, 17, 5), (20000, 128, 8), (17000, 24, 1)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -75,7 +76,7 @@ def test_route(T, E, k, renormalize, dtype):
     # the sum of up to E terms by E 2^-24 at the very most, the quotient by 2^-24
     tol = (4 + 20 + E) * 2.0 ** -23
     assert ((r.weights.cpu().double() - w).abs() <= tol * w + 1e-38).all()
-    if renormalize:
+    if renormalize and T:
         assert (r.weights.sum(1) - 1).abs().max() < tol
 
 
@@ -169,7 +170,7 @@ def test_gradient_of_a_masked_row_is_zero():
         assert torch.equal(leaf.grad, torch.zeros_like(leaf.grad))
 
 
-@pytest.mark.parametrize("T", [4, 3000])
+@pytest.mark.parametrize("T", [4, 3000, 20000])
 def test_route_on_another_stream_and_in_a_graph(T):
     from llm_reproducibility_b200.tbik.row_groups import route_topk
     x = torch.randn(T, 64, device="cuda")
@@ -189,3 +190,19 @@ def test_route_on_another_stream_and_in_a_graph(T):
         want = route_topk(x, 4)
         for a, b in zip((r.weights, r.ids, *r.groups), (want.weights, want.ids, *want.groups)):
             assert torch.equal(a, b)
+
+
+def test_gradient_of_no_tokens():
+    from llm_reproducibility_b200.tbik.autograd import tree_route_topk
+    x = torch.zeros(0, 8, device="cuda", requires_grad=True)
+    r = tree_route_topk(x, 2)
+    r.weights.sum().backward()
+    assert x.grad.shape == (0, 8) and r.groups.offsets.tolist() == [0] * 9
+
+
+def test_a_second_derivative_is_refused():
+    from llm_reproducibility_b200.tbik.autograd import tree_route_topk
+    x = torch.randn(4, 8, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(tree_route_topk(x, 2).weights[:, 0].sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
