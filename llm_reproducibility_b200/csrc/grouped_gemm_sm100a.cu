@@ -140,6 +140,10 @@ TBIK_DEVICE int quotient(int a, int b) {
   return a < (1 << 20) ? static_cast<int>(__fdividef(static_cast<float>(a) + 0.5f, static_cast<float>(b))) : a / b;
 }
 
+// Keeps the compiler from working out all of an unrolled loop's addresses ahead, in registers that are not there.
+template <typename V>
+TBIK_DEVICE void one_by_one(V*& p) { asm volatile("" : "+l"(p)); }
+
 // The group that a tile belongs to: before[g] <= tile < before[g + 1].
 TBIK_DEVICE int group_of(const int* before, int groups, int tile) {
   int lo = 0, hi = groups;
@@ -479,6 +483,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
       const Tile t = tile_at(tile);
       const int n0 = t.w0 + cta_rank * W_ROWS + q * 32;  // this warp's 32 columns of C
       const bool busy = h < C_::EPI_HALVES && q * 32 < W_ROWS && n0 < p.N;
+      const bool whole = pairs_ok && n0 + 32 <= p.N;
       // v[j]: column n0 + lane of token row tok + j.  A lane holds one column of 32 rows: lanes 2i and 2i + 1 swap halves
       // of two rows, so that a store instruction writes 64 whole bytes of each of two rows.
       auto store_chunk = [&](const float (&v)[CHUNK], int tok) {
@@ -488,26 +493,33 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
           const bool in = n0 + lane < p.N;
 #pragma unroll
           for (int j = 0; j < CHUNK; ++j, dst += p.ldc)
+          {
             if (j < left && in) *dst = v[j];
+            one_by_one(dst);
+          }
           return;
         }
-        const bool odd = (lane & 1) != 0;
-        const int col = lane & ~1;
-        uint16_t* dst = static_cast<uint16_t*>(p.C) + static_cast<int64_t>(t.t0 + tok + (lane & 1)) * p.ldc + n0 + col;
-        const bool both = pairs_ok && n0 + col + 1 < p.N, one = n0 + col < p.N, two = n0 + col + 1 < p.N;
+        if (whole) {
+          // every column exists and pairs of columns are aligned: straight-line code, a store is predicated on its row alone
+          const bool odd = (lane & 1) != 0;
+          uint16_t* dst = static_cast<uint16_t*>(p.C) + static_cast<int64_t>(t.t0 + tok + (lane & 1)) * p.ldc + n0 + (lane & ~1);
 #pragma unroll
-        for (int j = 0; j < CHUNK; j += 2, dst += 2 * p.ldc) {
-          const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1);
-          const float lo = odd ? other : v[j], hi = odd ? v[j + 1] : other;
-          const uint32_t w = p.half ? Pack16<__nv_bfloat16>::from_f32(lo, hi) : Pack16<__half>::from_f32(lo, hi);
-          if (j + (lane & 1) < left) {
-            if (both) {
-              *reinterpret_cast<uint32_t*>(dst) = w;
-            } else {
-              if (one) dst[0] = static_cast<uint16_t>(w & 0xFFFFu);
-              if (two) dst[1] = static_cast<uint16_t>(w >> 16);
-            }
+          for (int j = 0; j < CHUNK; j += 2, dst += 2 * p.ldc) {
+            const float other = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1);
+            const float lo = odd ? other : v[j], hi = odd ? v[j + 1] : other;
+            const uint32_t w = p.half ? Pack16<__nv_bfloat16>::from_f32(lo, hi) : Pack16<__half>::from_f32(lo, hi);
+            if (j + (lane & 1) < left) *reinterpret_cast<uint32_t*>(dst) = w;
+            one_by_one(dst);
           }
+          return;
+        }
+        uint16_t* dst = static_cast<uint16_t*>(p.C) + static_cast<int64_t>(t.t0 + tok) * p.ldc + n0 + lane;
+        const bool in = n0 + lane < p.N;
+#pragma unroll
+        for (int j = 0; j < CHUNK; ++j, dst += p.ldc) {
+          const uint32_t w = p.half ? Pack16<__nv_bfloat16>::from_f32(v[j], 0.0f) : Pack16<__half>::from_f32(v[j], 0.0f);
+          if (j < left && in) *dst = static_cast<uint16_t>(w & 0xFFFFu);
+          one_by_one(dst);
         }
       };
       // the open level-0 group, then the node that climbs the tree: fp32 in the registers that tcgen05.ld fills
