@@ -80,7 +80,7 @@ def _check_leaf(what, K: int, leaf: Optional[int]) -> int:
 def _check_out(what, y, out, *others):
     """The result's tensor.  It is written while the operands are read: it may be y itself, and else overlaps nothing."""
     if out is None:
-        return empty(y.shape[0], y.shape[1], y.dtype, y.device)
+        return torch.empty_like(y) if y.is_contiguous() else empty(y.shape[0], y.shape[1], y.dtype, y.device)
     same = out.data_ptr() == y.data_ptr() and out.stride() == y.stride()
     if any(overlap(out, t) for t in others + (() if same else (y,))):
         raise ValueError(f"{what}: out overlaps an operand")
@@ -90,16 +90,17 @@ def _check_out(what, y, out, *others):
     return out
 
 
-def _launch(what, dev, x, y, out, A, B, scales, h, groups, T, N, K, R, adapters, dtype, leaf):
-    order, offsets = groups.order.contiguous(), groups.offsets.contiguous()
-    px = ldx = py = ldy = po = ldo = 0
+def _launch(dev, x, y, out, A, B, scales, h, groups, T, N, K, R, adapters, dtype, leaf):
+    order, _, offsets = groups
+    order, offsets = order.contiguous(), offsets.contiguous()
+    px = ldx = pa = py = ldy = po = ldo = pb = ps = 0
     if x is not None:
-        px, ldx = x.data_ptr(), max(x.stride(0), K)
+        px, ldx, pa = x.data_ptr(), max(x.stride(0), K), A.data_ptr()
     if y is not None:
         py, ldy, po, ldo = y.data_ptr(), max(y.stride(0), N), out.data_ptr(), max(out.stride(0), N)
-    launch("tbik_adapters", dev, px, ldx, py, ldy, po, ldo, A.data_ptr() if A is not None else 0, B.data_ptr() if B is not None else 0,
-           scales.data_ptr() if scales is not None else 0, h.data_ptr() if h is not None else 0, order.data_ptr(), offsets.data_ptr(),
-           T, N, K, R, adapters, _DTYPE_CODE[dtype], leaf)
+        pb, ps = B.data_ptr(), scales.data_ptr()
+    launch("tbik_adapters", dev, px, ldx, py, ldy, po, ldo, pa, pb, ps, 0 if h is None else h.data_ptr(), order.data_ptr(),
+           offsets.data_ptr(), T, N, K, R, adapters, _DTYPE_CODE[dtype], leaf)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, groups: RowGroups, scales: torch.Tensor, *,
@@ -111,20 +112,21 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     rounded once.  Returns a new tensor, or `out`, which may be y itself."""
     what = "lora_add"
     refuse_grad(what, "adapters are a serving operator", y, x, A, B, scales)
-    if y.dim() != 2 or x.dim() != 2 or A.dim() != 3 or B.dim() != 3 or y.shape[0] != x.shape[0] or A.shape[0] != B.shape[0] or \
-            A.shape[1] != B.shape[2] or A.shape[2] != x.shape[1] or B.shape[1] != y.shape[1]:
-        raise ValueError(f"{what}: y [T, N], x [T, K], A [L, R, K], B [L, N, R]; got {tuple(y.shape)}, {tuple(x.shape)}, "
-                         f"{tuple(A.shape)}, {tuple(B.shape)}")
+    shape_y, shape_x, shape_a, shape_b = y.shape, x.shape, A.shape, B.shape
+    if len(shape_y) != 2 or len(shape_x) != 2 or len(shape_a) != 3 or shape_y[0] != shape_x[0] or shape_a[2] != shape_x[1] or \
+            shape_b != (shape_a[0], shape_y[1], shape_a[1]):
+        raise ValueError(f"{what}: y [T, N], x [T, K], A [L, R, K], B [L, N, R]; got {tuple(shape_y)}, {tuple(shape_x)}, "
+                         f"{tuple(shape_a)}, {tuple(shape_b)}")
     _types(what, x, y, A, B)
-    (T, K), N, (L, R, _) = x.shape, y.shape[1], A.shape
+    (T, K), N, (L, R, _) = shape_x, shape_y[1], shape_a
     if scales.shape != (L,) or scales.dtype != torch.float32:
         raise ValueError(f"{what}: scales must be [{L}] float32, got {tuple(scales.shape)} of {scales.dtype}")
     leaf = _check_leaf(what, K, leaf)
     dev = _check(what, T, groups, L, R, (K, N), x, y, A, B, scales)
     res = _check_out(what, y, out, x, A, B)
     if T:
-        src = y if res.data_ptr() == y.data_ptr() and res.stride() == y.stride() else _rows16(y)
-        _launch(what, dev, _rows16(x), src, res, _weights16(A), _weights16(B), scales.contiguous(), None, groups, T, N, K, R, L,
+        src = y if res is y or (res.data_ptr() == y.data_ptr() and res.stride() == y.stride()) else _rows16(y)
+        _launch(dev, _rows16(x), src, res, _weights16(A), _weights16(B), scales.contiguous(), None, groups, T, N, K, R, L,
                 x.dtype, leaf)
     return res
 
@@ -143,7 +145,7 @@ def lora_shrink(x: torch.Tensor, A: torch.Tensor, groups: RowGroups, *, leaf: Op
     dev = _check(what, T, groups, L, R, (K,), x, A)
     h = empty(T, R, torch.float32, dev)
     if T:
-        _launch(what, dev, _rows16(x), None, None, _weights16(A), None, None, h, groups, T, 8, K, R, L, x.dtype, leaf)
+        _launch(dev, _rows16(x), None, None, _weights16(A), None, None, h, groups, T, 8, K, R, L, x.dtype, leaf)
     return h
 
 
@@ -164,6 +166,6 @@ def lora_expand_add(y: torch.Tensor, h: torch.Tensor, B: torch.Tensor, groups: R
     dev = _check(what, T, groups, L, R, (N,), y, h, B, scales)
     res = _check_out(what, y, out, h, B)
     if T:
-        src = y if res.data_ptr() == y.data_ptr() and res.stride() == y.stride() else _rows16(y)
-        _launch(what, dev, None, src, res, None, _weights16(B), scales.contiguous(), _weights16(h), groups, T, N, 8, R, L, y.dtype, 0)
+        src = y if res is y or (res.data_ptr() == y.data_ptr() and res.stride() == y.stride()) else _rows16(y)
+        _launch(dev, None, src, res, None, _weights16(B), scales.contiguous(), _weights16(h), groups, T, N, 8, R, L, y.dtype, 0)
     return res

@@ -13,6 +13,7 @@ import torch
 from .. import _lib
 from .tree_based_matmul import _raw_stream
 
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _LOGITS_CODE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_FP16, torch.float32: _lib.DTYPE_FP32}
 
 
@@ -35,9 +36,8 @@ class Routing(NamedTuple):
 def launch(name: str, device: torch.device, *args) -> None:
     """Call the library's function `name` with `args` and, as its last argument, the current stream of `device`, which is
     made the current device for the call."""
-    fn = getattr(_lib.lib(), name)
-    index = device.index
-    if torch.cuda.current_device() == index:
+    fn, index = getattr(_lib.lib(), name), device.index
+    if _current_device() == index:  # (the callers hold CUDA tensors: there is a device)
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
