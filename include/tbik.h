@@ -332,8 +332,8 @@ int tbik_grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32
  * (h [T, R] fp32; rows of no adapter get zeros); `x` and A null: h is read instead of computed.  A row-split layer uses
  * the last two with the fixed-order sum of the ranks' h in between.
  * leaf: 0 = K/8 rounded up to a multiple of 32; else a multiple of 32 with at most 8 leaves covering K.
- * T below 2^25; R a multiple of 8, at most TBIK_MAX_RANK; K, N multiples of 8; pointers 16-byte aligned, strides multiples
- * of 8. */
+ * T below 2^25; R a multiple of 8, at most TBIK_MAX_RANK; K, N multiples of 8 below 2^24; pointers 16-byte aligned, strides
+ * multiples of 8. */
 #define TBIK_MAX_RANK 128
 int tbik_adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, int64_t ldo, const void* A,
                   const void* B, const float* scales, float* h, const int32_t* order, const int32_t* offsets, int64_t T,

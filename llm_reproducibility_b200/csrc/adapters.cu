@@ -10,10 +10,10 @@
 // second product the columns are permuted the same way, so that a lane ends up with 8 neighbouring results.
 //
 // One cluster of 1 .. 8 CTAs per (adapter, tile of rows), both products in one launch.  The CTAs split K by leaves, add
-// the leaves through distributed shared memory, and split N for the second product.  Few rows: 16-row tiles and bulk
-// copies of the leaf into shared memory, so that a decode step pays one memory latency; many rows: 32-row tiles, one
-// leaf per warp, operands straight into registers.  Either way a leaf is one chain of instructions over its columns, so
-// a row's bits depend on the row and its adapter alone.
+// the leaves through distributed shared memory, and split N for the second product.  Few rows: 16-row tiles and
+// asynchronous copies of a leaf into shared memory, so that a decode step pays one memory latency; many rows: 64-row tiles in
+// two groups of warps, whose warps take a leaf or a part of its columns each, operands straight into registers.  Either way
+// a leaf is one chain of instructions over its columns, so a row's bits depend on the row and its adapter alone.
 //
 // h is held in fp32; the second product reads it as the sum of two values of the operand type (16 bits of mantissa for
 // bf16, 22 for fp16, whose rows are scaled by a power of two into its range first).
@@ -21,6 +21,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "ptx_sm100a.cuh"
@@ -93,8 +94,8 @@ TBIK_DEVICE void prefetch_l2(const void* src, uint32_t bytes) {
 
 TBIK_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Shared memory: [rows TM][item 4][row factors TM] | leaf sums [8 / cluster][TM][R] | h [TM][R] |
-// h as operand [MT][ceil(R / 16)][32 lanes] x 32 bytes | two staging buffers
+// Shared memory: [rows TM][item 4], at 512 [row factors TM] | leaf sums [8 / cluster][TM][R] | h [TM][R] |
+// h as operand [TM / 16][ceil(R / 16)][32 lanes] x 32 bytes | two staging buffers
 struct Layout {
   uint32_t sums, h, frags, stage, total;
 };
@@ -118,16 +119,14 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   const Layout lay = layout<MT, RG, STAGED>(p.R, p.cluster);
   int* rows = reinterpret_cast<int*>(smem);                 // row index or -1
   int* item = rows + TM;                                    // adapter, first place, rows
-  float* factor = reinterpret_cast<float*>(smem + 512);     // what a row of h was divided by (fp16)
+  float* factor = reinterpret_cast<float*>(smem + 512);     // what a row of h was multiplied by (fp16)
   float* sums = reinterpret_cast<float*>(smem + lay.sums);
   float* hs = reinterpret_cast<float*>(smem + lay.h);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int C = p.cluster, rank = static_cast<int>(blockIdx.x) % C, want = static_cast<int>(blockIdx.x) / C;
   const int R = p.R, K = p.K;
 
-  if (tid == 0) {
-    item[0] = -2;
-  }
+  if (tid == 0) item[0] = -2;  // no item
   // ---- which adapter and rows: tiles of the groups in order, then tiles of the rows of no adapter
   {
     int* warp_sum = reinterpret_cast<int*>(smem + lay.sums);  // free until the leaves' sums
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
       // 16-byte pieces that 8 lanes read together lie in different banks.
       const uint32_t stage = stage_bytes(R), lines = static_cast<uint32_t>(R + count);
       const int whole = (p.leaf + 63) / 64 * 64;
-      const bool once = lines * (static_cast<uint32_t>(whole) * 2 + 64) <= 2 * stage;
+      const bool once = whole <= static_cast<int>((2 * stage / lines - 64) / 2);
       const int cols = once ? whole : static_cast<int>((stage / lines - 64) / 128 * 64);
       const uint32_t pitch = static_cast<uint32_t>(cols) * 2 + 64, second = once ? 0u : stage;
       const int per_leaf = ceil_div(p.leaf, cols), steps = own * per_leaf, ahead = once ? 1 : 2;
@@ -329,66 +328,66 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
       // groups read the same rows of A at about the same time: the second finds them in L1.
       const int parts = own < W ? W / own : 1, part = w % parts;
       for (int slot = w / parts; slot < own; slot += W / parts) {
-      const int leaf = rank * own + slot;
-      const int64_t kb = min(static_cast<int64_t>(leaf) * p.leaf, static_cast<int64_t>(K));
-      const int k0 = static_cast<int>(kb), k1 = static_cast<int>(min(kb + p.leaf, static_cast<int64_t>(K)));
-      // rows and column tiles beyond what there is repeat the last one; their results are not read
-      const T* xr[2 * MT];
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) xr[i] = x + static_cast<int64_t>(max(rows[min(first_row + i * 8 + g, count - 1)], 0)) * p.ldx + c * 8;
-      float* out = sums + (slot * TM + first_row) * R;
-      for (int n0 = part; n0 < ntiles; n0 += 4 * parts) {
-        float acc[MT][4][4];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
-        const T* ar[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ar[i] = A + static_cast<int64_t>(min(n0 + i * parts, ntiles - 1) * 8 + g) * K + c * 8;
-        // `in`: the lane's piece of the run of 32 columns exists
-        auto load = [&](int k, bool in, uint4 (&a)[2 * MT], uint4 (&b)[4]) {
-#pragma unroll
-          for (int i = 0; i < 2 * MT; ++i) a[i] = in ? load_stream(xr[i] + k) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) b[i] = in ? __ldg(reinterpret_cast<const uint4*>(ar[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
-        };
-        auto multiply = [&](const uint4 (&a)[2 * MT], const uint4 (&b)[4]) {
-#pragma unroll
+        const int leaf = rank * own + slot;
+        const int64_t kb = min(static_cast<int64_t>(leaf) * p.leaf, static_cast<int64_t>(K));
+        const int k0 = static_cast<int>(kb), k1 = static_cast<int>(min(kb + p.leaf, static_cast<int64_t>(K)));
+        // rows and column tiles beyond what there is repeat the last one; their results are not read
+        const T* xr[2 * MT];
+  #pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) xr[i] = x + static_cast<int64_t>(max(rows[min(first_row + i * 8 + g, count - 1)], 0)) * p.ldx + c * 8;
+        float* out = sums + (slot * TM + first_row) * R;
+        for (int n0 = part; n0 < ntiles; n0 += 4 * parts) {
+          float acc[MT][4][4];
+  #pragma unroll
           for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].x, a[2 * m + 1].x, a[2 * m].y, a[2 * m + 1].y), b[i].x, b[i].y);
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].z, a[2 * m + 1].z, a[2 * m].w, a[2 * m + 1].w), b[i].z, b[i].w);
-        };
-        // the next run is on its way while one is multiplied
-        uint4 a[2][2 * MT], b[2][4];
-        load(k0, k0 + c * 8 < k1, a[0], b[0]);
-#pragma unroll 1
-        for (int k = k0; k < k1; k += 64) {
-          if (k + 32 < k1) load(k + 32, k + 32 + c * 8 < k1, a[1], b[1]);
-          multiply(a[0], b[0]);
-          if (k + 32 < k1) {
-            if (k + 64 < k1) load(k + 64, k + 64 + c * 8 < k1, a[0], b[0]);
-            multiply(a[1], b[1]);
+  #pragma unroll
+            for (int i = 0; i < 4; ++i)
+  #pragma unroll
+              for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
+          const T* ar[4];
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) ar[i] = A + static_cast<int64_t>(min(n0 + i * parts, ntiles - 1) * 8 + g) * K + c * 8;
+          // `in`: the lane's piece of the run of 32 columns exists
+          auto load = [&](int k, bool in, uint4 (&a)[2 * MT], uint4 (&b)[4]) {
+  #pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) a[i] = in ? load_stream(xr[i] + k) : make_uint4(0u, 0u, 0u, 0u);
+  #pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = in ? __ldg(reinterpret_cast<const uint4*>(ar[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
+          };
+          auto multiply = [&](const uint4 (&a)[2 * MT], const uint4 (&b)[4]) {
+  #pragma unroll
+            for (int m = 0; m < MT; ++m)
+  #pragma unroll
+              for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].x, a[2 * m + 1].x, a[2 * m].y, a[2 * m + 1].y), b[i].x, b[i].y);
+  #pragma unroll
+            for (int m = 0; m < MT; ++m)
+  #pragma unroll
+              for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].z, a[2 * m + 1].z, a[2 * m].w, a[2 * m + 1].w), b[i].z, b[i].w);
+          };
+          // the next run is on its way while one is multiplied
+          uint4 a[2][2 * MT], b[2][4];
+          load(k0, k0 + c * 8 < k1, a[0], b[0]);
+  #pragma unroll 1
+          for (int k = k0; k < k1; k += 64) {
+            if (k + 32 < k1) load(k + 32, k + 32 + c * 8 < k1, a[1], b[1]);
+            multiply(a[0], b[0]);
+            if (k + 32 < k1) {
+              if (k + 64 < k1) load(k + 64, k + 64 + c * 8 < k1, a[0], b[0]);
+              multiply(a[1], b[1]);
+            }
           }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (n0 + i * parts < ntiles) {
-            const int n = (n0 + i * parts) * 8 + c * 2;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              *reinterpret_cast<float2*>(out + (m * 16 + g) * R + n) = make_float2(acc[m][i][0], acc[m][i][1]);
-              *reinterpret_cast<float2*>(out + (m * 16 + g + 8) * R + n) = make_float2(acc[m][i][2], acc[m][i][3]);
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (n0 + i * parts < ntiles) {
+              const int n = (n0 + i * parts) * 8 + c * 2;
+  #pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                *reinterpret_cast<float2*>(out + (m * 16 + g) * R + n) = make_float2(acc[m][i][0], acc[m][i][1]);
+                *reinterpret_cast<float2*>(out + (m * 16 + g + 8) * R + n) = make_float2(acc[m][i][2], acc[m][i][3]);
+              }
             }
           }
         }
-      }
       }
     }
     // ---- the leaves' sums, from wherever in the cluster they are
@@ -547,36 +546,36 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   bool done = false;
   if constexpr (!STAGED) {
     if (R <= 16 || R == 32) {
-    // h in one load of B per trip: the next trip's y and B are on their way while one is multiplied
-    auto run = [&](auto load_b, auto times, auto sample) {
-      uint4 yv[2][2 * MT];
-      decltype(sample) bv[2];
-      auto trip = [&](int blk, int at) {
-        if (blk + W < b1) {
-          load_y(blk + W, yv[1 - at]);
-          load_b(blk + W, bv[1 - at].v);
+      // h in one load of B per trip: the next trip's y and B are on their way while one is multiplied
+      auto run = [&](auto load_b, auto times, auto sample) {
+        uint4 yv[2][2 * MT];
+        decltype(sample) bv[2];
+        auto trip = [&](int blk, int at) {
+          if (blk + W < b1) {
+            load_y(blk + W, yv[1 - at]);
+            load_b(blk + W, bv[1 - at].v);
+          }
+  #pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            float acc[4][4];
+            clear(acc);
+            times(m, bv[at].v, acc);
+            finish(blk, m, yv[at], acc);
+          }
+        };
+        if (b0 < b1) {
+          load_y(b0, yv[0]);
+          load_b(b0, bv[0].v);
         }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          float acc[4][4];
-          clear(acc);
-          times(m, bv[at].v, acc);
-          finish(blk, m, yv[at], acc);
+  #pragma unroll 1
+        for (int blk = b0; blk < b1; blk += 2 * W) {
+          trip(blk, 0);
+          if (blk + W < b1) trip(blk + W, 1);
         }
       };
-      if (b0 < b1) {
-        load_y(b0, yv[0]);
-        load_b(b0, bv[0].v);
-      }
-#pragma unroll 1
-      for (int blk = b0; blk < b1; blk += 2 * W) {
-        trip(blk, 0);
-        if (blk + W < b1) trip(blk + W, 1);
-      }
-    };
-    if (R == 32) run([&](int blk, uint4 (&v)[4]) { load_wide(blk, 0, v); }, [&](int m, const uint4 (&v)[4], float (&acc)[4][4]) { multiply_wide(m, 0, v, acc); }, Four<uint4>{});
-    else run([&](int blk, uint2 (&v)[4]) { load_narrow(blk, 0, v); }, [&](int m, const uint2 (&v)[4], float (&acc)[4][4]) { multiply(m, 0, v, acc); }, Four<uint2>{});
-    done = true;
+      if (R == 32) run([&](int blk, uint4 (&v)[4]) { load_wide(blk, 0, v); }, [&](int m, const uint4 (&v)[4], float (&acc)[4][4]) { multiply_wide(m, 0, v, acc); }, Four<uint4>{});
+      else run([&](int blk, uint2 (&v)[4]) { load_narrow(blk, 0, v); }, [&](int m, const uint2 (&v)[4], float (&acc)[4][4]) { multiply(m, 0, v, acc); }, Four<uint2>{});
+      done = true;
     }
   } else if (R <= 16) {  // a trip or two: nothing to run ahead of
 #pragma unroll 1
@@ -664,13 +663,14 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
              const float* scales, float* h, const int32_t* order, const int32_t* offsets, int64_t T, int N, int K, int R,
              int adapters, int dtype, int leaf, cudaStream_t stream) {
   if (dtype != TBIK_DTYPE_BF16 && dtype != TBIK_DTYPE_FP16) return set_error(TBIK_ERR_DTYPE, "tbik_adapters supports bf16 and fp16");
-  if (T < 0 || T >= (int64_t(1) << 25) || N < 8 || N % 8 || N >= (1 << 28) || K < 8 || K % 8 || K >= (1 << 28))
-    return set_error(TBIK_ERR_SHAPE, "tbik_adapters: T in 0 .. 2^25 - 1, N and K positive multiples of 8 below 2^28");
+  if (T < 0 || T >= (int64_t(1) << 25) || N < 8 || N % 8 || N >= (1 << 24) || K < 8 || K % 8 || K >= (1 << 24))
+    return set_error(TBIK_ERR_SHAPE, "tbik_adapters: T in 0 .. 2^25 - 1, N and K positive multiples of 8 below 2^24");
   if (R < 8 || R % 8 || R > TBIK_MAX_RANK) return set_error(TBIK_ERR_SHAPE, "tbik_adapters: R must be a multiple of 8 up to 128");
   if (adapters < 1 || adapters > TBIK_MAX_GROUPS) return set_error(TBIK_ERR_SHAPE, "tbik_adapters: 1 .. 1024 adapters");
   if (leaf == 0) leaf = (K + 255) / 256 * 32;
   if (leaf < 0 || leaf % 32 || (static_cast<int64_t>(K) + leaf - 1) / leaf > kLeaves)
     return set_error(TBIK_ERR_SHAPE, "tbik_adapters: leaf must be a multiple of 32 with at most 8 leaves covering K");
+  leaf = std::min(leaf, (K + 31) / 32 * 32);  // one leaf of all K, however wide it was said to be
   if (T == 0) return TBIK_OK;
   const bool shrink = x != nullptr, expand = y != nullptr;
   if (!order || !offsets || (!shrink && !expand) || (shrink && !A) || (expand && (!out || !B || !scales)) || (shrink != expand && !h))

@@ -51,8 +51,8 @@ def _check(what, rows, groups: RowGroups, adapters: int, rank: int, widths, *ten
     if not 1 <= adapters <= _lib.MAX_GROUPS:
         raise ValueError(f"{what}: 1 .. {_lib.MAX_GROUPS} adapters, got {adapters}")
     for w in widths:
-        if w < 8 or w % 8:
-            raise ValueError(f"{what}: widths must be positive multiples of 8, got {widths}")
+        if not 8 <= w < 1 << 24 or w % 8:
+            raise ValueError(f"{what}: widths must be positive multiples of 8 below 2^24, got {widths}")
     order, _, offsets = groups
     if order.dtype != torch.int32 or order.shape != (rows,):
         raise ValueError(f"{what}: groups.order must be {rows} int32 values, got {tuple(order.shape)} of {order.dtype}")
@@ -74,7 +74,7 @@ def _check_leaf(what, K: int, leaf: Optional[int]) -> int:
         return 0
     if leaf < 32 or leaf % 32 or (K + leaf - 1) // leaf > 8:
         raise ValueError(f"{what}: leaf must be a multiple of 32 with at most 8 leaves covering K = {K}, got {leaf}")
-    return leaf
+    return min(leaf, (K + 31) // 32 * 32)  # (one leaf of all K, however wide it was said to be)
 
 
 def _check_out(what, y, out, *others):

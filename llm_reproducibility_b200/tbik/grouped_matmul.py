@@ -75,8 +75,8 @@ def _grouped(A, W, offsets, leaf=None, out=None, out_dtype=None, max_ctas=0):
     M, K = A.shape
     G, N, _ = W.shape
     offsets = _check_offsets(what, offsets, G)
-    if K < 1:
-        raise ValueError(f"{what}: K must be positive")
+    if not 1 <= K < 1 << 30 or N >= 1 << 30:
+        raise ValueError(f"{what}: K in 1 .. 2^30 - 1 and N below 2^30, got {K} and {N}")
     if leaf is not None and (leaf < 64 or leaf % 64 or K % leaf):
         raise ValueError(f"{what}: leaf must be a multiple of 64 that divides K = {K}, got {leaf}")
     if out_dtype not in (None, A.dtype, torch.float32):
@@ -128,8 +128,10 @@ def _weight_gradient(dC, A, offsets, out_dtype=None, max_ctas=0):
         raise ValueError(f"{what}: out_dtype is the operand type or torch.float32")
     groups = offsets.numel() - 1
     offsets = _check_offsets(what, offsets, groups)
-    dev = need_cuda(what, A, dC, offsets)
     M, N, K = A.shape[0], dC.shape[1], A.shape[1]
+    if N >= 1 << 30 or K >= 1 << 30:
+        raise ValueError(f"{what}: N and K below 2^30, got {N} and {K}")
+    dev = need_cuda(what, A, dC, offsets)
     dW = torch.empty((groups, N, K), dtype=out_dtype or A.dtype, device=dev)
     if N == 0 or K == 0:
         return dW

@@ -100,6 +100,18 @@ def test_shards_of_k_add_up_to_the_unsharded_bits(K, tp):
     assert torch.equal(parts[0], lora_shrink(x, A, groups))
 
 
+@pytest.mark.parametrize("R", [8, 128])
+@pytest.mark.parametrize("T", [1, 40, 1500])
+def test_a_leaf_wider_than_k_is_one_leaf_of_all_k(T, R):
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    K = 1000
+    y, x, A, B, ids, s = case(T, 3, R, K, 72, torch.bfloat16, "int")
+    groups, want = group_rows(ids, 3), ref(y, x, A, B, ids, s)[0].to(torch.bfloat16)
+    for leaf in (1024, 1 << 20, 1 << 28, (1 << 31) - 32, 1 << 40):
+        assert torch.equal(lora_add(y, x, A, B, groups, s, leaf=leaf), want)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("R", [8, 16, 24, 32, 40, 64, 128])
 def test_a_row_has_the_same_bits_in_every_batch(R, dtype):

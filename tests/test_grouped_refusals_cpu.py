@@ -130,6 +130,29 @@ def test_adapters_refuse():
         leaf_for_adapters(4096, 3)
 
 
+def test_widths_that_do_not_fit_the_kernels():
+    """Broadcast operands may be wider than any memory: a width must not wrap round on its way to the kernel."""
+    from llm_reproducibility_b200.tbik.adapters import lora_expand_add, lora_shrink
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent, grouped_weight_gradient
+    from llm_reproducibility_b200.tbik.row_groups import RowGroups
+    one = torch.zeros(1, dtype=BF16)
+    g = RowGroups(torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), off(0, 1))
+    for K in (1 << 24, (1 << 32) + 64):
+        with pytest.raises(ValueError, match="2\\^24"):
+            lora_shrink(one.expand(1, K), one.expand(1, 8, K), g)
+        with pytest.raises(ValueError, match="2\\^24"):
+            lora_expand_add(one.expand(1, K), torch.zeros(1, 8), one.expand(1, K, 8), g, torch.ones(1))
+    for n in (1 << 30, (1 << 32) + 64):
+        with pytest.raises(ValueError, match="2\\^30"):
+            grouped_matmul_tp_persistent(one.expand(1, n), one.expand(1, 8, n), off(0, 1))
+        with pytest.raises(ValueError, match="2\\^30"):
+            grouped_matmul_tp_persistent(one.expand(1, 64), one.expand(1, n, 64), off(0, 1))
+        with pytest.raises(ValueError, match="2\\^30"):
+            grouped_weight_gradient(one.expand(1, n), one.expand(1, 8), off(0, 1))
+        with pytest.raises(ValueError, match="2\\^30"):
+            grouped_weight_gradient(one.expand(1, 8), one.expand(1, n), off(0, 1))
+
+
 def test_c_abi_refuses_before_any_launch():
     from llm_reproducibility_b200 import _lib
     L = _lib.lib()
@@ -174,5 +197,6 @@ def test_c_abi_refuses_before_any_launch():
 
     assert lora(_12=0) == 0
     assert lora(_0=None) == -1 and lora(_2=None) == -1 and lora(_6=None) == -1 and lora(_10=None) == -1 and lora(_0=None, _2=None) == -1
+    assert lora(_13=1 << 24, _3=1 << 24, _5=1 << 24) == -2 and lora(_14=1 << 24, _1=1 << 24) == -2
     assert lora(_13=20) == -2 and lora(_14=12) == -2 and lora(_15=12) == -2 and lora(_15=136) == -2 and lora(_16=0) == -2 and lora(_18=40) == -2
     assert lora(_1=32) == -2 and lora(_3=16) == -2 and lora(_17=2) == -3 and lora(_2=p + 4) == -4 and lora(_1=65) == -4
