@@ -92,6 +92,7 @@ TBIK_DEVICE void prefetch_l2(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(src)), "r"(bytes) : "memory");
 }
 
+TBIK_DEVICE float4 add(const float4& a, const float4& b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 TBIK_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // Shared memory: [rows TM][item 4], at 512 [row factors TM] | leaf sums [8 / cluster][TM][R] | h [TM][R] |
@@ -333,41 +334,41 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
         const int k0 = static_cast<int>(kb), k1 = static_cast<int>(min(kb + p.leaf, static_cast<int64_t>(K)));
         // rows and column tiles beyond what there is repeat the last one; their results are not read
         const T* xr[2 * MT];
-  #pragma unroll
+#pragma unroll
         for (int i = 0; i < 2 * MT; ++i) xr[i] = x + static_cast<int64_t>(max(rows[min(first_row + i * 8 + g, count - 1)], 0)) * p.ldx + c * 8;
         float* out = sums + (slot * TM + first_row) * R;
         for (int n0 = part; n0 < ntiles; n0 += 4 * parts) {
           float acc[MT][4][4];
-  #pragma unroll
+#pragma unroll
           for (int m = 0; m < MT; ++m)
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; ++i)
-  #pragma unroll
+#pragma unroll
               for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
           const T* ar[4];
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 4; ++i) ar[i] = A + static_cast<int64_t>(min(n0 + i * parts, ntiles - 1) * 8 + g) * K + c * 8;
           // `in`: the lane's piece of the run of 32 columns exists
           auto load = [&](int k, bool in, uint4 (&a)[2 * MT], uint4 (&b)[4]) {
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 2 * MT; ++i) a[i] = in ? load_stream(xr[i] + k) : make_uint4(0u, 0u, 0u, 0u);
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 4; ++i) b[i] = in ? __ldg(reinterpret_cast<const uint4*>(ar[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
           };
           auto multiply = [&](const uint4 (&a)[2 * MT], const uint4 (&b)[4]) {
-  #pragma unroll
+#pragma unroll
             for (int m = 0; m < MT; ++m)
-  #pragma unroll
+#pragma unroll
               for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].x, a[2 * m + 1].x, a[2 * m].y, a[2 * m + 1].y), b[i].x, b[i].y);
-  #pragma unroll
+#pragma unroll
             for (int m = 0; m < MT; ++m)
-  #pragma unroll
+#pragma unroll
               for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].z, a[2 * m + 1].z, a[2 * m].w, a[2 * m + 1].w), b[i].z, b[i].w);
           };
           // the next run is on its way while one is multiplied
           uint4 a[2][2 * MT], b[2][4];
           load(k0, k0 + c * 8 < k1, a[0], b[0]);
-  #pragma unroll 1
+#pragma unroll 1
           for (int k = k0; k < k1; k += 64) {
             if (k + 32 < k1) load(k + 32, k + 32 + c * 8 < k1, a[1], b[1]);
             multiply(a[0], b[0]);
@@ -376,11 +377,11 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
               multiply(a[1], b[1]);
             }
           }
-  #pragma unroll
+#pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (n0 + i * parts < ntiles) {
               const int n = (n0 + i * parts) * 8 + c * 2;
-  #pragma unroll
+#pragma unroll
               for (int m = 0; m < MT; ++m) {
                 *reinterpret_cast<float2*>(out + (m * 16 + g) * R + n) = make_float2(acc[m][i][0], acc[m][i][1]);
                 *reinterpret_cast<float2*>(out + (m * 16 + g + 8) * R + n) = make_float2(acc[m][i][2], acc[m][i][3]);
@@ -390,22 +391,37 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
         }
       }
     }
-    // ---- the leaves' sums, from wherever in the cluster they are
+    // ---- the leaves' sums: this CTA's own first, a subtree of theirs, then one node from each CTA of the cluster
     cg::cluster_group cluster = cg::this_cluster();
-    if (C > 1) cluster.sync(); else __syncthreads();
-    for (int i = tid; i < TM * R / 4; i += kThreads) {
-      float4 s[kLeaves];
+    if (own > 1) {
+      __syncthreads();
+      for (int i = tid; i < TM * R / 4; i += kThreads) {
+        float4 s[kLeaves];
 #pragma unroll
-      for (int l = 0; l < kLeaves; ++l) {
-        const float* from = C > 1 ? cluster.map_shared_rank(sums, l / own) : sums;
-        s[l] = reinterpret_cast<const float4*>(from + (l % own) * TM * R)[i];
+        for (int l = 0; l < kLeaves; ++l)
+          if (l < own) s[l] = reinterpret_cast<const float4*>(sums + l * TM * R)[i];
+#pragma unroll
+        for (int d = 1; d < kLeaves; d *= 2)
+#pragma unroll
+          for (int l = 0; l < kLeaves; l += 2 * d)
+            if (l + d < own) s[l] = add(s[l], s[l + d]);
+        reinterpret_cast<float4*>(C > 1 ? sums : hs)[i] = s[0];
       }
+    }
+    if (C > 1) {
+      cluster.sync();
+      for (int i = tid; i < TM * R / 4; i += kThreads) {
+        float4 s[kLeaves];
 #pragma unroll
-      for (int d = 1; d < kLeaves; d *= 2)
+        for (int c = 0; c < kLeaves; ++c)
+          if (c < C) s[c] = reinterpret_cast<const float4*>(cluster.map_shared_rank(sums, c))[i];
 #pragma unroll
-        for (int l = 0; l < kLeaves; l += 2 * d)
-          s[l] = make_float4(s[l].x + s[l + d].x, s[l].y + s[l + d].y, s[l].z + s[l + d].z, s[l].w + s[l + d].w);
-      reinterpret_cast<float4*>(hs)[i] = s[0];
+        for (int d = 1; d < kLeaves; d *= 2)
+#pragma unroll
+          for (int c = 0; c < kLeaves; c += 2 * d)
+            if (c + d < C) s[c] = add(s[c], s[c + d]);
+        reinterpret_cast<float4*>(hs)[i] = s[0];
+      }
     }
     if (C > 1) cluster.sync(); else __syncthreads();  // nobody leaves while its sums may still be read
     if (!expand) {
@@ -555,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
             load_y(blk + W, yv[1 - at]);
             load_b(blk + W, bv[1 - at].v);
           }
-  #pragma unroll
+#pragma unroll
           for (int m = 0; m < MT; ++m) {
             float acc[4][4];
             clear(acc);
@@ -567,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
           load_y(b0, yv[0]);
           load_b(b0, bv[0].v);
         }
-  #pragma unroll 1
+#pragma unroll 1
         for (int blk = b0; blk < b1; blk += 2 * W) {
           trip(blk, 0);
           if (blk + W < b1) trip(blk + W, 1);
