@@ -53,11 +53,11 @@ def empty(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> tor
 
 def need_cuda(what: str, *tensors: torch.Tensor) -> torch.device:
     """The tensors' one CUDA device."""
-    device = tensors[0].device
+    device, index = tensors[0].device, tensors[0].get_device()  # (numbers compare quicker than devices; -1 off the GPU)
     for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError(f"{what} needs CUDA tensors (there is no CPU fallback)")
-        if t.device != device:
+        if t.get_device() != index or index < 0:
+            if not t.is_cuda or index < 0:
+                raise RuntimeError(f"{what} needs CUDA tensors (there is no CPU fallback)")
             raise RuntimeError(f"{what}: tensors on {device} and {t.device}")
     return device
 
