@@ -24,8 +24,11 @@
 //
 // The operands' contiguous index is the reduction index (K-major) or the other one (MN-major); the instruction takes
 // either, so the transposed weight and both operands of the weight gradient are read as they lie.  The weight gradient
-// reduces over a group's rows: its last step ends inside a box, and the rows of the next group that the box brought along
-// are overwritten with zeros in shared memory before the multiply, in both operands (a NaN there must not meet a zero).
+// reduces over a group's rows: its last step of 16 ends inside the group's last box, and the rows of the next group that the
+// box brought along must become zero before the multiply, in both operands (a NaN there must not meet a zero).  That step
+// has boxes of its own, loaded when the tile begins and cleared by warp 3, so that nobody waits for it when its turn comes
+// (16384 rows of 32 groups, K = N = 2048: cleared in the stage itself by the issuing warps 147 us, so 129 us; groups of whole
+// steps 126 us).
 //
 // PAIR: a cluster of two CTAs per tile (cta_group::2), each with its own 128 rows and half of the columns' operand.
 #include <cuda.h>
@@ -57,22 +60,22 @@ constexpr int GROUP_M = 8;  // row tiles that share a sweep over the columns
 __device__ uint32_t g_grouped_status[4];  // [0] a bounded wait ran out, [1] block, [2] role
 
 struct Maps {
-  CUtensorMap a[4];  // forward: A with boxes of 16, 32, 64, 128 rows; weight gradient: a[0] = dC, a[1] = dW
+  CUtensorMap a[4];  // forward: A with boxes of 16, 32, 64, 128 rows; weight gradient: dC, dW, dC and A with boxes of 16 rows
   CUtensorMap b;     // W; weight gradient: A
 };
 
 // What every role has to know of the groups, in shared memory: rows first[g] .. last[g] - 1, tiles of `per[g]` rows
-// (forward), before[g] tiles in the groups before g (G + 1 entries).
+// (forward), before[g] tiles in the groups before g (G + 1 entries; forward).
 struct Table {
   int *first, *last, *before, *per;
   int* warps;  // 3 x 16 words of scratch
-  static constexpr uint32_t bytes(int groups) { return 4u * (4 * groups + 1 + 48); }
-  TBIK_DEVICE Table(uint8_t* at, int groups) {
+  static constexpr uint32_t bytes(int groups, bool tiles) { return 4u * ((tiles ? 4 * groups + 1 : 2 * groups) + 48); }
+  TBIK_DEVICE Table(uint8_t* at, int groups, bool tiles) {
     first = reinterpret_cast<int*>(at);
     last = first + groups;
-    per = last + groups;
-    before = per + groups;
-    warps = before + groups + 1;
+    per = tiles ? last + groups : nullptr;
+    before = tiles ? per + groups : nullptr;
+    warps = tiles ? before + groups + 1 : last + groups;
   }
 };
 
@@ -128,6 +131,7 @@ TBIK_DEVICE void build_table(const int32_t* offsets, int groups, int M, const Ta
     if (g < groups) {
       t.first[g] = lo;
       t.last[g] = hi;
+      if (t.before == nullptr) continue;
       t.per[g] = per;
       t.before[g] = at + sum - tiles;
       if (g == groups - 1) t.before[groups] = at + sum;
@@ -192,7 +196,7 @@ struct ForwardCfg {
   static constexpr uint32_t OFF_ABORT = OFF_TMEM_PTR + 4;
   static constexpr uint32_t OFF_DEALT = (OFF_ABORT + 4 + 15) / 16 * 16;
   static constexpr uint32_t OFF_TABLE = OFF_DEALT + DEALT * 16;
-  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + Table::bytes(groups) + 1024; }
+  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + Table::bytes(groups, true) + 1024; }
   static_assert(smem_bytes(TBIK_MAX_GROUPS) <= 232448, "shared memory budget");
   // tokens per tile of a group of m rows: as few tiles as TN allows, evenly filled
   static TBIK_DEVICE int tokens(int m) {
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) forward_kernel(const __grid_co
   auto empty_bar = [&](int s) { return smem_base + C_::OFF_EMPTY + 8u * s; };
   auto tfull_bar = [&](int a) { return smem_base + C_::OFF_TFULL + 8u * a; };
   auto tempty_bar = [&](int a) { return smem_base + C_::OFF_TEMPTY + 8u * a; };
-  const Table table(smem_gen + C_::OFF_TABLE, p.groups);
+  const Table table(smem_gen + C_::OFF_TABLE, p.groups, true);
 
   if constexpr (PAIR) cluster_sync_all();
   if (threadIdx.x == 0) {
@@ -662,16 +666,19 @@ struct WgradCfg {
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_COLS * BK * 2;
   static constexpr int CW = BN / 2;  // columns per epilogue warp
   static constexpr int NCH = CW / CHUNK;
-  static constexpr uint32_t OFF_STAGING = STAGES * STAGE_BYTES;
+  static constexpr uint32_t TAIL_BYTES = STAGE_BYTES / BK * UMMA_K;  // a group's last step, of two tiles
+  static constexpr uint32_t OFF_TAIL = STAGES * STAGE_BYTES;
+  static constexpr uint32_t OFF_STAGING = OFF_TAIL + 2 * TAIL_BYTES;
   static constexpr uint32_t OFF_FULL = OFF_STAGING + NUM_EPI_WARPS * STAGING_BYTES_PER_WARP;
   static constexpr uint32_t OFF_EMPTY = OFF_FULL + 8 * STAGES;
   static constexpr uint32_t OFF_TFULL = OFF_EMPTY + 8 * STAGES;
   static constexpr uint32_t OFF_TEMPTY = OFF_TFULL + 16;
-  static constexpr uint32_t OFF_TMEM_PTR = OFF_TEMPTY + 16;
+  static constexpr uint32_t OFF_TAIL_BARS = OFF_TEMPTY + 16;  // landed, free, cleared: two each
+  static constexpr uint32_t OFF_TMEM_PTR = OFF_TAIL_BARS + 48;
   static constexpr uint32_t OFF_ABORT = OFF_TMEM_PTR + 4;
   static constexpr uint32_t OFF_DEALT = (OFF_ABORT + 4 + 15) / 16 * 16;
   static constexpr uint32_t OFF_TABLE = OFF_DEALT + DEALT * 32;
-  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + Table::bytes(groups) + 1024; }
+  static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + Table::bytes(groups, false) + 1024; }
   static_assert(smem_bytes(TBIK_MAX_GROUPS) <= 232448, "shared memory budget");
 };
 
@@ -696,7 +703,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
   auto empty_bar = [&](int s) { return smem_base + C_::OFF_EMPTY + 8u * s; };
   auto tfull_bar = [&](int a) { return smem_base + C_::OFF_TFULL + 8u * a; };
   auto tempty_bar = [&](int a) { return smem_base + C_::OFF_TEMPTY + 8u * a; };
-  const Table table(smem_gen + C_::OFF_TABLE, p.groups);
+  auto tail_landed_bar = [&](int b) { return smem_base + C_::OFF_TAIL_BARS + 8u * b; };
+  auto tail_free_bar = [&](int b) { return smem_base + C_::OFF_TAIL_BARS + 16 + 8u * b; };
+  auto tail_cleared_bar = [&](int b) { return smem_base + C_::OFF_TAIL_BARS + 32 + 8u * b; };
+  const Table table(smem_gen + C_::OFF_TABLE, p.groups, false);
 
   if constexpr (PAIR) cluster_sync_all();
   if (threadIdx.x == 0) {
@@ -708,6 +718,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
       mbar_init(tempty_bar(a), PAIR ? 2 * NUM_EPI_WARPS : NUM_EPI_WARPS);
+      mbar_init(tail_landed_bar(a), 1);
+      mbar_init(tail_free_bar(a), 1);
+      mbar_init(tail_cleared_bar(a), PAIR ? 2 : 1);  // pair: each CTA's warp 3, the leader's barrier alone
     }
     fence_mbar_init();
   }
@@ -755,12 +768,29 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
     // ------------------------------------------------------------ TMA producer
     if (elect_one()) {
       int stage = 0;
-      uint32_t phase = 0;
+      uint32_t phase = 0, tails = 0;
       bool ok = true;
       const uint64_t policy = l2_policy(0);
       for (int i = 0; ok && i < my_tiles; ++i) {
         const Tile t = tile_at(i);
-        for (int b = 0; b < t.count; b += BK) {
+        const int whole = t.count / UMMA_K * UMMA_K;  // rows in whole steps
+        const int row = t.row + cta_rank * BM, col = t.col + cta_rank * C_::B_COLS;
+        if (whole < t.count) {
+          const uint32_t buf = tails & 1u, bar = tail_landed_bar(buf);
+          if (!mbar_wait_bounded(tail_free_bar(buf), ((tails >> 1) & 1u) ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
+            ok = false;
+            role_failed = 6;
+            break;
+          }
+          ++tails;
+          const uint32_t sa = smem_base + C_::OFF_TAIL + buf * C_::TAIL_BYTES, sb = sa + C_::A_BYTES / BK * UMMA_K;
+          mbar_arrive_expect_tx(bar, C_::TAIL_BYTES);
+#pragma unroll
+          for (int u = 0; u < BM / 64; ++u) tma_load_2d_hint(sa + u * 2048, &maps.a[2], row + u * 64, t.r0 + whole, bar, policy);
+#pragma unroll
+          for (int u = 0; u < C_::B_COLS / 64; ++u) tma_load_2d_hint(sb + u * 2048, &maps.a[3], col + u * 64, t.r0 + whole, bar, policy);
+        }
+        for (int b = 0; b < whole; b += BK) {
           if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
             ok = false;
             role_failed = 1;
@@ -770,10 +800,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
           mbar_arrive_expect_tx(bar, STAGE_BYTES);
 #pragma unroll
           for (int u = 0; u < BM / 64; ++u)
-            tma_load_2d_hint(sa + u * 8192, &maps.a[0], t.row + cta_rank * BM + u * 64, t.r0 + b, bar, policy);
+            tma_load_2d_hint(sa + u * 8192, &maps.a[0], row + u * 64, t.r0 + b, bar, policy);
 #pragma unroll
           for (int u = 0; u < C_::B_COLS / 64; ++u)
-            tma_load_2d_hint(sb + u * 8192, &maps.b, t.col + cta_rank * C_::B_COLS + u * 64, t.r0 + b, bar, policy);
+            tma_load_2d_hint(sb + u * 8192, &maps.b, col + u * 64, t.r0 + b, bar, policy);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -787,96 +817,117 @@ __global__ void __launch_bounds__(NUM_THREADS, 1) wgrad_kernel(const __grid_cons
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ UMMA issuer (pair: the partner relays "stage landed")
-    // The whole warp walks along: it may have to clear rows.
-    const uint32_t idesc = umma_idesc_f16(static_cast<uint32_t>(p.half), TILE_M, BN) | kUmmaTransposeA | kUmmaTransposeB;
-    const uint64_t desc_a0 = umma_desc_sw128_mnmajor(smem_base, 8192u);
-    const uint64_t desc_b0 = umma_desc_sw128_mnmajor(smem_base + C_::A_BYTES, 8192u);
-    constexpr uint64_t STEP = 2048 >> 4;
-    int stage = 0;
-    uint32_t phase = 0, chain = 0;
-    bool ok = true;
-    // The lanes have to agree on the outcome: the warp-wide instructions that follow need all of them.
-    auto wait = [&](uint32_t bar, uint32_t parity, int role) {
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, parity, abort_flag, WAIT_LIMIT_NS)) != 0;
-      if (!ok) role_failed = role;
-      return ok;
-    };
-    auto commit = [&](uint32_t bar) {
-      if constexpr (PAIR) {
-        umma_commit_pair(bar);
-        umma_commit_pair(map_to_cta(bar, 1));
-      } else {
-        umma_commit(bar);
-      }
-    };
-    auto advance = [&]() {
-      if (++stage == STAGES) {
-        stage = 0;
-        phase ^= 1u;
-      }
-    };
-    // Rows left .. up to the next multiple of 16 of the staged boxes become zero.
-    auto zero_tail = [&](int left) {
-      const int upto = (left + UMMA_K - 1) / UMMA_K * UMMA_K;
-      uint8_t* st = smem_gen + stage * STAGE_BYTES;
-      constexpr int BOXES = static_cast<int>(STAGE_BYTES / 8192);
-      for (int i = lane; i < (upto - left) * 8 * BOXES; i += 32) {
-        const int piece = i & 7, box = (i >> 3) % BOXES, row = left + (i >> 3) / BOXES;
-        *reinterpret_cast<uint4*>(st + box * 8192 + row * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-    };
     if (PAIR && !leader) {
-      for (int i = 0; ok && i < my_tiles; ++i) {
-        const Tile t = tile_at(i);
-        for (int b = 0; b < t.count; b += BK) {
-          if (!wait(full_bar(stage), phase, 5)) break;
-          const int left = t.count - b;
-          const bool ragged = left < BK && left % UMMA_K != 0;
-          if (ragged) zero_tail(left);
-          if (elect_one()) {
-            const uint32_t to = map_to_cta(full_bar(stage), 0);
-            if (ragged) mbar_arrive_cluster_release(to); else mbar_arrive_cluster(to);
+      // ------------------------------------------------------------ partner: relay "stage landed" to the leader
+      if (elect_one()) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int i = 0; ok && i < my_tiles; ++i) {
+          const int whole = tile_at(i).count / UMMA_K * UMMA_K;
+          for (int b = 0; b < whole; b += BK) {
+            if (!mbar_wait_bounded(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
+              ok = false;
+              role_failed = 5;
+              break;
+            }
+            mbar_arrive_cluster(map_to_cta(full_bar(stage), 0));
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
-          __syncwarp();
-          advance();
         }
       }
-    } else {
+    } else if (elect_one()) {
+      // ------------------------------------------------------------ UMMA issuer
+      const uint32_t idesc = umma_idesc_f16(static_cast<uint32_t>(p.half), TILE_M, BN) | kUmmaTransposeA | kUmmaTransposeB;
+      const uint64_t desc_a0 = umma_desc_sw128_mnmajor(smem_base, 8192u);
+      const uint64_t desc_b0 = umma_desc_sw128_mnmajor(smem_base + C_::A_BYTES, 8192u);
+      const uint64_t tail_a0 = umma_desc_sw128_mnmajor(smem_base + C_::OFF_TAIL, 2048u);
+      const uint64_t tail_b0 = umma_desc_sw128_mnmajor(smem_base + C_::OFF_TAIL + C_::A_BYTES / BK * UMMA_K, 2048u);
+      constexpr uint64_t STEP = 2048 >> 4;
+      int stage = 0;
+      uint32_t phase = 0, chain = 0, tails = 0;
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity, int role) {
+        ok = mbar_wait_bounded(bar, parity, abort_flag, WAIT_LIMIT_NS);
+        if (!ok) role_failed = role;
+        return ok;
+      };
+      auto commit = [&](uint32_t bar) {
+        if constexpr (PAIR) {
+          umma_commit_pair(bar);
+          umma_commit_pair(map_to_cta(bar, 1));
+        } else {
+          umma_commit(bar);
+        }
+      };
+      auto multiply = [&](uint32_t d, uint64_t a, uint64_t b, bool first) {
+        if constexpr (PAIR) umma_f16_ss_pair(d, a, b, idesc, first ? 0u : 1u); else umma_f16_ss(d, a, b, idesc, first ? 0u : 1u);
+      };
       for (int i = 0; ok && i < my_tiles; ++i) {
-        const Tile t = tile_at(i);
-        if (t.count == 0) continue;  // an empty group: the epilogue writes zeros
+        const int count = tile_at(i).count, whole = count / UMMA_K * UMMA_K;
+        if (count == 0) continue;  // an empty group: the epilogue writes zeros
         const uint32_t a = chain & 1u;
         if (!wait(tempty_bar(a), ((chain >> 1) & 1u) ^ 1u, 2)) break;
         ++chain;
         tc_fence_after_sync();
         const uint32_t tmem_d = tmem_base + a * BN;
-        for (int b = 0; b < t.count; b += BK) {
+        for (int b = 0; b < whole; b += BK) {
           if (!wait(full_bar(stage), phase, 3)) break;
           tc_fence_after_sync();
-          const int left = t.count - b;
-          if (left < BK && left % UMMA_K != 0) {
-            if constexpr (PAIR) fence_acq_rel_cluster();  // the partner's zeros
-            zero_tail(left);
-          }
-          if (elect_one()) {
-            const uint64_t sd = static_cast<uint64_t>(stage) * (STAGE_BYTES >> 4);
-            const int steps = left >= BK ? BK / UMMA_K : (left + UMMA_K - 1) / UMMA_K;
+          const uint64_t sd = static_cast<uint64_t>(stage) * (STAGE_BYTES >> 4);
 #pragma unroll
-            for (int k = 0; k < BK / UMMA_K; ++k) {
-              if (k >= steps) break;
-              const uint32_t acc = (b | k) != 0 ? 1u : 0u;
-              if constexpr (PAIR) umma_f16_ss_pair(tmem_d, desc_a0 + sd + k * STEP, desc_b0 + sd + k * STEP, idesc, acc);
-              else umma_f16_ss(tmem_d, desc_a0 + sd + k * STEP, desc_b0 + sd + k * STEP, idesc, acc);
-            }
-            commit(empty_bar(stage));
-            if (left <= BK) commit(tfull_bar(a));
+          for (int k = 0; k < BK / UMMA_K; ++k)
+            if (b + k * UMMA_K < whole) multiply(tmem_d, desc_a0 + sd + k * STEP, desc_b0 + sd + k * STEP, (b | k) == 0);
+          commit(empty_bar(stage));
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
           }
-          __syncwarp();
-          advance();
         }
+        if (ok && whole < count) {
+          const uint32_t buf = tails & 1u;
+          const uint32_t parity = (tails >> 1) & 1u;
+          if (!wait(tail_cleared_bar(buf), parity, 7)) break;
+          if (PAIR && !mbar_acquire_cluster(tail_cleared_bar(buf), parity)) {  // the partner's zeros
+            ok = false;
+            role_failed = 7;
+            break;
+          }
+          ++tails;
+          tc_fence_after_sync();
+          const uint64_t sd = static_cast<uint64_t>(buf) * (C_::TAIL_BYTES >> 4);
+          multiply(tmem_d, tail_a0 + sd, tail_b0 + sd, whole == 0);
+          commit(tail_free_bar(buf));
+        }
+        if (ok) commit(tfull_bar(a));
+      }
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------ clears what follows the group in its last step
+    constexpr int BOXES = static_cast<int>(C_::TAIL_BYTES / 2048);
+    uint32_t tails = 0;
+    for (int i = 0; i < my_tiles; ++i) {
+      const int left = tile_at(i).count % UMMA_K;
+      if (left == 0) continue;
+      const uint32_t buf = tails & 1u;
+      // the lanes have to agree on the outcome
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(tail_landed_bar(buf), (tails >> 1) & 1u, abort_flag, WAIT_LIMIT_NS))) {
+        role_failed = 8;
+        break;
+      }
+      ++tails;
+      uint8_t* at = smem_gen + C_::OFF_TAIL + buf * C_::TAIL_BYTES;
+      for (int j = lane; j < (UMMA_K - left) * 8 * BOXES; j += 32) {
+        const int piece = j & 7, box = (j >> 3) % BOXES, row = left + (j >> 3) / BOXES;
+        *reinterpret_cast<uint4*>(at + box * 2048 + row * 128 + piece * 16) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_cluster_release(map_to_cta(tail_cleared_bar(buf), 0)); else mbar_arrive(tail_cleared_bar(buf));
       }
     }
   } else if (warp >= EPI_WARP0) {
@@ -1299,7 +1350,11 @@ int grouped_gemm_wgrad(const void* dC, const void* A, void* dW, const int32_t* o
   const int64_t dd[2] = {N, M}, sd[1] = {lddc}, da[2] = {K, M}, sa[1] = {lda};
   rc = make_map(&maps.a[0], dtype, dC, 2, dd, sd, BK);
   if (rc != TBIK_OK) return rc;
-  for (int i = 1; i < 4; ++i) maps.a[i] = maps.a[0];
+  maps.a[1] = maps.a[0];
+  rc = make_map(&maps.a[2], dtype, dC, 2, dd, sd, UMMA_K);
+  if (rc != TBIK_OK) return rc;
+  rc = make_map(&maps.a[3], dtype, A, 2, da, sa, UMMA_K);
+  if (rc != TBIK_OK) return rc;
   const int es = out_dtype == TBIK_DTYPE_FP32 ? 4 : 2;
   const bool tma_store = !bad_align(dW) && static_cast<int64_t>(K) * es % 16 == 0;
   if (tma_store) {
