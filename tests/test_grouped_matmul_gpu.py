@@ -190,6 +190,39 @@ def test_weight_gradient_depends_on_the_groups_own_rows_and_not_on_the_grid():
         assert torch.equal(grouped_weight_gradient(D, A, off, max_ctas=ctas), full)
 
 
+@pytest.mark.parametrize("N,K,sizes,ctas", [(38400, 64, [103, 97], 1), (8192, 64, [3, 0, 17, 5, 1, 16, 2, 9], 1), (520, 64, [30] * 600, 3)])
+def test_more_tiles_than_are_worked_out_ahead(N, K, sizes, ctas):
+    """Hundreds of tiles for one CTA, or one pair: the ones beyond the first 256 are found as they come."""
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent, grouped_weight_gradient
+    off = offsets_of(sizes).cuda()
+    A, W = make((sum(sizes), K), torch.bfloat16, "int", 1), make((len(sizes), N, K), torch.bfloat16, "int", 2)
+    got = grouped_matmul_tp_persistent(A, W, off, max_ctas=ctas)
+    assert torch.equal(got, forward_ref(A, W, off)[0].to(torch.bfloat16))
+    for n, k in ((2048, 2048), (100, 2304)):  # tiles of a pair, of one CTA
+        D, A = make((sum(sizes[:8]), n), torch.bfloat16, "int", 3), make((sum(sizes[:8]), k), torch.bfloat16, "int", 4)
+        some = torch.cat([off[:9], off[8:9].expand(24)]) if len(sizes) > 8 else off
+        some = some.clamp(max=D.shape[0]).contiguous()
+        want = wgrad_ref(D, A, some)[0].to(torch.bfloat16)
+        assert torch.equal(grouped_weight_gradient(D, A, some, max_ctas=ctas), want)
+
+
+@pytest.mark.parametrize("N,K", [(264, 136), (100, 520)])
+def test_weight_gradient_of_a_group_beside_infinities_and_nan(N, K):
+    """The rows behind a group's last step of 16 come along with it and belong to someone else."""
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_weight_gradient
+    sizes = [1, 1, 15, 3, 16, 2, 17, 1, 63, 9, 64, 5, 65, 4, 130, 7]
+    off = offsets_of(sizes).cuda()
+    D, A = make((sum(sizes), N), torch.bfloat16, "int", 1), make((sum(sizes), K), torch.bfloat16, "int", 2)
+    want = wgrad_ref(D, A, off)[0].to(torch.bfloat16)
+    at = off.tolist()
+    for g in range(1, len(sizes), 2):
+        D[at[g]:at[g + 1]] = float("nan")
+        A[at[g]:at[g + 1]] = float("inf")
+    for ctas in (0, 2):
+        got = grouped_weight_gradient(D, A, off, max_ctas=ctas)
+        assert torch.equal(got[::2], want[::2]) and got[1::2].isnan().all()
+
+
 def test_strided_and_unaligned_operands():
     from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent, grouped_weight_gradient
     M, G, K, N = 200, 3, 64, 48
