@@ -11,9 +11,9 @@
 //
 // One cluster of 1 .. 8 CTAs per (adapter, tile of rows), both products in one launch.  The CTAs split K by leaves, add
 // the leaves through distributed shared memory, and split N for the second product.  Few rows: 16-row tiles and
-// asynchronous copies of a leaf into shared memory, so that a decode step pays one memory latency; many rows: 64-row tiles in
-// two groups of warps, whose warps take a leaf or a part of its columns each, operands straight into registers.  Either way
-// a leaf is one chain of instructions over its columns, so a row's bits depend on the row and its adapter alone.
+// asynchronous copies of a leaf into shared memory, so that a decode step pays one memory latency; many rows: 32-row tiles,
+// whose warps take a leaf or a part of its columns of h each, operands straight into registers.  Either way a leaf is one
+// chain of instructions over its columns, so a row's bits depend on the row and its adapter alone.
 //
 // h is held in fp32; the second product reads it as the sum of two values of the operand type (16 bits of mantissa for
 // bf16, 22 for fp16, whose rows are scaled by a power of two into its range first).
@@ -100,24 +100,23 @@ TBIK_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
 struct Layout {
   uint32_t sums, h, frags, stage, total;
 };
-template <int MT, int RG, bool STAGED>
+template <int MT, bool STAGED>
 __host__ __device__ inline Layout layout(int R, int cluster) {
-  constexpr int TM = RG * MT * 16;
+  constexpr int TM = MT * 16;
   Layout l;
   l.sums = 1024;
   l.h = l.sums + (kLeaves / cluster) * TM * R * 4;
   l.frags = l.h + TM * R * 4;
-  l.stage = (l.frags + RG * MT * ((R + 15) / 16) * 1024 + 127) / 128 * 128;
+  l.stage = (l.frags + MT * ((R + 15) / 16) * 1024 + 127) / 128 * 128;
   l.total = l.stage + (STAGED ? 2 * stage_bytes(R) : 0);
   return l;
 }
 
-// RG groups of warps, each with MT x 16 rows of the tile.
-template <typename T, int MT, int RG, bool STAGED>
+template <typename T, int MT, bool STAGED>
 __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(const Params p) {
-  constexpr int TM = RG * MT * 16, W = kWarps / RG;  // rows of the tile, warps of a group
+  constexpr int TM = MT * 16;  // rows of the tile
   extern __shared__ __align__(128) uint8_t smem[];
-  const Layout lay = layout<MT, RG, STAGED>(p.R, p.cluster);
+  const Layout lay = layout<MT, STAGED>(p.R, p.cluster);
   int* rows = reinterpret_cast<int*>(smem);                 // row index or -1
   int* item = rows + TM;                                    // adapter, first place, rows
   float* factor = reinterpret_cast<float*>(smem + 512);     // what a row of h was multiplied by (fp16)
@@ -222,7 +221,6 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   }
 
   const int g = lane >> 2, c = lane & 3;  // the lane's row (and row + 8) and its place in a row
-  const int first_row = warp / W * (MT * 16), w = warp % W;  // of the warp's group of rows; its number there
   const int nblocks = ceil_div(p.N, 32);
   const T* B = static_cast<const T*>(p.B) + static_cast<int64_t>(adapter) * p.N * R;
 
@@ -325,67 +323,74 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
         }
       }
     } else {
-      // A group's W warps take a leaf each, in turns, or share the column tiles of a leaf where the CTA has fewer leaves.  Two
-      // groups read the same rows of A at about the same time: the second finds them in L1.
-      const int parts = own < W ? W / own : 1, part = w % parts;
-      for (int slot = w / parts; slot < own; slot += W / parts) {
-        const int leaf = rank * own + slot;
-        const int64_t kb = min(static_cast<int64_t>(leaf) * p.leaf, static_cast<int64_t>(K));
-        const int k0 = static_cast<int>(kb), k1 = static_cast<int>(min(kb + p.leaf, static_cast<int64_t>(K)));
-        // rows and column tiles beyond what there is repeat the last one; their results are not read
-        const T* xr[2 * MT];
+      // Eight leaves and eight warps: a warp takes one, or with C CTAs every C-th column tile of one.
+      static_assert(kWarps == kLeaves, "a warp per leaf");
+      const int slot = warp / C, parts = C, part = warp % C;
+      const int leaf = rank * own + slot;
+      const int64_t kb = min(static_cast<int64_t>(leaf) * p.leaf, static_cast<int64_t>(K));
+      const int k0 = static_cast<int>(kb), k1 = static_cast<int>(min(kb + p.leaf, static_cast<int64_t>(K)));
+      // rows and column tiles beyond what there is repeat the last one; their results are not read
+      const T* xr[2 * MT];
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) xr[i] = x + static_cast<int64_t>(max(rows[min(first_row + i * 8 + g, count - 1)], 0)) * p.ldx + c * 8;
-        float* out = sums + (slot * TM + first_row) * R;
-        for (int n0 = part; n0 < ntiles; n0 += 4 * parts) {
-          float acc[MT][4][4];
+      for (int i = 0; i < 2 * MT; ++i) xr[i] = x + static_cast<int64_t>(max(rows[min(i * 8 + g, count - 1)], 0)) * p.ldx + c * 8;
+      float* out = sums + slot * TM * R;
+      for (int n0 = part; n0 < ntiles; n0 += 4 * parts) {
+        float acc[MT][4][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
+        const T* ar[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ar[i] = A + static_cast<int64_t>(min(n0 + i * parts, ntiles - 1) * 8 + g) * K + c * 8;
+        // `in`: the lane's piece of the run of 32 columns exists
+        auto load = [&](int k, bool in, uint4 (&a)[2 * MT], uint4 (&b)[4]) {
+#pragma unroll
+          for (int i = 0; i < 2 * MT; ++i) a[i] = in ? load_stream(xr[i] + k) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) b[i] = in ? __ldg(reinterpret_cast<const uint4*>(ar[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        auto multiply = [&](const uint4 (&a)[2 * MT], const uint4 (&b)[4]) {
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].x, a[2 * m + 1].x, a[2 * m].y, a[2 * m + 1].y), b[i].x, b[i].y);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) acc[m][i][j] = 0.0f;
-          const T* ar[4];
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ar[i] = A + static_cast<int64_t>(min(n0 + i * parts, ntiles - 1) * 8 + g) * K + c * 8;
-          // `in`: the lane's piece of the run of 32 columns exists
-          auto load = [&](int k, bool in, uint4 (&a)[2 * MT], uint4 (&b)[4]) {
-#pragma unroll
-            for (int i = 0; i < 2 * MT; ++i) a[i] = in ? load_stream(xr[i] + k) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] = in ? __ldg(reinterpret_cast<const uint4*>(ar[i] + k)) : make_uint4(0u, 0u, 0u, 0u);
-          };
-          auto multiply = [&](const uint4 (&a)[2 * MT], const uint4 (&b)[4]) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].x, a[2 * m + 1].x, a[2 * m].y, a[2 * m + 1].y), b[i].x, b[i].y);
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].z, a[2 * m + 1].z, a[2 * m].w, a[2 * m + 1].w), b[i].z, b[i].w);
-          };
-          // the next run is on its way while one is multiplied
-          uint4 a[2][2 * MT], b[2][4];
-          load(k0, k0 + c * 8 < k1, a[0], b[0]);
+            for (int i = 0; i < 4; ++i) Half<T>::mma(acc[m][i], make_uint4(a[2 * m].z, a[2 * m + 1].z, a[2 * m].w, a[2 * m + 1].w), b[i].z, b[i].w);
+        };
+        // The next run is on its way while one is multiplied; whole runs go without a thought for the end of the leaf (1500 rows,
+        // rank 32, K = 12288: 41 us, without this loop 45; 8192 rows, K = 4096: 53 and 52).
+        uint4 a[2][2 * MT], b[2][4];
+        load(k0, k0 + c * 8 < k1, a[0], b[0]);
+        int k = k0;
 #pragma unroll 1
-          for (int k = k0; k < k1; k += 64) {
-            if (k + 32 < k1) load(k + 32, k + 32 + c * 8 < k1, a[1], b[1]);
-            multiply(a[0], b[0]);
-            if (k + 32 < k1) {
-              if (k + 64 < k1) load(k + 64, k + 64 + c * 8 < k1, a[0], b[0]);
-              multiply(a[1], b[1]);
-            }
+        for (; k + 96 <= k1; k += 64) {
+          load(k + 32, true, a[1], b[1]);
+          multiply(a[0], b[0]);
+          load(k + 64, true, a[0], b[0]);
+          multiply(a[1], b[1]);
+        }
+#pragma unroll 1
+        for (; k < k1; k += 64) {
+          if (k + 32 < k1) load(k + 32, k + 32 + c * 8 < k1, a[1], b[1]);
+          multiply(a[0], b[0]);
+          if (k + 32 < k1) {
+            if (k + 64 < k1) load(k + 64, k + 64 + c * 8 < k1, a[0], b[0]);
+            multiply(a[1], b[1]);
           }
+        }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (n0 + i * parts < ntiles) {
-              const int n = (n0 + i * parts) * 8 + c * 2;
+        for (int i = 0; i < 4; ++i) {
+          if (n0 + i * parts < ntiles) {
+            const int n = (n0 + i * parts) * 8 + c * 2;
 #pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                *reinterpret_cast<float2*>(out + (m * 16 + g) * R + n) = make_float2(acc[m][i][0], acc[m][i][1]);
-                *reinterpret_cast<float2*>(out + (m * 16 + g + 8) * R + n) = make_float2(acc[m][i][2], acc[m][i][3]);
-              }
+            for (int m = 0; m < MT; ++m) {
+              *reinterpret_cast<float2*>(out + (m * 16 + g) * R + n) = make_float2(acc[m][i][0], acc[m][i][1]);
+              *reinterpret_cast<float2*>(out + (m * 16 + g + 8) * R + n) = make_float2(acc[m][i][2], acc[m][i][3]);
             }
           }
         }
@@ -462,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   auto column = [&](int s, int at) { return wide ? 32 * (s >> 1) + 8 * at + 4 * (s & 1) : 16 * s + 4 * at; };
   uint4* frags = reinterpret_cast<uint4*>(smem + lay.frags);
   const int ksteps = (R + 15) / 16;
-  for (int i = tid; i < RG * MT * ksteps * 32; i += kThreads) {
+  for (int i = tid; i < MT * ksteps * 32; i += kThreads) {
     const int ln = i & 31, s = (i >> 5) % ksteps, m = (i >> 5) / ksteps;
     const int r = column(s, ln & 3);
     uint32_t hi[4], lo[4];
@@ -498,10 +503,9 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   [[maybe_unused]] float s_row[kScaled ? 2 * MT : 1];
 #pragma unroll
   for (int i = 0; i < 2 * MT; ++i) {
-    row[i] = first_row + i * 8 + g < count ? rows[first_row + i * 8 + g] : -1;
-    if constexpr (kScaled) s_row[i] = scale / factor[first_row + i * 8 + g];  // a power of two: exact
+    row[i] = i * 8 + g < count ? rows[i * 8 + g] : -1;
+    if constexpr (kScaled) s_row[i] = scale / factor[i * 8 + g];  // a power of two: exact
   }
-  const uint4* mine = frags + 2 * (first_row / 16) * ksteps * 32;
   auto load_y = [&](int blk, uint4 (&v)[2 * MT]) {
     const int col = blk * 32 + c * 8;  // the lane's 8 columns
 #pragma unroll
@@ -525,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   };
   // acc += rows 16 m .. of h, run s, times the four instructions' operands
   auto multiply = [&](int m, int s, const uint2 (&v)[4], float (&acc)[4][4]) {
-    const uint4 hi = mine[2 * ((m * ksteps + s) * 32 + lane)], lo = mine[2 * ((m * ksteps + s) * 32 + lane) + 1];
+    const uint4 hi = frags[2 * ((m * ksteps + s) * 32 + lane)], lo = frags[2 * ((m * ksteps + s) * 32 + lane) + 1];
 #pragma unroll
     for (int j = 0; j < 4; ++j) Half<T>::mma(acc[j], hi, v[j].x, v[j].y);
 #pragma unroll
@@ -558,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
   };
-  const int b0 = rank * per + w;
+  const int b0 = rank * per + warp;
   bool done = false;
   if constexpr (!STAGED) {
     if (R <= 16 || R == 32) {
@@ -567,9 +571,9 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
         uint4 yv[2][2 * MT];
         decltype(sample) bv[2];
         auto trip = [&](int blk, int at) {
-          if (blk + W < b1) {
-            load_y(blk + W, yv[1 - at]);
-            load_b(blk + W, bv[1 - at].v);
+          if (blk + kWarps < b1) {
+            load_y(blk + kWarps, yv[1 - at]);
+            load_b(blk + kWarps, bv[1 - at].v);
           }
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
@@ -584,9 +588,9 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
           load_b(b0, bv[0].v);
         }
 #pragma unroll 1
-        for (int blk = b0; blk < b1; blk += 2 * W) {
+        for (int blk = b0; blk < b1; blk += 2 * kWarps) {
           trip(blk, 0);
-          if (blk + W < b1) trip(blk + W, 1);
+          if (blk + kWarps < b1) trip(blk + kWarps, 1);
         }
       };
       if (R == 32) run([&](int blk, uint4 (&v)[4]) { load_wide(blk, 0, v); }, [&](int m, const uint4 (&v)[4], float (&acc)[4][4]) { multiply_wide(m, 0, v, acc); }, Four<uint4>{});
@@ -595,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
     }
   } else if (R <= 16) {  // a trip or two: nothing to run ahead of
 #pragma unroll 1
-    for (int blk = b0; blk < b1; blk += W) {
+    for (int blk = b0; blk < b1; blk += kWarps) {
       uint4 yv[2 * MT];
       uint2 v[4];
       load_y(blk, yv);
@@ -612,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   }
   if (!done) {
 #pragma unroll 1
-    for (int blk = b0; blk < b1; blk += W) {
+    for (int blk = b0; blk < b1; blk += kWarps) {
       uint4 yv[2 * MT];
       load_y(blk, yv);
       float acc[MT][4][4];
@@ -644,9 +648,9 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
 // ---------------------------------------------------------------- host side
 constexpr int kMaxDevices = 64;
 
-template <typename T, int MT, int RG, bool STAGED>
+template <typename T, int MT, bool STAGED>
 int launch(const Params& p, int64_t items, cudaStream_t stream) {
-  auto kernel = adapters_kernel<T, MT, RG, STAGED>;
+  auto kernel = adapters_kernel<T, MT, STAGED>;
   static std::atomic<bool> configured[kMaxDevices];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -658,7 +662,7 @@ int launch(const Params& p, int64_t items, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(items * p.cluster));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = layout<MT, RG, STAGED>(p.R, p.cluster).total;
+  cfg.dynamicSmemBytes = layout<MT, STAGED>(p.R, p.cluster).total;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -697,15 +701,20 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
     return set_error(TBIK_ERR_ALIGN, "tbik_adapters: pointers must be 16-byte aligned, row strides multiples of 8 elements");
   Params p{x, y, A, B, out, scales, h, order, offsets, T, ldx, ldy, ldo, N, K, R, adapters, leaf, 1, 0};
   p.rest = (expand ? out != y : 1) ? 1 : 0;
-  // Few rows: 16-row tiles.  CTAs per tile: as many as keep the grid near two CTAs per SM; with large ranks enough for the
-  // leaves' sums of 64 rows to fit.
+  // CTAs per tile.  Few rows: as many as keep the grid within three CTAs per SM.  Many rows: no more than one wave of two per SM,
+  // and few, because the eight warps of a CTA that has fewer leaves share a leaf by columns of h and each reads all of x: two
+  // (1500 rows, rank 32, K = 12288, N = 4096: 45 us, with four 58), one where K is long (3000 rows, K = 6 N: 46 us, with two 59),
+  // eight for a wide result (1100 rows, N = 8 K: 23 us, with two 27); with large ranks a warp has that many passes over x to
+  // share.  The leaves' sums have to leave room for the second CTA.
   const bool few = T <= 1024;
-  const int rows = few ? 16 : 64;
+  const int rows = few ? 16 : 32;
   const int64_t items = T / rows + (T < adapters ? T : adapters) + (p.rest ? 1 : 0);
-  while (p.cluster < kLeaves && (items * p.cluster * 2 <= 2 * 148 + 148 || (!few && kLeaves / p.cluster * R > 256))) p.cluster *= 2;
+  const int64_t most = few ? 3 * 148 : 2 * 148;
+  const int cap = few || N >= 4 * K ? kLeaves : std::max(K >= 4 * N ? 1 : 2, R / 32);
+  while (p.cluster < kLeaves && ((p.cluster < cap && items * p.cluster * 2 <= most) || (!few && kLeaves / p.cluster * R > 512))) p.cluster *= 2;
   if (dtype == TBIK_DTYPE_BF16)
-    return few ? launch<__nv_bfloat16, 1, 1, true>(p, items, stream) : launch<__nv_bfloat16, 2, 2, false>(p, items, stream);
-  return few ? launch<__half, 1, 1, true>(p, items, stream) : launch<__half, 2, 2, false>(p, items, stream);
+    return few ? launch<__nv_bfloat16, 1, true>(p, items, stream) : launch<__nv_bfloat16, 2, false>(p, items, stream);
+  return few ? launch<__half, 1, true>(p, items, stream) : launch<__half, 2, false>(p, items, stream);
 }
 
 }  // namespace tbik
