@@ -706,7 +706,9 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
   // (1500 rows, rank 32, K = 12288, N = 4096: 45 us, with four 58), one where K is long (3000 rows, K = 6 N: 46 us, with two 59),
   // eight for a wide result (1100 rows, N = 8 K: 23 us, with two 27); with large ranks a warp has that many passes over x to
   // share.  The leaves' sums have to leave room for the second CTA.
-  const bool few = T <= 1024;
+  // What few rows are: rank 16, K = N = 4096, 1000 rows 17 us staged and 20 straight; rank 32, 400 rows 16 and 20.5, 700 rows 23
+  // and 20.6; rank 64, 700 rows 31 and 29.
+  const bool few = T <= (R <= 16 ? 1024 : 512);
   const int rows = few ? 16 : 32;
   const int64_t items = T / rows + (T < adapters ? T : adapters) + (p.rest ? 1 : 0);
   const int64_t most = few ? 3 * 148 : 2 * 148;
