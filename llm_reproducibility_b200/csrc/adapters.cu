@@ -59,6 +59,11 @@ template <> struct Half<__nv_bfloat16> {
   TBIK_DEVICE static float f32(uint32_t w, int hi) { return __uint_as_float(hi ? (w & 0xFFFF0000u) : (w << 16)); }
   TBIK_DEVICE static uint32_t pack(float lo, float hi) { return Pack16<__nv_bfloat16>::from_f32(lo, hi); }
   TBIK_DEVICE static float round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
+  TBIK_DEVICE static bool any_nan(const uint32_t (&w)[4]) {
+    const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(w);
+    const __nv_bfloat162 top = __hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3]));
+    return !__hbeq2(top, top);
+  }
   TBIK_DEVICE static void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
@@ -71,6 +76,11 @@ template <> struct Half<__half> {
   }
   TBIK_DEVICE static uint32_t pack(float lo, float hi) { return Pack16<__half>::from_f32(lo, hi); }
   TBIK_DEVICE static float round(float v) { return __half2float(__float2half_rn(v)); }
+  TBIK_DEVICE static bool any_nan(const uint32_t (&w)[4]) {
+    const __half2* v = reinterpret_cast<const __half2*>(w);
+    const __half2 top = __hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3]));
+    return !__hbeq2(top, top);
+  }
   TBIK_DEVICE static void mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
@@ -553,8 +563,30 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         o[j] = Half<T>::pack(fmaf(s, acc[j][2 * u], Half<T>::f32(yw[j], 0)), fmaf(s, acc[j][2 * u + 1], Half<T>::f32(yw[j], 1)));
-      *reinterpret_cast<uint4*>(out + row[i] * p.ldo + col) = make_uint4(o[0], o[1], o[2], o[3]);
+      T* dst = out + row[i] * p.ldo + col;
+      if (!Half<T>::any_nan(o)) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+        continue;
+      }
+      // An infinite entry of B against a part of h that is zero, or against parts of either sign, is NaN where their sum
+      // times it is not: such elements are taken again from h itself.  (In place, y is read just before it is written.)
+      const T* yp = y + row[i] * p.ldy + col;
+#pragma unroll 1
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t w = q < 4 ? (q < 2 ? o[0] : o[1]) : (q < 6 ? o[2] : o[3]);
+        float v = Half<T>::f32(w, q & 1);
+        if (v != v) {
+          const float* hr = hs + (i * 8 + g) * R;
+          const T* br = B + static_cast<int64_t>(col + q) * R;
+          float sum = 0.0f;
+#pragma unroll 1
+          for (int r = 0; r < R; ++r) sum = fmaf(hr[r], static_cast<float>(br[r]), sum);
+          v = fmaf(scale, sum, static_cast<float>(yp[q]));
+        }
+        dst[q] = static_cast<T>(v);
+      }
     }
+    __syncwarp();  // (the instructions of the next trip are the warp's)
   };
   auto clear = [](float (&acc)[4][4]) {
 #pragma unroll

@@ -152,6 +152,30 @@ def test_infinities_and_nan_stay_in_their_rows():
         assert torch.equal(got[fine], want[fine]) and not got[9].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["int", "normal"])
+@pytest.mark.parametrize("R", [8, 16, 24, 32, 64])
+@pytest.mark.parametrize("T", [1, 40, 1500])
+def test_an_infinite_entry_of_b_gives_what_the_sum_gives(T, R, kind, dtype):
+    """+-inf where h is not zero there, NaN where it is or where two infinities meet with both signs; nothing else moves."""
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    inf = float("inf")
+    y, x, A, B, ids, s = case(T, 2, R, 64, 72, dtype, kind, none=0.0)
+    x[:, :16] = 0                     # rows 3 and 4 of A see nothing else: h = 0 there
+    A[:, 3:5, 16:] = 0
+    clean = lora_add(y, x, A, B, group_rows(ids, 2), s)
+    B[0, 5, 1], B[0, 6, 3], B[1, 9, 2], B[1, 9, R - 1], B[1, 70, 0] = inf, -inf, -inf, inf, inf
+    groups, (want, _, size) = group_rows(ids, 2), ref(y, x, A, B, ids, s)
+    got = lora_add(y, x, A, B, groups, s)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    assert torch.equal(got[got.isinf()].double(), want[want.isinf()])
+    assert torch.equal(got[want.isfinite()], clean[want.isfinite()])
+    if T > 1:
+        assert want.isnan().any() and want.isinf().any()
+    assert torch.equal(lora_add(y, x, A, B, groups, s, out=y).nan_to_num(0.0, 1.0, -1.0), got.nan_to_num(0.0, 1.0, -1.0))
+
+
 def test_no_adapters_at_all_and_no_rows():
     from llm_reproducibility_b200.tbik.adapters import lora_add, lora_shrink
     from llm_reproducibility_b200.tbik.row_groups import group_rows
