@@ -15,8 +15,11 @@
 // whose warps take a leaf or a part of its columns of h each, operands straight into registers.  Either way a leaf is one
 // chain of instructions over its columns, so a row's bits depend on the row and its adapter alone.
 //
-// h is held in fp32; the second product reads it as the sum of two values of the operand type (16 bits of mantissa for
-// bf16, 22 for fp16, whose rows are scaled by a power of two into its range first).
+// h is held in fp32 and multiplied whole: the second product reads it as the sum of three values of the operand type, each the
+// rounding of what the ones before leave (three times 8 bits for bf16, 11 for fp16, whose rows are scaled by a power of two
+// into its range first), the smallest first.  Two values, 16 bits for bf16, lost the result's last bits where the adapter's
+// terms or y nearly cancel; the third costs what its instructions cost (8192 rows, K = N = 4096: rank 32 51.7 -> 52.8 us, rank 64
+// 80 -> 87, rank 128 137 -> 182).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -35,6 +38,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kLeaves = 8;
+constexpr int kParts = 3;  // values of the operand type that make up one of h
 // One of the two buffers of a staged leaf.  Three CTAs per SM for the usual ranks, whose leaf then comes in one piece (96 rows of 48
 // adapters, rank 16, K = 12288: 24 KiB 18.5 us, 30 KiB 17.4 us, 36 KiB and two CTAs 22.6 us); more columns at a time for the large ones.
 __host__ __device__ constexpr uint32_t stage_bytes(int R) { return R <= 32 ? 30720 : 49152; }
@@ -51,11 +55,14 @@ struct Params {
   int rest;        // rows of no adapter have work to do too (copy y, or zero h)
 };
 
+constexpr float kInf = __builtin_huge_valf();
+
 template <bool B> struct Bool { static constexpr bool value = B; };
 template <typename V> struct Four { V v[4]; };
 
 template <typename T> struct Half;
 template <> struct Half<__nv_bfloat16> {
+  static constexpr float kLargest = 0x1.FEp127f;
   TBIK_DEVICE static float f32(uint32_t w, int hi) { return __uint_as_float(hi ? (w & 0xFFFF0000u) : (w << 16)); }
   TBIK_DEVICE static uint32_t pack(float lo, float hi) { return Pack16<__nv_bfloat16>::from_f32(lo, hi); }
   TBIK_DEVICE static float round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
@@ -70,6 +77,7 @@ template <> struct Half<__nv_bfloat16> {
   }
 };
 template <> struct Half<__half> {
+  static constexpr float kLargest = 65504.0f;
   TBIK_DEVICE static float f32(uint32_t w, int hi) {
     const __half2 v = *reinterpret_cast<const __half2*>(&w);
     return hi ? __high2float(v) : __low2float(v);
@@ -106,7 +114,7 @@ TBIK_DEVICE float4 add(const float4& a, const float4& b) { return make_float4(a.
 TBIK_DEVICE int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // Shared memory: [rows TM][item 4], at 512 [row factors TM] | leaf sums [8 / cluster][TM][R] | h [TM][R] |
-// h as operand [TM / 16][ceil(R / 16)][32 lanes] x 32 bytes | two staging buffers
+// h as operand [TM / 16][ceil(R / 16)][32 lanes] x 48 bytes | two staging buffers
 struct Layout {
   uint32_t sums, h, frags, stage, total;
 };
@@ -117,7 +125,7 @@ __host__ __device__ inline Layout layout(int R, int cluster) {
   l.sums = 1024;
   l.h = l.sums + (kLeaves / cluster) * TM * R * 4;
   l.frags = l.h + TM * R * 4;
-  l.stage = (l.frags + MT * ((R + 15) / 16) * 1024 + 127) / 128 * 128;
+  l.stage = (l.frags + MT * ((R + 15) / 16) * kParts * 512 + 127) / 128 * 128;
   l.total = l.stage + (STAGED ? 2 * stage_bytes(R) : 0);
   return l;
 }
@@ -456,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
     __syncthreads();
   }
 
-  // ---- h as an operand: high and low parts, arranged per lane
+  // ---- h as an operand: its parts, arranged per lane
   constexpr bool kScaled = sizeof(T) == 2 && Pack16<T>::kUmmaFmt == 0;  // fp16
   if constexpr (kScaled) {
     for (int i = warp; i < TM; i += kWarps) {
@@ -466,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
       // the largest of the row to about 2^14; 0 and infinity as they are
       int e = 0;
-      if (top > 0.0f && top < __uint_as_float(0x7F800000u)) e = min(max(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
+      if (top > 0.0f && top < kInf) e = min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 100);
       if (lane == 0) factor[i] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
     }
     __syncthreads();
@@ -480,27 +488,33 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   for (int i = tid; i < MT * ksteps * 32; i += kThreads) {
     const int ln = i & 31, s = (i >> 5) % ksteps, m = (i >> 5) / ksteps;
     const int r = column(s, ln & 3);
-    uint32_t hi[4], lo[4];
+    uint32_t part[kParts][4];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {  // rows ln / 4 and + 8
       const int row = m * 16 + (ln >> 2) + 8 * u;
-      float4 v = r < R ? *reinterpret_cast<const float4*>(hs + row * R + r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const float4 v = r < R ? *reinterpret_cast<const float4*>(hs + row * R + r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float left[4] = {v.x, v.y, v.z, v.w};
       if constexpr (kScaled) {
         const float f = factor[row];
-        v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-      }
-      const float t[4] = {Half<T>::round(v.x), Half<T>::round(v.y), Half<T>::round(v.z), Half<T>::round(v.w)};
-      const float w[4] = {v.x, v.y, v.z, v.w};
-      float d[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) d[j] = fabsf(t[j]) < __uint_as_float(0x7F800000u) ? w[j] - t[j] : 0.0f;  // infinity has no low part
-      hi[u] = Half<T>::pack(t[0], t[1]);
-      hi[u + 2] = Half<T>::pack(t[2], t[3]);
-      lo[u] = Half<T>::pack(d[0], d[1]);
-      lo[u + 2] = Half<T>::pack(d[2], d[3]);
+        for (int j = 0; j < 4; ++j) left[j] *= f;
+      }
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) {
+        float t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          t[j] = Half<T>::round(left[j]);
+          // a number beyond the type's largest starts with that one; infinity and NaN have no further parts
+          if (fabsf(t[j]) == kInf && fabsf(left[j]) < kInf) t[j] = copysignf(Half<T>::kLargest, left[j]);
+          left[j] = fabsf(t[j]) < kInf ? left[j] - t[j] : 0.0f;
+        }
+        part[k][u] = Half<T>::pack(t[0], t[1]);
+        part[k][u + 2] = Half<T>::pack(t[2], t[3]);
+      }
     }
-    frags[2 * i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    frags[2 * i + 1] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) frags[kParts * i + k] = make_uint4(part[k][0], part[k][1], part[k][2], part[k][3]);
   }
   __syncthreads();
 
@@ -539,11 +553,12 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(cons
   };
   // acc += rows 16 m .. of h, run s, times the four instructions' operands
   auto multiply = [&](int m, int s, const uint2 (&v)[4], float (&acc)[4][4]) {
-    const uint4 hi = frags[2 * ((m * ksteps + s) * 32 + lane)], lo = frags[2 * ((m * ksteps + s) * 32 + lane) + 1];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) Half<T>::mma(acc[j], hi, v[j].x, v[j].y);
+    for (int k = kParts - 1; k >= 0; --k) {
+      const uint4 part = frags[kParts * ((m * ksteps + s) * 32 + lane) + k];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) Half<T>::mma(acc[j], lo, v[j].x, v[j].y);
+      for (int j = 0; j < 4; ++j) Half<T>::mma(acc[j], part, v[j].x, v[j].y);
+    }
   };
   auto multiply_wide = [&](int m, int s2, const uint4 (&v)[4], float (&acc)[4][4]) {
     const uint2 lo8[4] = {{v[0].x, v[0].y}, {v[1].x, v[1].y}, {v[2].x, v[2].y}, {v[3].x, v[3].y}};

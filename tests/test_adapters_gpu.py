@@ -139,6 +139,54 @@ def test_values_beyond_the_operand_types_range_in_h():
     assert torch.equal(got, torch.full_like(got, 1 + (R - 3) * 2.0 ** 18 * 2.0 ** -14))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R", [8, 16, 24, 32, 64, 128])
+@pytest.mark.parametrize("T", [1, 40, 1500])
+def test_h_is_multiplied_with_all_its_bits(T, R, dtype):
+    """What is left where y and the adapter's terms cancel: the last bits of h."""
+    from llm_reproducibility_b200.tbik.adapters import lora_expand_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    g, N = torch.Generator(device="cuda").manual_seed(R), 72
+    groups, one = group_rows(torch.zeros(T, dtype=torch.int32, device="cuda"), 1), torch.ones(1, device="cuda")
+    # h against itself without its last five bits, through entries of 1: the sum of the two is those bits, exactly
+    h = torch.randn(T, R, generator=g, device="cuda") + 3.0
+    cut = (h.view(torch.int32) & -32).view(torch.float32)
+    B = torch.zeros(1, N, R, dtype=dtype, device="cuda")
+    for n in range(N):
+        B[0, n, n % R] = B[0, n, (n + 1) % R] = 1.0
+    pair = torch.where(torch.arange(R, device="cuda") % 2 == 0, h, -cut.roll(1, 1))
+    want = torch.stack([pair[:, n % R].double() + pair[:, (n + 1) % R].double() for n in range(N)], 1)
+    got = lora_expand_add(torch.zeros(T, N, dtype=dtype, device="cuda"), pair, B, groups, one)
+    even = torch.arange(N, device="cuda") % R % 2 == 0
+    assert want[:, even].abs().max() < 2.0 ** -16 and want[:, even].abs().max() > 0
+    # (fp16: below its smallest normal number a result is off by half of its smallest step, 2^-25, at most)
+    assert ((got.double() - want)[:, even].abs() <= HALF[dtype] * want[:, even].abs() + 2.0 ** -25 * (dtype == torch.float16)).all()
+    # any entries, y the rounded opposite of the adapter's term: R products of three parts and one sum with y, each addition off by at
+    # most 2^-23 of the magnitudes, then the rounding of the result
+    B, s = (torch.randn(1, N, R, generator=g, device="cuda") * 0.3).to(dtype), torch.tensor([0.75], device="cuda")
+    term, size = 0.75 * (h.double() @ B[0].double().t()), 0.75 * (h.double().abs() @ B[0].double().abs().t())
+    y = (-term).to(dtype)
+    want = y.double() + term
+    tol = HALF[dtype] * want.abs() + ((3 * R + 3) * size + 2 * y.double().abs()) * 2.0 ** -23 + 2.0 ** -25
+    assert ((lora_expand_add(y, h, B, groups, s).double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("R", [8, 32, 64])
+@pytest.mark.parametrize("T", [1, 40, 1500])
+def test_h_beyond_the_operand_types_largest_number(T, R):
+    from llm_reproducibility_b200.tbik.adapters import lora_expand_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    groups, one = group_rows(torch.zeros(T, dtype=torch.int32, device="cuda"), 1), torch.ones(1, device="cuda")
+    # bf16: fp32's largest number, which rounds to bf16's infinity; fp16: 2^120, of either sign, against bits of 2^-14
+    for dtype, big, small in ((torch.bfloat16, torch.finfo(torch.float32).max, 2.0 ** -120), (torch.float16, 2.0 ** 120, 2.0 ** -14)):
+        h, B = torch.zeros(T, R, device="cuda"), torch.zeros(1, 72, R, dtype=dtype, device="cuda")
+        h[:, 1], h[:, 5], B[0, :, 5] = big, -big, small
+        B[0, ::2, 1] = small
+        want = h.double() @ B[0].double().t()
+        got = lora_expand_add(torch.zeros(T, 72, dtype=dtype, device="cuda"), h, B, groups, one)
+        assert torch.equal(got, want.to(dtype)) and (got[:, ::2] == 0).all()
+
+
 def test_infinities_and_nan_stay_in_their_rows():
     from llm_reproducibility_b200.tbik.adapters import lora_add
     from llm_reproducibility_b200.tbik.row_groups import group_rows
