@@ -16,7 +16,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .row_groups import RowGroups, empty, launch, need_cuda, overlap, refuse_grad
+from .row_groups import RowGroups, empty, launch, need_cuda, overlap, overwritten, refuse_grad
 from .tree_based_matmul import _DTYPE_CODE
 
 
@@ -111,7 +111,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     R up to 128; adapters of several ranks are padded with zeros.  Both products are taken in fp32 and the result is
     rounded once.  Returns a new tensor, or `out`, which may be y itself."""
     what = "lora_add"
-    refuse_grad(what, "adapters are a serving operator", y, x, A, B, scales)
+    refuse_grad(what, "adapters are a serving operator", y, x, A, B, scales, out)
     shape_y, shape_x, shape_a, shape_b = y.shape, x.shape, A.shape, B.shape
     if len(shape_y) != 2 or len(shape_x) != 2 or len(shape_a) != 3 or shape_y[0] != shape_x[0] or shape_a[2] != shape_x[1] or \
             shape_b != (shape_a[0], shape_y[1], shape_a[1]):
@@ -128,6 +128,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
         src = y if res is y or (res.data_ptr() == y.data_ptr() and res.stride() == y.stride()) else _rows16(y)
         _launch(dev, _rows16(x), src, res, _weights16(A), _weights16(B), scales.contiguous(), None, groups, T, N, K, R, L,
                 x.dtype, leaf)
+        if out is not None:
+            overwritten(out)
     return res
 
 
@@ -154,7 +156,7 @@ def lora_expand_add(y: torch.Tensor, h: torch.Tensor, B: torch.Tensor, groups: R
     """y + scales[a] * B[a] h, the second half of `lora_add`: h [T, R] float32 as `lora_shrink` (summed over the ranks)
     gives it.  Returns a new tensor, or `out`, which may be y itself."""
     what = "lora_expand_add"
-    refuse_grad(what, "adapters are a serving operator", y, h, B, scales)
+    refuse_grad(what, "adapters are a serving operator", y, h, B, scales, out)
     if y.dim() != 2 or h.dim() != 2 or B.dim() != 3 or y.shape[0] != h.shape[0] or B.shape[1] != y.shape[1] or B.shape[2] != h.shape[1]:
         raise ValueError(f"{what}: y [T, N], h [T, R], B [L, N, R]; got {tuple(y.shape)}, {tuple(h.shape)}, {tuple(B.shape)}")
     _types(what, y, B)
@@ -168,4 +170,6 @@ def lora_expand_add(y: torch.Tensor, h: torch.Tensor, B: torch.Tensor, groups: R
     if T:
         src = y if res is y or (res.data_ptr() == y.data_ptr() and res.stride() == y.stride()) else _rows16(y)
         _launch(dev, None, src, res, None, _weights16(B), scales.contiguous(), _weights16(h), groups, T, N, 8, R, L, y.dtype, 0)
+        if out is not None:
+            overwritten(out)
     return res

@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .row_groups import empty, launch, need_cuda, overlap, refuse_grad
+from .row_groups import empty, launch, need_cuda, overlap, overwritten, refuse_grad
 from .tree_based_matmul import _DTYPE_CODE
 
 
@@ -63,7 +63,7 @@ def grouped_matmul_tp_persistent(A: torch.Tensor, W: torch.Tensor, offsets: torc
     `leaf_for_fp32_nodes(K_total, max_tp)`.  Default: K is one leaf, and may then be any size.
     `out_dtype=torch.float32`: the unrounded sums, what a tensor-parallel rank contributes to the cross-rank levels.
     `tbik.autograd.tree_grouped_linear` is the differentiable form."""
-    refuse_grad("grouped_matmul_tp_persistent", "use tbik.autograd.tree_grouped_linear", A, W)
+    refuse_grad("grouped_matmul_tp_persistent", "use tbik.autograd.tree_grouped_linear", A, W, out)
     return _grouped(A, W, offsets, leaf, out, out_dtype, max_ctas)
 
 
@@ -106,6 +106,8 @@ def _grouped(A, W, offsets, leaf=None, out=None, out_dtype=None, max_ctas=0):
     launch("tbik_grouped_gemm", dev, A.data_ptr(), W.data_ptr(), C.data_ptr(), offsets.data_ptr(), M, N, K, G, A.stride(0), ldw,
            step_w, max(C.stride(0), N), layout, code, _lib.DTYPE_FP32 if c_dtype == torch.float32 else code, leaf or 0, out is None,
            max_ctas)
+    if out is not None:
+        overwritten(out)
     return C
 
 

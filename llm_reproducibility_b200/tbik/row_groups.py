@@ -9,6 +9,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 from .tree_based_matmul import _raw_stream
@@ -63,11 +64,18 @@ def need_cuda(what: str, *tensors: torch.Tensor) -> torch.device:
 
 
 def refuse_grad(what: str, instead: str, *tensors) -> None:
-    """A call that records no gradient must not swallow one."""
+    """A call that records no gradient must not swallow one: of an operand, or of the tensor that it overwrites (which may be
+    None)."""
     if torch.is_grad_enabled():
         for t in tensors:
-            if t.requires_grad:
+            if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} records no gradient: {instead}")
+
+
+def overwritten(out: torch.Tensor) -> None:
+    """Tells autograd that a kernel has written into a caller's tensor, as torch's own operators do: a backward pass that saved
+    what it held before then fails instead of reading what it holds now."""
+    increment_version(out)
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:

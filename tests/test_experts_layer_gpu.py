@@ -132,3 +132,29 @@ def test_adapters_beside_the_shared_projection():
             assert torch.equal(forward(rows, tp), full[rows])
     plain = matmul_tp_persistent(x, W.t(), leaf=leaf)
     assert torch.equal(full[ids < 0], plain[ids < 0]) and not torch.equal(full[ids >= 0], plain[ids >= 0])
+
+
+@pytest.mark.parametrize("what", ["grouped", "lora_add", "lora_expand_add"])
+def test_a_saved_tensor_that_is_overwritten_is_noticed(what):
+    """What autograd saved and a kernel then overwrote must not pass for the gradient."""
+    from llm_reproducibility_b200.tbik.adapters import lora_add, lora_expand_add
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    ones = lambda *s: torch.ones(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    groups, scales = group_rows(torch.zeros(4, dtype=torch.int32, device="cuda"), 1), torch.ones(1, device="cuda")
+    leaf, y = ones(4, 16).requires_grad_(True), ones(4, 16)
+    z = (leaf * y).sum()  # y is saved for leaf's gradient
+    before = y._version
+    if what == "grouped":
+        got = grouped_matmul_tp_persistent(ones(4, 64), ones(1, 16, 64), groups.offsets, out=y)
+    elif what == "lora_add":
+        got = lora_add(y, ones(4, 64), ones(1, 8, 64), ones(1, 16, 8), groups, scales, out=y)
+    else:
+        got = lora_expand_add(y, torch.ones(4, 8, device="cuda"), ones(1, 16, 8), groups, scales, out=y)
+    assert got is y and y._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    with torch.inference_mode():  # tensors without a version
+        y = ones(4, 16)
+        assert lora_expand_add(y, torch.ones(4, 8, device="cuda"), ones(1, 16, 8), groups, scales, out=y) is y
+    assert lora_expand_add(y, torch.ones(4, 8, device="cuda"), ones(1, 16, 8), groups, scales, out=y) is y and (y == 17).all()

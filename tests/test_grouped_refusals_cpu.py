@@ -130,6 +130,24 @@ def test_adapters_refuse():
         leaf_for_adapters(4096, 3)
 
 
+def test_a_result_tensor_that_requires_a_gradient_is_refused():
+    """It would come back with its old graph.  Without recording the call goes on (to the check of the device)."""
+    from llm_reproducibility_b200.tbik.adapters import lora_add, lora_expand_add
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent
+    from llm_reproducibility_b200.tbik.row_groups import RowGroups
+    g = RowGroups(torch.arange(4, dtype=torch.int32), torch.arange(4, dtype=torch.int32), off(0, 2, 4))
+    x, A, B, s = torch.zeros(4, 64, dtype=BF16), torch.zeros(2, 8, 64, dtype=BF16), torch.zeros(2, 16, 8, dtype=BF16), torch.ones(2)
+    leaf = torch.zeros(4, 16, dtype=BF16, requires_grad=True)
+    for out in (leaf, leaf * 2, leaf[:, :]):
+        for call in (lambda: grouped_matmul_tp_persistent(x, torch.zeros(2, 16, 64, dtype=BF16), g.offsets, out=out),
+                     lambda: lora_add(torch.zeros(4, 16, dtype=BF16), x, A, B, g, s, out=out),
+                     lambda: lora_expand_add(torch.zeros(4, 16, dtype=BF16), torch.zeros(4, 8), B, g, s, out=out)):
+            with pytest.raises(RuntimeError, match="records no gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+                call()
+
+
 def test_widths_that_do_not_fit_the_kernels():
     """Broadcast operands may be wider than any memory: a width must not wrap round on its way to the kernel."""
     from llm_reproducibility_b200.tbik.adapters import lora_expand_add, lora_shrink
