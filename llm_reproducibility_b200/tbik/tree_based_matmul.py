@@ -10,6 +10,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 
@@ -164,6 +165,8 @@ def matmul_tp_persistent(A: torch.Tensor, B: torch.Tensor, bias: Optional[torch.
     if A.dtype not in _LEAF:
         raise NotImplementedError(f"matmul_tp_persistent: dtype {A.dtype} is not supported by the sm_100a kernel")
     assert B.dtype == A.dtype
+    if out is not None and out.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("matmul_tp_persistent records no gradient: out must not require one")
     M, K = A.shape
     _, N = B.shape
     node = _node_code(A, node_dtype, out_dtype)
@@ -186,6 +189,8 @@ def matmul_tp_persistent(A: torch.Tensor, B: torch.Tensor, bias: Optional[torch.
             rc = _launch(A, W, C, M, N, K, leaf, dev, max_ctas, node)
     if rc != 0:
         _lib.check(rc, "tbik_gemm_ws")
+    if out is not None:
+        increment_version(out)  # what a backward pass saved of it must not pass for what it holds now
     if bias is not None:
         C += bias
     return C

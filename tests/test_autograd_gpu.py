@@ -47,3 +47,18 @@ def test_input_gradient_is_batch_invariant():
     A2 = A.detach()[:19].clone().requires_grad_(True)
     tree_matmul(A2, W.detach().t()).backward(dC[:19])
     assert torch.equal(bits(A2.grad), bits(full[:19]))
+
+
+def test_a_result_tensor_of_the_dense_product_is_not_overwritten_behind_autograd():
+    from llm_reproducibility_b200.tbik.tree_based_matmul import matmul_tp_persistent
+    A, W = (torch.ones(16, 256, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    leaf, y = torch.ones(16, 16, dtype=torch.bfloat16, device="cuda", requires_grad=True), torch.ones(16, 16, dtype=torch.bfloat16, device="cuda")
+    for out in (leaf, leaf * 2):
+        with pytest.raises(RuntimeError, match="records no gradient"):
+            matmul_tp_persistent(A, W.t(), out=out)
+    with torch.no_grad():
+        assert (matmul_tp_persistent(A, W.t(), out=leaf.clone()) == 256).all()
+    z = (leaf * y).sum()  # y is saved for leaf's gradient
+    assert matmul_tp_persistent(A, W.t(), out=y) is y and (y == 256).all()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
