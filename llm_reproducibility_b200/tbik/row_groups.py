@@ -9,6 +9,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from .. import _lib
@@ -64,12 +65,16 @@ def need_cuda(what: str, *tensors: torch.Tensor) -> torch.device:
 
 
 def refuse_grad(what: str, instead: str, *tensors) -> None:
-    """A call that records no gradient must not swallow one: of an operand, or of the tensor that it overwrites (which may be
-    None)."""
+    """A call that records no gradient must not swallow one, backward or forward: of an operand, or of the tensor that it
+    overwrites (which may be None)."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} records no gradient: {instead}")
+    if forward_ad._current_level >= 0:  # inside a dual level: a tangent says nothing through requires_grad
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} carries no tangent (there is no forward-mode derivative)")
 
 
 def overwritten(out: torch.Tensor) -> None:

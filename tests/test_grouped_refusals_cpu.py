@@ -148,6 +148,34 @@ def test_a_result_tensor_that_requires_a_gradient_is_refused():
                 call()
 
 
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor does not require a gradient; its tangent must not be dropped without a word."""
+    import torch.autograd.forward_ad as fwd
+    from llm_reproducibility_b200.tbik.adapters import lora_add, lora_expand_add, lora_shrink
+    from llm_reproducibility_b200.tbik.autograd import tree_grouped_linear, tree_route_topk
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent, grouped_weight_gradient
+    from llm_reproducibility_b200.tbik.row_groups import RowGroups, route_topk
+    g = RowGroups(torch.arange(4, dtype=torch.int32), torch.arange(4, dtype=torch.int32), off(0, 2, 4))
+    x, A, B, s = torch.zeros(4, 64, dtype=BF16), torch.zeros(2, 8, 64, dtype=BF16), torch.zeros(2, 16, 8, dtype=BF16), torch.ones(2)
+    y, h, W = torch.zeros(4, 16, dtype=BF16), torch.zeros(4, 8), torch.zeros(2, 16, 64, dtype=BF16)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: route_topk(dual(x), 2), lambda: grouped_matmul_tp_persistent(dual(x), W, g.offsets),
+                     lambda: grouped_matmul_tp_persistent(x, dual(W), g.offsets), lambda: grouped_matmul_tp_persistent(x, W, g.offsets, out=dual(y)),
+                     lambda: grouped_weight_gradient(dual(y), x, g.offsets), lambda: lora_add(y, x, A, dual(B), g, s),
+                     lambda: lora_add(y, x, A, B, g, dual(s)), lambda: lora_add(y, x, A, B, g, s, out=dual(y)),
+                     lambda: lora_shrink(dual(x), A, g), lambda: lora_expand_add(y, dual(h), B, g, s)):
+            with pytest.raises(RuntimeError, match="no tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no tangent"):
+                call()
+        for call in (lambda: tree_grouped_linear(dual(x), W, g.offsets), lambda: tree_route_topk(dual(x), 2)):
+            with pytest.raises(RuntimeError):  # (NotImplementedError is one: no jvp)
+                call()
+        with pytest.raises(RuntimeError, match="CUDA"):
+            lora_shrink(x, A, g)
+
+
 def test_widths_that_do_not_fit_the_kernels():
     """Broadcast operands may be wider than any memory: a width must not wrap round on its way to the kernel."""
     from llm_reproducibility_b200.tbik.adapters import lora_expand_add, lora_shrink
