@@ -35,7 +35,7 @@ def leaf_for_adapters(K_total: int, max_tp: int = 8) -> int:
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """Rows of contiguous elements on 16-byte boundaries; anything else is copied once."""
     step, one = t.stride()
-    if one == 1 and step % 8 == 0 and step >= t.shape[1] and t.data_ptr() % 16 == 0:
+    if one == 1 and (t.shape[0] == 1 or (step % 8 == 0 and step >= t.shape[1])) and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -79,15 +79,20 @@ def _check_leaf(what, K: int, leaf: Optional[int]) -> int:
 
 def _check_out(what, y, out, *others):
     """The result's tensor.  It is written while the operands are read: it may be y itself, and else overlaps nothing."""
+    rows, cols = y.shape
     if out is None:
-        return torch.empty_like(y) if y.is_contiguous() else empty(y.shape[0], y.shape[1], y.dtype, y.device)
-    same = out.data_ptr() == y.data_ptr() and out.stride() == y.stride()
-    if any(overlap(out, t) for t in others + (() if same else (y,))):
+        return empty(rows, cols, y.dtype, y.device)
+    if any(overlap(out, t) for t in others + (() if _same(out, y) else (y,))):
         raise ValueError(f"{what}: out overlaps an operand")
-    if out.shape != y.shape or out.dtype != y.dtype or out.device != y.device or out.stride(1) != 1 or out.stride(0) % 8 or \
-            out.data_ptr() % 16 or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
+    if out.shape != y.shape or out.dtype != y.dtype or out.device != y.device or out.stride(1) != 1 or out.data_ptr() % 16 or \
+            (rows > 1 and (out.stride(0) % 8 or out.stride(0) < cols)):
         raise ValueError(f"{what}: out must be like y, with contiguous 16-byte aligned rows")
     return out
+
+
+def _same(out, y) -> bool:
+    """Whether out is y, element for element (the stride between the rows of one row says nothing)."""
+    return out is y or (out.data_ptr() == y.data_ptr() and out.shape == y.shape and out.stride()[y.shape[0] == 1:] == y.stride()[y.shape[0] == 1:])
 
 
 def _launch(dev, x, y, out, A, B, scales, h, groups, T, N, K, R, adapters, dtype, leaf):
@@ -95,9 +100,9 @@ def _launch(dev, x, y, out, A, B, scales, h, groups, T, N, K, R, adapters, dtype
     order, offsets = order.contiguous(), offsets.contiguous()
     px = ldx = pa = py = ldy = po = ldo = pb = ps = 0
     if x is not None:
-        px, ldx, pa = x.data_ptr(), max(x.stride(0), K), A.data_ptr()
+        px, ldx, pa = x.data_ptr(), x.stride(0) if T > 1 else K, A.data_ptr()
     if y is not None:
-        py, ldy, po, ldo = y.data_ptr(), max(y.stride(0), N), out.data_ptr(), max(out.stride(0), N)
+        py, ldy, po, ldo = y.data_ptr(), y.stride(0) if T > 1 else N, out.data_ptr(), out.stride(0) if T > 1 else N
         pb, ps = B.data_ptr(), scales.data_ptr()
     launch("tbik_adapters", dev, px, ldx, py, ldy, po, ldo, pa, pb, ps, 0 if h is None else h.data_ptr(), order.data_ptr(),
            offsets.data_ptr(), T, N, K, R, adapters, _DTYPE_CODE[dtype], leaf)
@@ -125,7 +130,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
     dev = _check(what, T, groups, L, R, (K, N), x, y, A, B, scales)
     res = _check_out(what, y, out, x, A, B)
     if T:
-        src = y if res is y or (res.data_ptr() == y.data_ptr() and res.stride() == y.stride()) else _rows16(y)
+        src = y if _same(res, y) else _rows16(y)
         _launch(dev, _rows16(x), src, res, _weights16(A), _weights16(B), scales.contiguous(), None, groups, T, N, K, R, L,
                 x.dtype, leaf)
         if out is not None:
@@ -168,7 +173,7 @@ def lora_expand_add(y: torch.Tensor, h: torch.Tensor, B: torch.Tensor, groups: R
     dev = _check(what, T, groups, L, R, (N,), y, h, B, scales)
     res = _check_out(what, y, out, h, B)
     if T:
-        src = y if res is y or (res.data_ptr() == y.data_ptr() and res.stride() == y.stride()) else _rows16(y)
+        src = y if _same(res, y) else _rows16(y)
         _launch(dev, None, src, res, None, _weights16(B), scales.contiguous(), _weights16(h), groups, T, N, 8, R, L, y.dtype, 0)
         if out is not None:
             overwritten(out)

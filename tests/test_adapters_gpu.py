@@ -256,6 +256,28 @@ def test_strides_and_neighbours():
     assert torch.equal(lora_add(y, same, A, B, groups, s), ref(y, same, A, B, ids, s)[0].to(torch.bfloat16))
 
 
+def test_one_row_of_a_buffer_with_an_odd_pitch():
+    """The stride between the rows of a single row is never stepped and says nothing: not of x, y, h, nor of out."""
+    from llm_reproducibility_b200.tbik.adapters import lora_add, lora_expand_add, lora_shrink
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    K, N, R = 64, 72, 16
+    for ids in (torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full((1,), -1, dtype=torch.int32, device="cuda")):
+        y, x, A, B, _, s = case(1, 3, R, K, N, torch.bfloat16, "int")
+        groups, (want, h, _) = group_rows(ids, 3), ref(y, x, A, B, ids, s)
+        want = want.to(torch.bfloat16)
+        wide = lambda t, pitch: torch.zeros(4, pitch, dtype=t.dtype, device="cuda")[:1, :t.shape[1]].copy_(t)  # noqa: E731
+        for px, py in ((K + 3, N + 3), (K, N + 1), (K + 5, N + 8)):
+            wx, wy, wh = wide(x, px), wide(y, py), wide(h.float(), R + 3)
+            assert torch.equal(lora_shrink(wx, A, groups).double(), h)
+            for f in (lambda **kw: lora_add(wy, wx, A, B, groups, s, **kw), lambda **kw: lora_expand_add(wy, wh, B, groups, s, **kw)):
+                assert torch.equal(f(), want) and torch.equal(wy, y)
+                buf = torch.full((3, N + 11), 9.0, dtype=torch.bfloat16, device="cuda")
+                assert torch.equal(f(out=buf[:1, :N]), want) and (buf[1:] == 9).all() and (buf[:, N:] == 9).all()
+                again = wy.as_strided((1, N), (N, 1))  # the same row, said otherwise
+                assert torch.equal(f(out=again), want) and torch.equal(wy, want)
+                wy.copy_(y)
+
+
 def test_bad_tables_touch_nothing_outside():
     from llm_reproducibility_b200.tbik.adapters import lora_add
     from llm_reproducibility_b200.tbik.row_groups import RowGroups
