@@ -304,7 +304,8 @@ int tbik_route_topk_backward(const void* logits, int64_t ld, int64_t T, int E, i
  * bits, with the weight chosen by the row's group.
  *   A [M, K] row stride lda; W [G, N, K] with group stride stride_w and, by w_layout, TBIK_W_K_CONTIGUOUS: rows of K
  *   contiguous elements, row stride ldw; TBIK_W_N_CONTIGUOUS: element (n, k) at k * ldw + n (a transposed weight,
- *   what the input gradient multiplies with).  C [M, N] row stride ldc.
+ *   what the input gradient multiplies with).  The groups lie one behind the other or row by row in turn ([N, G, K]
+ *   memory: stride_w = K, ldw = G * K).  C [M, N] row stride ldc.
  *   dtype bf16 or fp16; out_dtype the same, or TBIK_DTYPE_FP32 for the unrounded sums.
  *   leaf: width of the leaves of the reduction tree over K (a multiple of 64 that divides K); 0 = K is one leaf, and K
  *   may then be any positive number.  At most 3 tree levels on 128-column tiles, 15 in all, as with tbik_gemm.

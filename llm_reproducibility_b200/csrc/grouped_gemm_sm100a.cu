@@ -1295,7 +1295,9 @@ int grouped_gemm(const void* A, const void* W, void* C, const int32_t* offsets, 
   if (!A || !W || !C || !offsets) return set_error(TBIK_ERR_ARG, "tbik_grouped_gemm: null pointer");
   const bool kc = w_layout == TBIK_W_K_CONTIGUOUS;
   const int64_t w_row = kc ? K : N, w_rows = kc ? N : K;
-  if (lda < K || ldw < w_row || ldc < N || (groups > 1 && stride_w < (w_rows - 1) * ldw + w_row))
+  // one group behind the other, or their rows in turn ([N, G, K] seen as [G, N, K]): a tensor map steps over either
+  const bool behind = stride_w >= (w_rows - 1) * ldw + w_row, in_turn = stride_w >= w_row && ldw >= (groups - 1) * stride_w + w_row;
+  if (lda < K || ldw < w_row || ldc < N || (groups > 1 && !behind && !in_turn))
     return set_error(TBIK_ERR_SHAPE, "tbik_grouped_gemm: stride smaller than what it steps over");
   if (bad_align(A) || bad_align(W) || lda % 8 || ldw % 8 || stride_w % 8)
     return set_error(TBIK_ERR_ALIGN, "tbik_grouped_gemm: A and W must be 16-byte aligned with strides that are multiples of 8 elements");

@@ -18,7 +18,8 @@ from .tree_based_matmul import _DTYPE_CODE
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """t [.., rows, cols] with contiguous elements in a row, 16-byte aligned rows; anything else is copied once."""
+    """t [.., rows, cols] with contiguous elements in a row, 16-byte aligned rows; of matrices, one behind the other or their
+    rows in turn.  Anything else is copied once."""
     cols = t.shape[-1]
     *steps, last = t.stride()
     # (a stride that is never stepped says nothing, but the kernel's tensor maps read it all the same)
@@ -27,7 +28,11 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
             if s % 8 or s < cols:
                 break
         else:
-            return t
+            if len(steps) == 1:
+                return t
+            outer, inner = steps
+            if outer >= (t.shape[1] - 1) * inner + cols or inner >= (t.shape[0] - 1) * outer + cols or t.shape[0] == 1:
+                return t
     pad = (cols + 7) // 8 * 8
     buf = torch.empty(t.shape[:-1] + (pad,), dtype=t.dtype, device=t.device)
     buf[..., :cols].copy_(t)

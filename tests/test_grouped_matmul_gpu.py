@@ -238,6 +238,30 @@ def test_strided_and_unaligned_operands():
             assert torch.equal(grouped_weight_gradient(D, A, off), wgrad_ref(D, A, off)[0].to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("M,G,K,N", [(200, 3, 64, 48), (9, 4, 520, 264), (3000, 2, 320, 384), (40, 5, 13, 7)])
+def test_weights_whose_groups_lie_row_by_row_in_turn(M, G, K, N):
+    """[N, G, K] and [K, G, N] memory seen as [G, N, K], windows that overlap, forward and backward: the copied weight's bits."""
+    from llm_reproducibility_b200.tbik.autograd import tree_grouped_linear
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent
+    off = offsets_of(ragged(M, G, M)).cuda()
+    A, D = make((M, K), torch.bfloat16, "normal", 1), make((M, N), torch.bfloat16, "normal", 2)
+    nested = make((N, G, K), torch.bfloat16, "normal", 3).permute(1, 0, 2)
+    other = make((K, G, N), torch.bfloat16, "normal", 4).permute(1, 2, 0)
+    step = (K + 7) // 8 * 8
+    window = make((G * (step + 8) + N * step,), torch.bfloat16, "normal", 5).as_strided((G, N, K), (step + 8, step, 1))
+    for W in (nested, other, window):
+        want = grouped_matmul_tp_persistent(A, W.contiguous(), off)
+        check(want, *forward_ref(A, W, off), "normal", K)
+        assert torch.equal(grouped_matmul_tp_persistent(A, W, off), want)
+        x, w, w2 = A.clone().requires_grad_(True), W.detach().requires_grad_(True), W.contiguous().requires_grad_(True)
+        got = torch.autograd.grad(tree_grouped_linear(x, w, off), (x, w), D)
+        for g, v in zip(got, torch.autograd.grad(tree_grouped_linear(x, w2, off), (x, w2), D)):
+            assert torch.equal(g, v)
+    if K % 64 == 0:
+        leaf = K // (K // 64)
+        assert torch.equal(grouped_matmul_tp_persistent(A, nested, off, leaf=leaf), grouped_matmul_tp_persistent(A, nested.contiguous(), off, leaf=leaf))
+
+
 def test_out_with_a_wide_stride_and_neighbours_untouched():
     from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent
     for M, N, wide in ((300, 128, 160), (300, 100, 101), (77, 7, 9), (1, 40, 64)):

@@ -246,3 +246,16 @@ def test_c_abi_refuses_before_any_launch():
     assert lora(_13=1 << 24, _3=1 << 24, _5=1 << 24) == -2 and lora(_14=1 << 24, _1=1 << 24) == -2
     assert lora(_13=20) == -2 and lora(_14=12) == -2 and lora(_15=12) == -2 and lora(_15=136) == -2 and lora(_16=0) == -2 and lora(_18=40) == -2
     assert lora(_1=32) == -2 and lora(_3=16) == -2 and lora(_17=2) == -3 and lora(_2=p + 4) == -4 and lora(_1=65) == -4
+
+
+def test_c_abi_takes_groups_that_lie_row_by_row_in_turn():
+    """[N, G, K] memory passes the strides' check (the next one, of the alignment, is what refuses here); strides at which
+    groups meet do not."""
+    from llm_reproducibility_b200 import _lib
+    L, p = _lib.lib(), 1 << 20
+
+    def gemm(ldw, stride_w, groups=4, N=8, K=128, layout=0):
+        return L.tbik_grouped_gemm(p, p + 8, p, p, 4, N, K, groups, K, ldw, stride_w, N, layout, 0, 0, 0, 0, 0, None)
+
+    assert gemm(128, 1024) == -4 and gemm(512, 128) == -4 and gemm(528, 128) == -4 and gemm(512, 64) == -2 and gemm(504, 128) == -2
+    assert gemm(32, 8, layout=1) == -4 and gemm(24, 8, layout=1) == -2
