@@ -80,7 +80,9 @@ class _TreeGroupedLinear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, offsets = ctx.saved_tensors
-        dx = _grouped(dy, weight.transpose(1, 2), offsets) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:  # (a weight of no columns: sums over nothing)
+            dx = _grouped(dy, weight.transpose(1, 2), offsets) if weight.shape[1] else torch.zeros_like(x)
         dw = _weight_gradient(dy, x, offsets) if ctx.needs_input_grad[1] else None
         return dx, dw, None, None
 

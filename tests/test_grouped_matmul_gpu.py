@@ -262,6 +262,15 @@ def test_weights_whose_groups_lie_row_by_row_in_turn(M, G, K, N):
         assert torch.equal(grouped_matmul_tp_persistent(A, nested, off, leaf=leaf), grouped_matmul_tp_persistent(A, nested.contiguous(), off, leaf=leaf))
 
 
+@pytest.mark.parametrize("M,N", [(5, 0), (0, 7), (0, 0)])
+def test_gradients_of_no_columns_and_of_no_rows(M, N):
+    from llm_reproducibility_b200.tbik.autograd import tree_grouped_linear
+    x, w = (make(s, torch.bfloat16, "int", 1).requires_grad_(True) for s in ((M, 64), (2, N, 64)))
+    y = tree_grouped_linear(x, w, offsets_of([M // 2, M - M // 2]).cuda())
+    dx, dw = torch.autograd.grad(y, (x, w), torch.ones(M, N, dtype=torch.bfloat16, device="cuda"))
+    assert y.shape == (M, N) and torch.equal(dx, torch.zeros_like(x)) and torch.equal(dw, torch.zeros_like(w))
+
+
 def test_out_with_a_wide_stride_and_neighbours_untouched():
     from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent
     for M, N, wide in ((300, 128, 160), (300, 100, 101), (77, 7, 9), (1, 40, 64)):
