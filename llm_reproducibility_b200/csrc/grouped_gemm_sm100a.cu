@@ -198,10 +198,11 @@ struct ForwardCfg {
   static constexpr uint32_t OFF_TABLE = OFF_DEALT + DEALT * 16;
   static constexpr uint32_t smem_bytes(int groups) { return OFF_TABLE + Table::bytes(groups, true) + 1024; }
   static_assert(smem_bytes(TBIK_MAX_GROUPS) <= 232448, "shared memory budget");
-  // tokens per tile of a group of m rows: as few tiles as TN allows, evenly filled
+  // tokens per tile of a group of m rows: as few tiles as TN allows, evenly filled (m may be close to 2^31: m plus the number
+  // of tiles would not fit)
   static TBIK_DEVICE int tokens(int m) {
     const int tiles = (m + TN - 1) / TN;
-    return tiles == 0 ? STEP : (quotient(m + tiles - 1, tiles) + STEP - 1) / STEP * STEP;
+    return tiles == 0 ? STEP : (quotient(m - 1, tiles) + STEP) / STEP * STEP;
   }
 };
 

@@ -489,3 +489,19 @@ def test_refusals_on_the_device():
             f(A, W, off, out=out)
     with pytest.raises(ValueError, match="overlaps"):
         f(A, W, off, out=A)
+
+
+def test_a_group_of_almost_2_31_rows():
+    """Rows and tiles of one group together pass 2^31: the tile's height must not wrap round."""
+    from llm_reproducibility_b200.tbik.grouped_matmul import grouped_matmul_tp_persistent
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    M, K, period = 2 ** 31 - 300, 8, 4096
+    some = make((period, K), torch.bfloat16, "int", 1)
+    A = some.repeat(M // period + 1, 1)[:M]
+    W = make((2, 1, K), torch.bfloat16, "int", 2)
+    C = grouped_matmul_tp_persistent(A, W, torch.tensor([0, 5, M], dtype=torch.int32, device="cuda")).flatten()
+    first, rest = ((some.double() @ W[g, 0].double()).to(torch.bfloat16) for g in range(2))
+    assert torch.equal(C[:5], first[:5]) and torch.equal(C[5:period], rest[5:])
+    whole = M // period * period
+    assert (C[period:whole].view(-1, period) == rest).all() and torch.equal(C[whole:], rest[:M - whole])
