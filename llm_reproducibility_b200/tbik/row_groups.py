@@ -84,14 +84,22 @@ def overwritten(out: torch.Tensor) -> None:
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the spans of memory that two tensors step over meet."""
+    """Whether two tensors may share memory: whether the spans that they step over meet, unless both are columns of one
+    matrix, each its own."""
     def span(t):
         if t.numel() == 0:
             return 0, 0
         steps = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
         return t.data_ptr(), t.data_ptr() + (steps + 1) * t.element_size()
     (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if a0 >= b1 or b0 >= a1:
+        return False
+    if a.dim() == b.dim() == 2 and a.stride() == b.stride() and a.stride(1) == 1 and a.element_size() == b.element_size():
+        pitch = a.stride(0) * a.element_size()
+        if pitch:
+            at = (b0 - a0) % pitch  # b's first byte in a row of the matrix that begins with a's
+            return at < a.shape[1] * a.element_size() or at + b.shape[1] * b.element_size() > pitch
+    return True
 
 
 def _empty_groups(M: int, groups: int, device: torch.device):

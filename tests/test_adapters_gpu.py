@@ -256,6 +256,20 @@ def test_strides_and_neighbours():
     assert torch.equal(lora_add(y, same, A, B, groups, s), ref(y, same, A, B, ids, s)[0].to(torch.bfloat16))
 
 
+def test_x_and_the_result_are_columns_of_one_buffer():
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    T, K, N = 37, 64, 72
+    y, x, A, B, ids, s = case(T, 3, 16, K, N, torch.bfloat16, "int")
+    groups, want = group_rows(ids, 3), ref(y, x, A, B, ids, s)[0].to(torch.bfloat16)
+    for at_x, at_y in ((0, K), (N, 0)):
+        buf = torch.zeros(T, K + N, dtype=torch.bfloat16, device="cuda")
+        vx, vy = buf[:, at_x:at_x + K].copy_(x), buf[:, at_y:at_y + N].copy_(y)
+        assert lora_add(vy, vx, A, B, groups, s, out=vy) is vy and torch.equal(vy, want) and torch.equal(vx, x)
+        with pytest.raises(ValueError, match="overlaps"):
+            lora_add(y, vx, A, B, groups, s, out=buf[:, 8:8 + N])
+
+
 def test_one_row_of_a_buffer_with_an_odd_pitch():
     """The stride between the rows of a single row is never stepped and says nothing: not of x, y, h, nor of out."""
     from llm_reproducibility_b200.tbik.adapters import lora_add, lora_expand_add, lora_shrink

@@ -259,3 +259,24 @@ def test_c_abi_takes_groups_that_lie_row_by_row_in_turn():
 
     assert gemm(128, 1024) == -4 and gemm(512, 128) == -4 and gemm(528, 128) == -4 and gemm(512, 64) == -2 and gemm(504, 128) == -2
     assert gemm(32, 8, layout=1) == -4 and gemm(24, 8, layout=1) == -2
+
+
+def test_overlap_of_tensors():
+    """Against the sets of bytes that two tensors touch: never false where they share one, true where only spans meet but for columns
+    of one matrix."""
+    from llm_reproducibility_b200.tbik.row_groups import overlap
+
+    def touched(t):
+        at = torch.arange(t.untyped_storage().nbytes() // t.element_size()).as_strided(t.shape, t.stride(), t.storage_offset())
+        return {int(i) * t.element_size() + j for i in at.flatten() for j in range(t.element_size())}
+
+    buf = torch.zeros(6, 40, dtype=BF16)
+    flat = buf.view(-1)
+    views = [buf, buf[:, :16], buf[:, 16:32], buf[:, 15:17], buf[2:, 32:], buf[:1], buf[1:2, :8], buf[:3, 8:24], buf[3:, 8:24], buf[:, ::2], buf[:0],
+             buf[:, 5:5], flat[30:].as_strided((4, 20), (40, 1)), flat.as_strided((3, 16), (80, 1)), flat.as_strided((4, 30), (20, 1)), flat[20:60],
+             buf.view(torch.float32)[:, 2:9], buf[1].expand(4, 40), buf.t()]
+    for a in views:
+        for b in views:
+            assert overlap(a, b) or not (touched(a) & touched(b)), (a.shape, a.stride(), b.shape, b.stride())
+    for a, b in ((buf[:, :16], buf[:, 16:32]), (buf[:, 16:32], buf[:, :16]), (buf[:, 8:16], buf[2:, 24:]), (buf[:3], buf[3:]), (buf[:, 0:1], buf[:, 39:])):
+        assert not overlap(a, b)
