@@ -40,7 +40,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kLeaves = 8;
 constexpr int kParts = 3;  // values of the operand type that make up one of h
 // One of the two buffers of a staged leaf.  Three CTAs per SM for the usual ranks, whose leaf then comes in one piece (96 rows of 48
-// adapters, rank 16, K = 12288: 24 KiB 18.5 us, 30 KiB 17.4 us, 36 KiB and two CTAs 22.6 us); more columns at a time for the large ones.
+// adapters, rank 16, K = 12288: 24 KiB 18.5 us, 30 KiB 17.4 us, 36 KiB and two CTAs 22.6 us); more columns at a time for the large
+// ones, of which two CTAs (rank 64) or one (rank 128) are resident.
 __host__ __device__ constexpr uint32_t stage_bytes(int R) { return R <= 32 ? 30720 : 49152; }
 
 struct Params {
@@ -130,8 +131,10 @@ __host__ __device__ inline Layout layout(int R, int cluster) {
   return l;
 }
 
+// Staged: three CTAs per SM are what shared memory leaves room for, and 80 registers (the case above 16.5 us; 64 registers, which would
+// let a fourth in, 17.5 us: more spills).
 template <typename T, int MT, bool STAGED>
-__global__ void __launch_bounds__(kThreads, STAGED ? 4 : 2) adapters_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, STAGED ? 3 : 2) adapters_kernel(const Params p) {
   constexpr int TM = MT * 16;  // rows of the tile
   extern __shared__ __align__(128) uint8_t smem[];
   const Layout lay = layout<MT, STAGED>(p.R, p.cluster);
