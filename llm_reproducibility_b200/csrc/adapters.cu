@@ -751,17 +751,19 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
     return set_error(TBIK_ERR_ALIGN, "tbik_adapters: pointers must be 16-byte aligned, row strides multiples of 8 elements");
   Params p{x, y, A, B, out, scales, h, order, offsets, T, ldx, ldy, ldo, N, K, R, adapters, leaf, 1, 0};
   p.rest = (expand ? out != y : 1) ? 1 : 0;
-  // CTAs per tile.  Few rows: as many as keep the grid within three CTAs per SM.  Many rows: no more than one wave of two per SM,
+  // CTAs per tile.  Few rows: as many as keep the grid within three CTAs per SM.  Above rank 32 fewer are resident and the grid takes
+  // more than one wave, yet fewer CTAs per tile are no faster, each having more leaves in turn (96 rows of 48 adapters, K = N = 4096,
+  // two, four and eight: rank 64 36, 38 and 36 us, rank 128 107, 108 and 87).  Many rows: no more than one wave of two per SM,
   // and few, because the eight warps of a CTA that has fewer leaves share a leaf by columns of h and each reads all of x: two
-  // (1500 rows, rank 32, K = 12288, N = 4096: 45 us, with four 58), one where K is long (3000 rows, K = 6 N: 46 us, with two 59),
-  // eight for a wide result (1100 rows, N = 8 K: 23 us, with two 27); with large ranks a warp has that many passes over x to
+  // (1500 rows, rank 32, K = 12288, N = 4096: 39 us, with four 43), one where K is long (3000 rows, K = 6 N: 46 us, with two 59),
+  // eight for a wide result (1100 rows, N = 8 K: 23 us, with two 28); with large ranks a warp has that many passes over x to
   // share.  The leaves' sums have to leave room for the second CTA.
   // What few rows are: rank 16, K = N = 4096, 1000 rows 17 us staged and 20 straight; rank 32, 400 rows 16 and 20.5, 700 rows 23
   // and 20.6; rank 64, 700 rows 31 and 29.
   const bool few = T <= (R <= 16 ? 1024 : 512);
   const int rows = few ? 16 : 32;
   const int64_t items = T / rows + (T < adapters ? T : adapters) + (p.rest ? 1 : 0);
-  const int64_t most = few ? 3 * 148 : 2 * 148;
+  const int64_t most = (few ? 3 : 2) * sm_count();
   const int cap = few || N >= 4 * K ? kLeaves : std::max(K >= 4 * N ? 1 : 2, R / 32);
   while (p.cluster < kLeaves && ((p.cluster < cap && items * p.cluster * 2 <= most) || (!few && kLeaves / p.cluster * R > 512))) p.cluster *= 2;
   if (dtype == TBIK_DTYPE_BF16)

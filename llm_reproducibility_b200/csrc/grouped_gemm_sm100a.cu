@@ -1167,22 +1167,6 @@ int make_map(CUtensorMap* tm, int dtype, const void* base, int rank, const int64
 
 constexpr int kMaxDevices = 64;
 
-int sms() {
-  static std::atomic<int> cached[kMaxDevices];
-  int dev = 0, n = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= kMaxDevices) dev = 0;
-  n = cached[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
-      (void)cudaGetLastError();
-      n = 148;
-    }
-    cached[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
-
 // `most`: more tiles than that cannot exist
 template <typename Kernel, typename P>
 int launch(Kernel kernel, std::atomic<bool>* configured, size_t smem_max, size_t smem, bool pair, const Maps& maps, const P& p,
@@ -1194,7 +1178,7 @@ int launch(Kernel kernel, std::atomic<bool>* configured, size_t smem_max, size_t
     if (e != cudaSuccess) return set_cuda_error(e, "cudaFuncSetAttribute(grouped product)");
     if (dev >= 0 && dev < kMaxDevices) configured[dev].store(true, std::memory_order_release);
   }
-  int ctas = sms();
+  int ctas = sm_count();
   if (max_ctas > 0 && max_ctas < ctas) ctas = max_ctas;
   int64_t units = pair ? (ctas / 2 > 0 ? ctas / 2 : 1) : ctas;
   if (units > most) units = most > 0 ? most : 1;
@@ -1279,6 +1263,22 @@ int forward(const Shape& c, const Maps& maps, const ForwardParams& p, int64_t mo
 }
 
 }  // namespace
+
+int sm_count() {
+  static std::atomic<int> cached[kMaxDevices];
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices) dev = 0;
+  n = cached[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = 148;
+    }
+    cached[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 
 int grouped_gemm(const void* A, const void* W, void* C, const int32_t* offsets, int64_t M, int N, int K, int groups,
                  int64_t lda, int64_t ldw, int64_t stride_w, int64_t ldc, int w_layout, int dtype, int out_dtype, int leaf,

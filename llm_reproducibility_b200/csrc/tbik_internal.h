@@ -49,6 +49,8 @@ int ar_graph_meta(tbik_ar_t h, void* handles_out, int64_t* offsets_out);
 int ar_register_graph_buffers(tbik_ar_t h, const void* const* handles, const int64_t* const* offsets);
 int ar_status(tbik_ar_t h, uint32_t out[8]);
 
+int sm_count();  // of the current device
+
 size_t group_workspace_bytes(int64_t M, int groups);
 int group_rows(const int32_t* ids, int64_t M, int groups, int32_t* order, int32_t* position, int32_t* offsets, void* workspace,
                size_t workspace_bytes, cudaStream_t stream);
