@@ -757,14 +757,17 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
   // and few, because the eight warps of a CTA that has fewer leaves share a leaf by columns of h and each reads all of x: two
   // (1500 rows, rank 32, K = 12288, N = 4096: 39 us, with four 43), one where K is long (3000 rows, K = 6 N: 46 us, with two 59),
   // eight for a wide result (1100 rows, N = 8 K: 23 us, with two 28); with large ranks a warp has that many passes over x to
-  // share.  The leaves' sums have to leave room for the second CTA.
+  // share.  The first product alone is the case of a long K (600 rows, rank 32, K = 4096: one, two and four CTAs 11.9, 12.4 and
+  // 12.1 us; 4000 rows 13.3, 16.7 and 31.7), the second alone that of a wide result (N = 4096, two, four and eight: 600 rows 13.5, 8.8
+  // and 7.7 us; 2000 rows, where eight are more than a wave, 14.8, 12.8 and 16.7).  The leaves' sums have to leave room for the
+  // second CTA.
   // What few rows are: rank 16, K = N = 4096, 1000 rows 17 us staged and 20 straight; rank 32, 400 rows 16 and 20.5, 700 rows 23
   // and 20.6; rank 64, 700 rows 31 and 29.
   const bool few = T <= (R <= 16 ? 1024 : 512);
   const int rows = few ? 16 : 32;
   const int64_t items = T / rows + (T < adapters ? T : adapters) + (p.rest ? 1 : 0);
   const int64_t most = (few ? 3 : 2) * sm_count();
-  const int cap = few || N >= 4 * K ? kLeaves : std::max(K >= 4 * N ? 1 : 2, R / 32);
+  const int cap = few || !shrink || (expand && N >= 4 * K) ? kLeaves : std::max(!expand || K >= 4 * N ? 1 : 2, R / 32);
   while (p.cluster < kLeaves && ((p.cluster < cap && items * p.cluster * 2 <= most) || (!few && kLeaves / p.cluster * R > 512))) p.cluster *= 2;
   if (dtype == TBIK_DTYPE_BF16)
     return few ? launch<__nv_bfloat16, 1, true>(p, items, stream) : launch<__nv_bfloat16, 2, false>(p, items, stream);

@@ -88,6 +88,29 @@ def test_shrink_and_expand_are_the_two_halves(T, L, R, K, N, dtype):
     assert torch.equal(lora_expand_add(y, h, B, groups, s), lora_add(y, x, A, B, groups, s))
 
 
+@pytest.mark.parametrize("T", [5, 700])
+def test_the_halves_do_not_read_the_width_that_they_have_no_part_in(T):
+    """Through the C ABI, where a caller may pass any: the same bits."""
+    from llm_reproducibility_b200 import _lib
+    from llm_reproducibility_b200.tbik.adapters import lora_expand_add, lora_shrink
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    y, x, A, B, ids, s = case(T, 3, 16, 520, 264, torch.bfloat16, "normal")
+    g = group_rows(ids, 3)
+    stream = torch.cuda.current_stream().cuda_stream
+    want = lora_shrink(x, A, g)
+    for N in (8, 4096, (1 << 24) - 8):
+        h = torch.empty_like(want)
+        assert _lib.lib().tbik_adapters(x.data_ptr(), 520, 0, 0, 0, 0, A.data_ptr(), 0, 0, h.data_ptr(), g.order.data_ptr(),
+                                        g.offsets.data_ptr(), T, N, 520, 16, 3, 0, 0, stream) == 0
+        assert torch.equal(h, want)
+    want = lora_expand_add(y, h, B, g, s)
+    for K in (8, 4096, (1 << 24) - 8):
+        out = torch.empty_like(y)
+        assert _lib.lib().tbik_adapters(0, 0, y.data_ptr(), 264, out.data_ptr(), 264, 0, B.data_ptr(), s.data_ptr(), h.data_ptr(),
+                                        g.order.data_ptr(), g.offsets.data_ptr(), T, 264, K, 16, 3, 0, 0, stream) == 0
+        assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("K,tp", [(4096, 2), (4096, 8), (768, 4), (256, 8)])
 def test_shards_of_k_add_up_to_the_unsharded_bits(K, tp):
     from llm_reproducibility_b200.tbik.adapters import leaf_for_adapters, lora_shrink
