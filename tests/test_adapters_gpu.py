@@ -224,6 +224,23 @@ def test_infinities_and_nan_stay_in_their_rows():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R", [8, 16, 24, 32, 64, 128])
+@pytest.mark.parametrize("K,leaf", [(9224, None), (1000, 1024), (5000, 5024), (12288, 4096)])
+def test_a_leaf_in_several_pieces_has_the_bits_of_a_leaf_in_one(K, leaf, R, dtype):
+    """Few rows bring a leaf to shared memory in pieces whose width goes by the rank and the rows of the tile; many rows walk it."""
+    from llm_reproducibility_b200.tbik.adapters import lora_add, lora_shrink
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    y, x, A, B, ids, s = case(1100, 5, R, K, 72, dtype, "normal", none=0.1)
+    groups = group_rows(ids, 5)
+    full, h = lora_add(y, x, A, B, groups, s, leaf=leaf), lora_shrink(x, A, groups, leaf=leaf)
+    for rows in (slice(0, 1), slice(5, 9), slice(100, 140), slice(400, 900)):
+        part = group_rows(ids[rows], 5)
+        assert torch.equal(lora_shrink(x[rows], A, part, leaf=leaf), h[rows])
+        assert torch.equal(lora_add(y[rows], x[rows], A, B, part, s, leaf=leaf), full[rows])
+    check(full, ref(y, x, A, B, ids, s), "normal")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("kind", ["int", "normal"])
 @pytest.mark.parametrize("R", [8, 16, 24, 32, 64])
 @pytest.mark.parametrize("T", [1, 40, 1500])

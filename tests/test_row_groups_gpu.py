@@ -98,6 +98,68 @@ def test_route_of_masked_rows_infinities_and_nan():
         check_grouping(r.groups, r.ids.flatten(), 4)
 
 
+def hard_rows(E, dtype):
+    """Rows of E scores at which a key can go wrong: masks, infinities, NaN of either sign, zeros of either sign, the type's lowest and
+    smallest numbers, ties."""
+    inf, nan, f = math.inf, math.nan, torch.finfo(dtype)
+    g = torch.Generator().manual_seed(E)
+    normal = torch.randn(E, generator=g)
+    fill = lambda v: torch.full((E,), float(v))  # noqa: E731
+    at = lambda row, v, *places: row.clone().index_fill_(0, torch.tensor([q % E for q in places]), float(v))  # noqa: E731
+    rows = [fill(-inf), at(fill(-inf), 1.0, 1), at(fill(-inf), -3.0, E - 1, 0, 7), torch.tensor([0.0, -0.0]).repeat(E)[:E],
+            torch.tensor([-0.0, 0.0, 0.0]).repeat(E)[:E], at(normal, nan, 1, 3), at(normal, nan, E - 1), fill(nan), at(fill(-inf), nan, 2),
+            -at(normal, nan, 4), fill(f.min), at(fill(f.min), -inf, 0, 5, E - 1), at(fill(-inf), f.min, 3), at(normal, inf, 2), at(normal, inf, 0, E - 1),
+            at(at(normal, inf, 3), -inf, 1), at(at(normal, inf, 1), nan, 2), at(normal, -inf, *range(0, E, 2)), at(normal, f.max, 0, 1),
+            at(normal, f.min, 0, 1), torch.arange(E) * f.smallest_normal * f.eps - 3 * f.smallest_normal * f.eps, fill(f.smallest_normal * f.eps),
+            at(fill(-f.smallest_normal * f.eps), 0.0, 2), (normal * 2).round(), fill(1.0)]
+    return torch.stack(rows).to(dtype)
+
+
+def hard_ref(x, k, renormalize):
+    """Ids by (NaN first, then value, lower index first); weights by the definition, whose NaN are kept."""
+    x = x.double()
+    by_value = torch.sort(torch.where(x.isnan(), 0.0, x), dim=1, descending=True, stable=True).indices
+    nan_first = torch.sort(x.isnan().gather(1, by_value).int(), dim=1, descending=True, stable=True).indices
+    ids = by_value.gather(1, nan_first)[:, :k]
+    top = x.gather(1, ids)
+    over = top if renormalize else x
+    peak = top[:, :1]
+    w = torch.exp(top - peak) / torch.exp(over - peak).sum(1, keepdim=True)
+    return torch.where(peak == -math.inf, torch.zeros_like(w), w), ids
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("E,k", [(9, 3), (8, 8), (128, 8), (127, 5), (300, 8), (1024, 8), (40, 9), (128, 32), (300, 16), (512, 12), (1000, 32)])
+def test_route_of_hard_rows_in_every_form(E, k, renormalize, dtype):
+    from llm_reproducibility_b200.tbik.autograd import tree_route_topk
+    from llm_reproducibility_b200.tbik.row_groups import route_topk
+    x = hard_rows(E, dtype)
+    w, ids = hard_ref(x, k, renormalize)
+    for times in (1, 700):  # one launch, and the form of many tokens
+        r = route_topk(x.cuda().repeat(times, 1), k, renormalize=renormalize)
+        got = r.weights.cpu().double()
+        for part in (slice(0, len(x)), slice(-len(x), None)):
+            assert torch.equal(r.ids[part].cpu().long(), ids)
+            assert torch.equal(got[part].isnan(), w.isnan())
+            # as in test_route; the arguments of exp reach 2^128, whose rounding is of results that are 0
+            assert ((got[part] - w).abs()[~w.isnan()] <= ((4 + 20 + E) * 2.0 ** -23 * w + 1e-38)[~w.isnan()]).all()
+        check_grouping(r.groups, r.ids.flatten(), E)
+    # the gradient: 0 where every expert is masked, and at masked experts; the definition's where the weights are numbers
+    dw = torch.randn(len(x), k, generator=torch.Generator().manual_seed(k))
+    leaf = x.cuda().requires_grad_(True)
+    tree_route_topk(leaf, k, renormalize=renormalize).weights.backward(dw.cuda())
+    p = torch.zeros(x.shape, dtype=torch.float64).scatter(1, ids, w) if renormalize else torch.softmax(x.double(), 1)
+    p = torch.where((x == -math.inf).all(1, keepdim=True), torch.zeros_like(p), p)
+    dp = torch.zeros(x.shape, dtype=torch.float64).scatter(1, ids, dw.double())
+    want = p * (dp - (p * dp).sum(1, keepdim=True))
+    size = p * (dp.abs() + (p * dp.abs()).sum(1, keepdim=True))
+    tol = (64 + 2 * E) * 2.0 ** -23 * size + torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -25
+    fine = ~w.isnan().any(1)
+    assert fine.sum() > 10 and ((leaf.grad.cpu().double() - want).abs() <= tol)[fine].all()
+    assert (leaf.grad.cpu()[fine][(x == -math.inf)[fine]] == 0).all()
+
+
 @pytest.mark.parametrize("T", [3, 700])
 def test_route_reads_strided_and_broadcast_rows(T):
     from llm_reproducibility_b200.tbik.row_groups import route_topk
