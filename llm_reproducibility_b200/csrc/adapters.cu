@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "ptx_sm100a.cuh"
 #include "tbik_internal.h"
@@ -698,31 +699,90 @@ __global__ void __launch_bounds__(kThreads, STAGED ? 3 : 2) adapters_kernel(cons
 // ---------------------------------------------------------------- host side
 constexpr int kMaxDevices = 64;
 
+// A launch of `items` clusters; the kernel may use as much shared memory as there is.
 template <typename T, int MT, bool STAGED>
-int launch(const Params& p, int64_t items, cudaStream_t stream) {
-  auto kernel = adapters_kernel<T, MT, STAGED>;
+int configure(int R, int cluster, int64_t items, cudaStream_t stream, cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr) {
   static std::atomic<bool> configured[kMaxDevices];
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices || !configured[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    const cudaError_t e = cudaFuncSetAttribute(adapters_kernel<T, MT, STAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) return set_cuda_error(e, "cudaFuncSetAttribute(adapters_kernel)");
     if (dev >= 0 && dev < kMaxDevices) configured[dev].store(true, std::memory_order_release);
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * p.cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = layout<MT, STAGED>(p.R, p.cluster).total;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(p.cluster);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  *cfg = cudaLaunchConfig_t{};
+  cfg->gridDim = dim3(static_cast<unsigned>(items * cluster));
+  cfg->blockDim = dim3(kThreads);
+  cfg->dynamicSmemBytes = layout<MT, STAGED>(R, cluster).total;
+  cfg->stream = stream;
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = 1;
+  return TBIK_OK;
+}
+
+template <typename T, int MT, bool STAGED>
+int launch(const Params& p, int64_t items, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  const int rc = configure<T, MT, STAGED>(p.R, p.cluster, items, stream, &cfg, &attr);
+  if (rc != TBIK_OK) return rc;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, adapters_kernel<T, MT, STAGED>, p);
   return e == cudaSuccess ? TBIK_OK : set_cuda_error(e, "adapters_kernel launch");
+}
+
+// Clusters of staged CTAs that the device holds at once, asked once per device, rank and cluster (0: it could not be asked).
+template <typename T>
+int resident(int R, int cluster) {
+  static std::atomic<int> known[kMaxDevices][TBIK_MAX_RANK / 8][2];
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  const bool keep = dev >= 0 && dev < kMaxDevices;
+  if (keep) n = known[dev][R / 8 - 1][cluster == 8].load(std::memory_order_relaxed);
+  if (n > 0) return n - 1;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attr;
+  if (configure<T, 1, true>(R, cluster, 1, nullptr, &cfg, &attr) != TBIK_OK) return 0;
+  if (cudaOccupancyMaxActiveClusters(&n, adapters_kernel<T, 1, true>, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  if (keep) known[dev][R / 8 - 1][cluster == 8].store(n + 1, std::memory_order_relaxed);
+  return n;
+}
+
+template <typename T>
+int choose_and_launch(Params p, cudaStream_t stream) {
+  const bool shrink = p.x != nullptr, expand = p.y != nullptr;
+  const int R = p.R, N = p.N, K = p.K;
+  const int64_t rows = p.T, groups = rows < p.adapters ? rows : p.adapters;
+  // Tiles of 16 rows from shared memory, for few rows that are done in one wave: its chain of latencies once, eight CTAs per tile, or
+  // four up to rank 32.  What rows can be expected to make, drawn from `adapters`: one tile per adapter in use, or every adapter's
+  // last one half full (the grid has room for the most that there can be).  K = N = 4096, staged and straight: 96 rows of 48
+  // adapters, rank 32 18 and 23 us, rank 64 (not one wave) 36 and 31, rank 128 87 and 43; 300 rows of 48, rank 32 19 and 23; 64 rows
+  // of 32 adapters, rank 64 21 and 30; 300 rows of 1000, rank 16 42 and 32.  What few rows are: 8 adapters, rank 16, 1000 rows 17
+  // and 23, 1500 rows 20 and 23 (K = 512: 18 and 14); rank 32, 500 rows 17 and 25.
+  if (rows <= (R <= 16 ? 1024 : 512)) {
+    const double used = p.adapters * -std::expm1(-static_cast<double>(rows) / p.adapters);
+    const int tiles = static_cast<int>(std::max(used, rows / 16.0 + used / 2) + 0.5);
+    for (p.cluster = kLeaves; p.cluster >= (R <= 32 ? 4 : kLeaves); p.cluster /= 2)
+      if (tiles <= resident<T>(R, p.cluster)) return launch<T, 1, true>(p, rows / 16 + groups + p.rest, stream);
+  }
+  // Tiles of 32 rows, straight.  No more CTAs than one wave of two per SM, and few per tile, because the eight warps of a CTA that has
+  // fewer leaves share a leaf by columns of h and each reads all of x: two (1500 rows, rank 32, K = 12288, N = 4096: 39 us, with four
+  // 43), one where K is long (3000 rows, K = 6 N: 46 us, with two 59), eight for a wide result (1100 rows, N = 8 K: 23 us, with two 28);
+  // with large ranks a warp has that many passes over x to share.  The first product alone is the case of a long K (600 rows, rank
+  // 32, K = 4096: one, two and four CTAs 11.9, 12.4 and 12.1 us; 4000 rows 13.3, 16.7 and 31.7), the second alone that of a wide
+  // result (N = 4096, two, four and eight: 600 rows 13.5, 8.8 and 7.7 us; 2000 rows, where eight are more than a wave, 14.8, 12.8 and
+  // 16.7).  The leaves' sums have to leave room for the second CTA.
+  const int64_t items = rows / 32 + groups + p.rest, most = 2 * sm_count();
+  const int cap = !shrink || (expand && N >= 4 * K) ? kLeaves : std::max(!expand || K >= 4 * N ? 1 : 2, R / 32);
+  p.cluster = 1;
+  while (p.cluster < kLeaves && ((p.cluster < cap && items * p.cluster * 2 <= most) || kLeaves / p.cluster * R > 512)) p.cluster *= 2;
+  return launch<T, 2, false>(p, items, stream);
 }
 
 bool bad_align(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
@@ -751,27 +811,7 @@ int adapters(const void* x, int64_t ldx, const void* y, int64_t ldy, void* out, 
     return set_error(TBIK_ERR_ALIGN, "tbik_adapters: pointers must be 16-byte aligned, row strides multiples of 8 elements");
   Params p{x, y, A, B, out, scales, h, order, offsets, T, ldx, ldy, ldo, N, K, R, adapters, leaf, 1, 0};
   p.rest = (expand ? out != y : 1) ? 1 : 0;
-  // CTAs per tile.  Few rows: as many as keep the grid within three CTAs per SM.  Above rank 32 fewer are resident and the grid takes
-  // more than one wave, yet fewer CTAs per tile are no faster, each having more leaves in turn (96 rows of 48 adapters, K = N = 4096,
-  // two, four and eight: rank 64 36, 38 and 36 us, rank 128 107, 108 and 87).  Many rows: no more than one wave of two per SM,
-  // and few, because the eight warps of a CTA that has fewer leaves share a leaf by columns of h and each reads all of x: two
-  // (1500 rows, rank 32, K = 12288, N = 4096: 39 us, with four 43), one where K is long (3000 rows, K = 6 N: 46 us, with two 59),
-  // eight for a wide result (1100 rows, N = 8 K: 23 us, with two 28); with large ranks a warp has that many passes over x to
-  // share.  The first product alone is the case of a long K (600 rows, rank 32, K = 4096: one, two and four CTAs 11.9, 12.4 and
-  // 12.1 us; 4000 rows 13.3, 16.7 and 31.7), the second alone that of a wide result (N = 4096, two, four and eight: 600 rows 13.5, 8.8
-  // and 7.7 us; 2000 rows, where eight are more than a wave, 14.8, 12.8 and 16.7).  The leaves' sums have to leave room for the
-  // second CTA.
-  // What few rows are: rank 16, K = N = 4096, 1000 rows 17 us staged and 20 straight; rank 32, 400 rows 16 and 20.5, 700 rows 23
-  // and 20.6; rank 64, 700 rows 31 and 29.
-  const bool few = T <= (R <= 16 ? 1024 : 512);
-  const int rows = few ? 16 : 32;
-  const int64_t items = T / rows + (T < adapters ? T : adapters) + (p.rest ? 1 : 0);
-  const int64_t most = (few ? 3 : 2) * sm_count();
-  const int cap = few || !shrink || (expand && N >= 4 * K) ? kLeaves : std::max(!expand || K >= 4 * N ? 1 : 2, R / 32);
-  while (p.cluster < kLeaves && ((p.cluster < cap && items * p.cluster * 2 <= most) || (!few && kLeaves / p.cluster * R > 512))) p.cluster *= 2;
-  if (dtype == TBIK_DTYPE_BF16)
-    return few ? launch<__nv_bfloat16, 1, true>(p, items, stream) : launch<__nv_bfloat16, 2, false>(p, items, stream);
-  return few ? launch<__half, 1, true>(p, items, stream) : launch<__half, 2, false>(p, items, stream);
+  return dtype == TBIK_DTYPE_BF16 ? choose_and_launch<__nv_bfloat16>(p, stream) : choose_and_launch<__half>(p, stream);
 }
 
 }  // namespace tbik

@@ -148,6 +148,19 @@ def test_a_row_has_the_same_bits_in_every_batch(R, dtype):
         assert torch.equal(part, full[rows])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,L,R", [(96, 48, 32), (96, 48, 64), (96, 48, 128), (64, 1000, 64), (256, 1000, 16), (500, 1000, 32), (1000, 48, 16), (300, 4, 128)])
+def test_few_rows_of_many_adapters_and_of_large_ranks(T, L, R, dtype):
+    """Batches on either side of where tiles come through shared memory: the definition's values, and each row's bits alone."""
+    from llm_reproducibility_b200.tbik.adapters import lora_add
+    from llm_reproducibility_b200.tbik.row_groups import group_rows
+    y, x, A, B, ids, s = case(T, L, R, 1032, 264, dtype, "normal")
+    full = lora_add(y, x, A, B, group_rows(ids, L), s)
+    check(full, ref(y, x, A, B, ids, s), "normal")
+    for t in (0, T // 3, T - 1):
+        assert torch.equal(lora_add(y[t:t + 1], x[t:t + 1], A, B, group_rows(ids[t:t + 1], L), s), full[t:t + 1])
+
+
 def test_values_beyond_the_operand_types_range_in_h():
     """h is held in 32 bits: it may pass fp16's largest number."""
     from llm_reproducibility_b200.tbik.adapters import lora_add
