@@ -3,11 +3,12 @@
 //   h[t]   = A_a x[t]                       fp32, K cut into at most 8 leaves, ((0+1)+(2+3))+((4+5)+(6+7))
 //   out[t] = round(y[t] + s_a B_a h[t])     fp32, a = adapter of row t
 //
-// Both products are skinny (R = 8 .. 128), so what has to move is x, y, out and the adapters in use: memory bound, and
-// mma.sync m16n8k16 keeps up with it while its operands come straight from global memory -- no tensor-memory round trip
-// for 16 columns.  The k index of an instruction may be permuted as long as both operands agree: a lane takes 8
-// neighbouring elements of its row as its share of two instructions, which makes every operand load 16 bytes wide; in the
-// second product the columns are permuted the same way, so that a lane ends up with 8 neighbouring results.
+// Both products are skinny (R = 8 .. 128), so what has to move is x, y, out and the adapters in use, and mma.sync m16n8k16 takes its
+// operands straight from global memory -- no tensor-memory round trip for 16 columns (8192 rows, rank 32, K = N = 4096: 52 us, HBM
+// 41 % busy, tensor pipe 37 %, issue slots 34 %: the loads that 14 warps per SM have in flight are the limit; rank 128: 180 us, tensor
+// pipe 41 %).  The k index of an instruction may be permuted as long as both operands agree: a lane takes 8 neighbouring elements
+// of its row as its share of two instructions, which makes every operand load 16 bytes wide; in the second product the columns are
+// permuted the same way, so that a lane ends up with 8 neighbouring results.
 //
 // One cluster of 1 .. 8 CTAs per (adapter, tile of rows), both products in one launch.  The CTAs split K by leaves, add
 // the leaves through distributed shared memory, and split N for the second product.  Few rows: 16-row tiles and
