@@ -71,7 +71,7 @@ def refuse_grad(what: str, instead: str, *tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} records no gradient: {instead}")
-    if forward_ad._current_level >= 0:  # inside a dual level: a tangent says nothing through requires_grad
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # inside a dual level: a tangent says nothing through requires_grad
         for t in tensors:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise RuntimeError(f"{what} carries no tangent (there is no forward-mode derivative)")

@@ -505,3 +505,5 @@ def test_a_group_of_almost_2_31_rows():
     assert torch.equal(C[:5], first[:5]) and torch.equal(C[5:period], rest[5:])
     whole = M // period * period
     assert (C[period:whole].view(-1, period) == rest).all() and torch.equal(C[whole:], rest[:M - whole])
+    del A, C
+    torch.cuda.empty_cache()
